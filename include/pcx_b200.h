@@ -572,6 +572,31 @@ int pcx_colplan_jobs(const void* planner, const uint8_t* dense, void** blob, cha
 int pcx_colplan_blob(const void* blob, const int32_t** data, int64_t* n_data, const int64_t** meta, int64_t* n_meta);
 int pcx_colplan_blob_free(void* blob);
 
+/* ---- Language-model operators: selection over a vocabulary ----------------------------------------------------------
+ * dtype: 0 fp32, 1 bf16, 2 fp16.  n (entries of an answer) is at most 128.  `scratch`: pcx_vocab_scratch_bytes(rows, splits,
+ * n) bytes, 16-byte aligned, used by one call at a time; `splits`: CTAs per row (pcx_vocab_splits gives a good number).
+ * Rows may start at any multiple of the element size; the elements of a row are adjacent.  [No counterpart in the
+ * reference.] */
+int pcx_vocab_splits(int64_t rows, int64_t vocab);
+int64_t pcx_vocab_scratch_bytes(int64_t rows, int splits, int n);
+/* The n largest logits of every row (largest first, a lower id first among equals; -inf and NaN are none: id -1, value
+ * -inf) and norms[r] = log sum_v exp(logits[r][v] / temperature). */
+int pcx_top_logits(int64_t* ids, void* values, float* norms, void* scratch, const void* logits, int dtype, int64_t rows,
+                   int vocab, int64_t row_stride, int n, int splits, double temperature, void* stream);
+/* The n best of scores[b][k] + logits[b][k][v] - (normalize ? log sum_v exp(logits[b][k][v]) : 0) over k and v, compared in 64
+ * bits, a lower k * vocab + v first among equals.  Beams whose score is -inf or NaN are dead; a beam flagged in `finished`
+ * (null = none) has one candidate, pad_id at its own score.  Missing entries: score -inf, parent 0, token -1.
+ * beams <= 128, beams * vocab < 2^31. */
+int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* scratch, const void* logits, int dtype,
+                    const float* scores, const uint8_t* finished, int64_t batch, int beams, int vocab, int64_t stride_batch,
+                    int64_t stride_beam, int n, int pad_id, int normalize, int splits, void* stream);
+/* dst[o, b * n + j, :] = src[o, b * beams + parents[b][j], :] for up to 8 tensors at once; zeros for a parent outside
+ * [0, beams).  `states` (HOST memory): per tensor source, destination, outer rows, bytes per beam, strides in bytes of outer
+ * rows and of beams in the source; all of them multiples of `unit` (1, 2, 4, 8 or 16).  parents: int32, or int64 if
+ * wide_ids. */
+int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int wide_ids, int64_t batch, int beams, int n,
+                int unit, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,7 +11,7 @@ import contextlib
 import ctypes
 import os
 import threading
-from ctypes import c_float, c_int, c_int64, c_void_p
+from ctypes import c_double, c_float, c_int, c_int64, c_void_p
 from typing import Optional
 
 import torch
@@ -20,7 +20,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # PCX_B200_LIB points at another build of the library (e.g. one with development switches compiled in)
 LIB_PATH = os.environ.get("PCX_B200_LIB") or os.path.join(_HERE, "csrc", "libpcx_b200.so")
 
-P, I, L, F = c_void_p, c_int, c_int64, c_float
+P, I, L, F, D = c_void_p, c_int, c_int64, c_float, c_double
 
 # name -> argument types, in the order of include/pcx_b200.h (the trailing stream is appended below)
 SIGNATURES = {
@@ -78,12 +78,16 @@ SIGNATURES = {
     "pcx_sum_bwd_ele_dense2": [P, P, P, P, P, P, P, P, I, I, P, P, I, P, L, L, I, I, I, I, I],
     "pcx_sum_par_dense2_stage": [P, P, P, P, P, P, P, P, I, L, I, I, I, I, I, I, I],
     "pcx_sum_par_dense2_gemm": [P, P, P, P, P, P, P, L, I, I, I],
+    "pcx_top_logits": [P, P, P, P, P, I, L, I, L, I, I, D],
+    "pcx_beam_select": [P, P, P, P, P, I, P, P, L, I, I, L, L, I, I, I, I],
+    "pcx_reorder": [P, I, P, I, L, I, I, I],
 }
 
 # entry points without a stream argument
 PLAIN = {"pcx_build_arch": [], "pcx_column_clusters": [I, I], "pcx_column_chain_clusters": [I], "pcx_column_chain_bytes": [I, I, I, I], "pcx_set_sum_mode": [I], "pcx_set_dependent_launch": [I], "pcx_set_stage_event": [P], "pcx_get_status": [], "pcx_clear_status": [],
          "pcx_packed_tile_count": [L, I, I, I, I], "pcx_dense_scratch_bytes": [I, I, I],
-         "pcx_sm_packed_bytes": [L, I, I], "pcx_dense2_scratch_bytes": [I, I, I]}
+         "pcx_sm_packed_bytes": [L, I, I], "pcx_dense2_scratch_bytes": [I, I, I],
+         "pcx_vocab_splits": [L, L], "pcx_vocab_scratch_bytes": [L, I, I]}
 # the planner of the column program (host only; the last two arguments of those that may refuse: a text buffer and its size)
 PLAIN.update({"pcx_colplan_new": [P, L, P, L, P, P, I], "pcx_colplan_free": [P], "pcx_colplan_info": [P, P, P, P],
               "pcx_colplan_suits": [P, L, P], "pcx_colplan_cut": [P, L, P, L, L, P, P, I], "pcx_colplan_tied": [P, P, P, I],
@@ -148,7 +152,8 @@ def load() -> ctypes.CDLL:
     for name, args in PLAIN.items():
         fn = getattr(lib, name)
         fn.restype = c_int64 if name in ("pcx_packed_tile_count", "pcx_dense_scratch_bytes", "pcx_sm_packed_bytes",
-                                        "pcx_dense2_scratch_bytes", "pcx_column_chain_bytes") else c_int
+                                        "pcx_dense2_scratch_bytes", "pcx_column_chain_bytes",
+                                        "pcx_vocab_scratch_bytes") else c_int
         fn.argtypes = list(args)
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)

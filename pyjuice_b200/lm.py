@@ -1,0 +1,200 @@
+"""Operators of language-model circuits: learning from a teacher's top logits, and answering with beams.
+
+``top_logits`` takes the largest logits of a teacher's vocabulary rows, ``expected_log_probs`` scores tables of leaf
+log-probabilities against them (and is what a compiled circuit computes at its leaves when it is called with a
+:class:`TopLogits` instead of categories), ``beam_select`` picks the best continuations over beams and vocabulary and
+``reorder`` moves the states of the beams along.  Everything runs in the CUDA library on torch's current stream of the
+tensors' device; nothing synchronises, and every call can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import List, NamedTuple, Optional, Tuple
+
+import torch
+
+from . import _lib
+
+MAX_TOP = 128                  # entries of one selection
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class TopLogits(NamedTuple):
+    """What is kept of a teacher's distributions: the ids of a few categories per position and their logits.
+
+    ``ids`` and ``logits`` have the same shape, slots last (for a circuit ``[B, num_vars, K]``); ids are int32 or int64,
+    logits float32, bfloat16 or float16.  A slot is empty when its id is negative or its logit is -inf or NaN.  The weight
+    of a slot is ``exp(logits / temperature - log_norm)``; without ``log_norm`` (the shape of ``ids`` less its last
+    dimension), or where it is not finite, the weights of a position's slots sum to one.  A position whose slots are all
+    empty says nothing: it is marginalised.  Logits of +inf share the whole weight of their position."""
+    ids: torch.Tensor
+    logits: torch.Tensor
+    temperature: float = 1.0
+    log_norm: Optional[torch.Tensor] = None
+
+    def _check(self):
+        if self.ids.dtype not in (torch.int32, torch.int64):
+            raise TypeError("ids must be int32 or int64")
+        if self.logits.dtype not in _TYPES:
+            raise TypeError("logits must be float32, bfloat16 or float16")
+        if self.ids.shape != self.logits.shape or self.ids.dim() < 1:
+            raise ValueError(f"ids {tuple(self.ids.shape)} and logits {tuple(self.logits.shape)} must have the same shape")
+        if not 0.0 < self.temperature < float("inf"):
+            raise ValueError("`temperature` should be positive")
+        if self.log_norm is not None and (self.log_norm.shape != self.ids.shape[:-1] or self.log_norm.dtype != torch.float32):
+            raise ValueError("`log_norm` must be float32 with one value per position")
+
+
+def _require_cuda(*tensors):
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and not t.is_cuda:
+            raise NotImplementedError("language-model operators run on CUDA only (no CPU path)")
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors on {device} and {t.device}")
+
+
+def _scratch(rows: int, vocab: int, n: int, device) -> Tuple[torch.Tensor, int]:
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        splits = lib.pcx_vocab_splits(rows, vocab)
+    return torch.empty(lib.pcx_vocab_scratch_bytes(rows, splits, n), dtype=torch.uint8, device=device), splits
+
+
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The ``k`` largest logits of every row of ``logits`` ``[..., V]``, largest first, a lower id first among equals, and
+    the rows' log-normalisers ``log sum_v exp(logits[v] / temperature)``.
+
+    Returns a :class:`TopLogits` of ids (int64) and logits (in the type of the input) ``[..., k]`` and ``log_norm``
+    ``[...]`` (float32).  Logits of -inf and NaN are no candidates and count nothing; a slot without a candidate has the id
+    -1 and the logit -inf.  No gradient passes.  ``k`` is at most 128."""
+    if logits.dtype not in _TYPES:
+        raise TypeError("logits must be float32, bfloat16 or float16")
+    if logits.dim() < 1 or not 1 <= logits.size(-1) < 2 ** 30:
+        raise ValueError("logits need a vocabulary in their last dimension")
+    V, lead = logits.size(-1), logits.shape[:-1]
+    if not 1 <= k <= min(MAX_TOP, V):
+        raise ValueError(f"`k` should be in [1, {min(MAX_TOP, V)}], got {k}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError("`temperature` should be positive")
+    _require_cuda(logits)
+    x = logits.detach()
+    if x.dim() != 2 or x.stride(1) != 1:
+        x = x.reshape(-1, V)
+        x = x if x.stride(1) == 1 or V == 1 else x.contiguous()
+    rows, device = x.size(0), x.device
+    ids = torch.empty((*lead, k), dtype=torch.int64, device=device)
+    values = torch.empty((*lead, k), dtype=x.dtype, device=device)
+    norms = torch.empty(lead, dtype=torch.float32, device=device)
+    if rows > 0:
+        scratch, splits = _scratch(rows, V, k, device)
+        _lib.call("pcx_top_logits", ids, values, norms, scratch, x, _TYPES[x.dtype], rows, V, x.stride(0), k, splits,
+                  float(temperature))
+    return TopLogits(ids, values, temperature, norms)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[int] = None,
+                finished: Optional[torch.Tensor] = None, pad_id: int = 0, normalize: bool = True):
+    """The ``num_out`` best continuations of every sequence's beams.
+
+    ``logits`` ``[B, K, V]`` over the vocabulary, ``scores`` ``[B, K]`` (float32) of the beams so far.  Continuing beam k
+    with token v scores ``scores[k] + logits[k, v] - logsumexp(logits[k])`` (``normalize=False``: the logits are
+    log-probabilities already and are added as they are).  Sums are compared in 64 bits, larger first, a lower
+    ``k * V + v`` first among equals.  A beam whose score is -inf or NaN is dead; logits of -inf or NaN are no
+    continuations, and a row that holds +inf has none under ``normalize``.  A beam marked in ``finished`` (bool ``[B, K]``)
+    has one continuation, ``pad_id`` at its own score.
+
+    Returns scores (float32), parent beams and tokens (int64), each ``[B, num_out]``, best first; where there are fewer
+    continuations the rest has the score -inf, parent 0 and token -1.  ``num_out`` defaults to K and is at most 128.  Not
+    differentiable."""
+    if logits.dtype not in _TYPES:
+        raise TypeError("logits must be float32, bfloat16 or float16")
+    if logits.dim() != 3:
+        raise ValueError("logits must be [B, K, V]")
+    B, K, V = logits.shape
+    if scores.shape != (B, K) or scores.dtype != torch.float32:
+        raise ValueError("scores must be float32 [B, K]")
+    if finished is not None and (finished.shape != (B, K) or finished.dtype != torch.bool):
+        raise ValueError("`finished` must be bool [B, K]")
+    if not 1 <= K <= MAX_TOP or V < 1 or K * V >= 2 ** 31:
+        raise ValueError(f"1 to {MAX_TOP} beams over a vocabulary with K * V < 2^31 are supported")
+    n = K if num_out is None else int(num_out)
+    if not 1 <= n <= min(MAX_TOP, K * V):
+        raise ValueError(f"`num_out` should be in [1, {min(MAX_TOP, K * V)}], got {n}")
+    if not 0 <= pad_id < V:
+        raise ValueError("`pad_id` is not in the vocabulary")
+    _require_cuda(logits, scores, finished)
+    x = logits.detach()
+    x = x if x.stride(2) == 1 or V == 1 else x.contiguous()
+    scores = scores.detach().contiguous()
+    finished = None if finished is None else finished.contiguous()
+    device = x.device
+    out = torch.empty(B, n, dtype=torch.float32, device=device)
+    parents, tokens = torch.empty(2, B, n, dtype=torch.int64, device=device)
+    if B > 0:
+        scratch, splits = _scratch(B * K, V, n, device)
+        _lib.call("pcx_beam_select", out, parents, tokens, scratch, x, _TYPES[x.dtype], scores, finished, B, K, V,
+                  x.stride(0), x.stride(1), n, pad_id, int(bool(normalize)), splits)
+    return out, parents, tokens
+
+
+def _beam_rows(x: torch.Tensor, dim: int):
+    """(tensor, outer rows, bytes per beam, strides in bytes of outer rows and beams) of a state as the kernel walks it: a
+    copy where the dimensions before or after the beams are not laid out as one."""
+    size, stride, es = x.shape, x.stride(), x.element_size()
+    inner = 1
+    for d in range(x.dim() - 1, dim, -1):
+        if size[d] != 1 and stride[d] != inner:
+            return _beam_rows(x.contiguous(), dim)
+        inner *= size[d]
+    outer, step = 1, 0
+    for d in range(dim - 1, -1, -1):
+        if size[d] != 1:
+            if outer == 1:
+                step = stride[d]
+            elif stride[d] != step * outer:
+                return _beam_rows(x.contiguous(), dim)
+            outer *= size[d]
+    return x, outer, inner * es, step * es, stride[dim] * es
+
+
+def reorder(parents: torch.Tensor, *states: torch.Tensor, dim: int = 0) -> List[torch.Tensor]:
+    """The states of the beams that were continued: ``parents`` ``[B, n]`` (int32 or int64) names, for every new beam of a
+    sequence, the old beam it continues; every state has B * K beams in dimension ``dim``, those of a sequence together.
+
+    Returns the new states, contiguous, with B * n beams in that dimension.  A parent outside [0, K) gives zeros.  States
+    may have any real type, other shapes than each other, and any strides; they are not differentiable."""
+    if parents.dim() != 2 or parents.dtype not in (torch.int32, torch.int64):
+        raise ValueError("`parents` must be int32 or int64 [B, n]")
+    B, n = parents.shape
+    moved, beams = [], None
+    for x in states:
+        if x.dim() < 1 or not -x.dim() <= dim < x.dim():
+            raise ValueError(f"a state of shape {tuple(x.shape)} has no dimension {dim}")
+        at = dim % x.dim()
+        if x.is_complex():
+            raise TypeError("states must be real")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("`reorder` is not differentiable: call it under torch.no_grad()")
+        if B > 0 and (x.size(at) % B != 0 or x.size(at) == 0 or (beams is not None and x.size(at) != B * beams)):
+            raise ValueError(f"a state with {x.size(at)} beams does not fit {B} sequences" +
+                             (f" of {beams}" if beams is not None else ""))
+        beams = x.size(at) // B if B > 0 else 1
+        moved.append((x, at))
+    _require_cuda(parents, *states)
+    parents = parents.contiguous()
+    out, by_unit = [], {}
+    for x, at in moved:
+        x, outer, nbytes, outer_step, beam_step = _beam_rows(x, at)
+        y = torch.empty((*x.shape[:at], B * n, *x.shape[at + 1:]), dtype=x.dtype, device=x.device)
+        out.append(y)
+        if y.numel() == 0:
+            continue
+        bits = x.data_ptr() | nbytes | outer_step | beam_step | 16
+        by_unit.setdefault(bits & -bits, []).append((x, (x.data_ptr(), y.data_ptr(), outer, nbytes, outer_step, beam_step)))
+    for unit, group in by_unit.items():
+        for i in range(0, len(group), 8):
+            part = [v for _, row in group[i:i + 8] for v in row]
+            _lib.call("pcx_reorder", (ctypes.c_int64 * len(part))(*part), len(part) // 6, parents,
+                      int(parents.dtype == torch.int64), B, beams, n, unit)
+    return out
