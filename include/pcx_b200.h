@@ -597,6 +597,53 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
 int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int wide_ids, int64_t batch, int beams, int n,
                 int unit, void* stream);
 
+/* ---- Language-model operators: leaf tables under a teacher's top logits ---------------------------------------------
+ * entries[v][b][k] = (category or -1, weight) (8 bytes each; v < vars, b < width, k < slots), made by pcx_teacher_prep from ids
+ * and logits of any strides (in elements): a weight is exp(logit / temperature - norm), norm = norms[b, v], or (norms null, or
+ * not finite) the logsumexp over the position's slots.  Negative ids, logits of -inf and NaN and columns from `batch` on are
+ * empty.
+ *   fwd   out[row0 + m, b] = sum_k weight[var][b][k] * log p_m(category)            (a category >= cats: -inf)
+ *   bwd   table flow of (m, c) = sum over the group's vectors, b and k with category c of weight * flow[row0 + m, b]
+ * A PcxTeacherGeo lists the leaf vectors (PcxTeacherSeg), the groups of vectors that share a table (PcxTeacherGroup) and the
+ * sets of variables whose entries a group sums over; or, with all four tables null, `positions` vectors of `nodes` nodes, with
+ * one table (tied: one group and set) or one each.  [No counterpart in the reference on this path.] */
+typedef struct PcxTeacherSeg {
+    int32_t var, nodes, cats, col;      /* col: first column in a transposed table */
+    int64_t row0, table;                /* first row of the value buffers, first parameter */
+    int64_t flow_col;                   /* sum of nodes rounded up to 4 over the vectors before it, in the order of groups */
+} PcxTeacherSeg;
+typedef struct PcxTeacherGroup {
+    int32_t set, nodes, cats, col;
+    int64_t out, flow_col;              /* first accumulator; flow_col of the group's first vector */
+} PcxTeacherGroup;
+typedef struct PcxTeacherGeo {
+    const void* segs;                   /* device: PcxTeacherSeg [n_segs] */
+    const void* groups;                 /* device: PcxTeacherGroup [n_groups] */
+    const int32_t* set_first;           /* device: [n_sets + 1], into */
+    const int32_t* set_vars;            /* device: variables of the sets, in the order of their groups' vectors */
+    int64_t flow_cols;                  /* sum of nodes rounded up to 4 over all vectors */
+    int32_t positions, nodes, cats, tied;       /* nodes, cats: the largest of any vector */
+    int32_t n_segs, n_groups, n_sets, max_vars; /* max_vars: variables of the largest set */
+    int32_t total_vars, width, slots, pad_;     /* total_vars: over all sets */
+} PcxTeacherGeo;
+int pcx_teacher_prep(void* entries, const void* ids, int wide_ids, int64_t ids_b, int64_t ids_v, int64_t ids_k, const void* logits,
+                     int dtype, int64_t logits_b, int64_t logits_v, int64_t logits_k, const float* norms, int64_t norms_b,
+                     int64_t norms_v, int batch, int vars, int slots, int width, double temperature, void* stream);
+/* out[c * stride + r] = table[r * cats + c], 0 for r in [rows, stride). */
+int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int64_t stride, void* stream);
+/* Nodes per CTA of form 2 of the forward pass; 0: tables of that many categories do not fit. */
+int pcx_teacher_staged_nodes(int cats, int nodes);
+/* form 0: the tables are read where they lie; 1: `table` is turned ([cats][turned_stride]); 2: the tables go through shared
+ * memory; 3: as 1, with turned_stride and all `col` multiples of 4.  take_log (forms 0, 2): the tables hold probabilities. */
+int pcx_teacher_fwd(float* out, const float* table, const void* entries, const PcxTeacherGeo* geo, int form, int64_t turned_stride,
+                    int take_log, void* stream);
+/* mode 0: all of `out` is written (runs: only categories that occur, the caller has cleared it); 1: added; 2: added to a turned
+ * table, touched[c] = 1 for the categories that occur.  runs: visit only categories that occur.  logspace: flows are
+ * logarithms.  `scratch`: pcx_teacher_bwd_scratch_bytes, 256-byte aligned. */
+int64_t pcx_teacher_bwd_scratch_bytes(const PcxTeacherGeo* geo, int runs);
+int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* flows, const void* entries, const PcxTeacherGeo* geo,
+                    int mode, int runs, int64_t turned_stride, int logspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -54,6 +54,96 @@ def _require_cuda(*tensors):
             raise ValueError(f"tensors on {device} and {t.device}")
 
 
+class _Geo(ctypes.Structure):
+    """`PcxTeacherGeo` of the library: the leaf vectors that look at a teacher, and how wide it is."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("segs", "groups", "set_first", "set_vars")] + [("flow_cols", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("positions", "nodes", "cats", "tied", "n_segs", "n_groups", "n_sets", "max_vars",
+                                       "total_vars", "width", "slots", "pad_")]
+
+
+def _prepare(teacher: TopLogits, width: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Categories and weights of a teacher's slots, ``[T, width, K]`` pairs of 32 bits, from ids ``[B, T, K]``."""
+    ids, x, norm = teacher.ids, teacher.logits.detach(), teacher.log_norm
+    B, T, K = ids.shape
+    if out is None:
+        out = torch.empty(T, width, K, 2, dtype=torch.int32, device=ids.device)
+    if out.numel() > 0:
+        nb, nv = (0, 0) if norm is None else norm.stride()
+        _lib.call("pcx_teacher_prep", out, ids, int(ids.dtype == torch.int64), *ids.stride(), x, _TYPES[x.dtype], *x.stride(),
+                  None if norm is None else norm.detach(), nb, nv, B, T, K, width, float(teacher.temperature))
+    return out
+
+
+class _Expected(torch.autograd.Function):
+    """Values of leaf tables under prepared entries; the gradient of the tables."""
+
+    @staticmethod
+    def forward(ctx, log_probs, entries):
+        T, W, K, _ = entries.shape
+        M, C = log_probs.shape[-2:]
+        tied = log_probs.dim() == 2
+        M4 = -(-M // 4) * 4
+        n = 1 if tied else T
+        geo = _Geo(flow_cols=T * M4, positions=T, nodes=M, cats=C, tied=int(tied), n_segs=T, n_groups=n, n_sets=n,
+                   max_vars=T if tied else 1, total_vars=T, width=W, slots=K)
+        ctx.geo, ctx.shape = geo, log_probs.shape
+        ctx.save_for_backward(entries)
+        out = torch.empty(T, M, W, dtype=torch.float32, device=log_probs.device)
+        if out.numel() == 0 or K == 0:
+            return out.zero_()
+        table, form, stride = log_probs.contiguous(), 0, 0
+        named = geo.max_vars * W * K                    # slots that look a table up
+        if not tied and named * 8 >= C and M > 1 and _lib.load().pcx_teacher_staged_nodes(C, M) > 0:
+            form = 2
+        elif M > 1 and named * 4 >= C:
+            rows = n * M
+            stride = -(-rows // 4) * 4
+            turned = torch.empty(C, stride, dtype=torch.float32, device=table.device)
+            _lib.call("pcx_teacher_turn", turned, table, rows, C, stride)
+            table, form = turned, 3 if tied or M % 4 == 0 else 1
+        _lib.call("pcx_teacher_fwd", out, table, entries, ctypes.addressof(geo), form, stride, 0)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        entries, = ctx.saved_tensors
+        geo = ctx.geo
+        runs = geo.max_vars * geo.width * geo.slots * 16 < geo.cats
+        out = (torch.zeros if runs else torch.empty)(ctx.shape, dtype=torch.float32, device=entries.device)
+        if grad.numel() == 0 or geo.slots == 0:
+            return out.zero_(), None
+        scratch = torch.empty(_lib.load().pcx_teacher_bwd_scratch_bytes(ctypes.addressof(geo), int(runs)), dtype=torch.uint8,
+                              device=entries.device)
+        _lib.call("pcx_teacher_bwd", out, None, scratch, grad.contiguous(), entries, ctypes.addressof(geo), 0, int(runs), 0, 0)
+        return out, None
+
+
+def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Tensor:
+    """Log-probabilities of leaf tables expected under a teacher: ``out[t, m, b] = sum_k w[b, t, k] * log_probs[t, m, ids[b, t,
+    k]]`` with the weights of ``teacher`` (see :class:`TopLogits`), whose ids are ``[B, T, K]``.
+
+    ``log_probs`` (float32) is ``[M, C]``, one table of M nodes for all T positions, or ``[T, M, C]``, a table for each.
+    Empty slots add nothing, whatever they hold; a weight of zero takes nothing of a log-probability of -inf; an id of C
+    or more has the log-probability -inf.  Returns float32 ``[T, M, B]``.  The gradient goes to ``log_probs`` (sums in a
+    fixed order: the same bits on every call), none to the teacher.  Up to a million categories.  A backward pass captured
+    into a CUDA graph needs, as torch's own do, that no eager graph of the same leaf is alive while it is captured."""
+    teacher._check()
+    if log_probs.dtype != torch.float32 or log_probs.dim() not in (2, 3):
+        raise TypeError("log_probs must be float32 [M, C] or [T, M, C]")
+    if teacher.ids.dim() != 3:
+        raise ValueError("the teacher's ids must be [B, T, K]")
+    B, T, K = teacher.ids.shape
+    if log_probs.dim() == 3 and log_probs.size(0) != T:
+        raise ValueError(f"{log_probs.size(0)} tables for {T} positions")
+    if not 1 <= log_probs.size(-1) <= 1000000:
+        raise ValueError("tables of 1 to 1000000 categories are supported")
+    if max(B * K, 1) * (T if log_probs.dim() == 2 else 1) >= 2 ** 30:
+        raise ValueError("more than 2^30 slots share a table")
+    _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
+    return _Expected.apply(log_probs, _prepare(teacher, B))
+
+
 def _scratch(rows: int, vocab: int, n: int, device) -> Tuple[torch.Tensor, int]:
     lib = _lib.load()
     with torch.cuda.device(device):
