@@ -19,6 +19,7 @@ import torch.nn as nn
 from . import _lib
 from .compiler import (compile_input, compile_prod, compile_sum_backward, compile_sum_forward,
                        reorder_input_nodes)
+from .lm import Entries, LeafTables
 from .nodes import BitSet, as_bitset
 
 _I32_MAX = 2 ** 31 - 1
@@ -38,7 +39,12 @@ def _rows(*bufs):
 
 
 def _pad_data(data: torch.Tensor, width: int) -> torch.Tensor:
-    """``[V, B]`` categories, padded with category 0 to the row width of the value buffers."""
+    """``[V, B]`` categories, padded with category 0 to the row width of the value buffers.  (Slots of a teacher are prepared
+    at that width.)"""
+    if isinstance(data, Entries):
+        if data.width != width:
+            raise ValueError(f"slots of {data.width} samples for rows of {width}")
+        return data
     return data.contiguous() if data.size(1) == width else nn.functional.pad(data, (0, width - data.size(1)))
 
 
@@ -243,6 +249,9 @@ class InputLayer(Layer, nn.Module):
         for name in ("vids", "s_pids", "s_pfids", "s_mids", "nids", "source_nids", "node_id2source_id", "metadata"):
             self.register_buffer(name, t[name])
         self.tied2source_nids = t["tied2source_nids"]
+        # (variable, nodes, categories, first row, first parameter, first flow or None for a tied vector) of the leaf vectors
+        self._vectors = [(ns.scope.to_list()[0], ns.num_nodes, ns.dist.num_parameters(), ns._output_ind_range[0],
+                          ns._param_range[0], None if ns.is_tied() else ns._param_flow_range[0]) for ns in nodes]
         self.num_nodes = t["num_nodes"]
         self.num_parameters = t["num_parameters"]
         self.num_param_flows = t["num_param_flows"]
@@ -254,6 +263,7 @@ class InputLayer(Layer, nn.Module):
         self.params = nn.Parameter(torch.empty([max(self.num_parameters, 1)], dtype=torch.float32), requires_grad=False)
         self._shadow = None
         self._param_epoch = 0
+        self._teacher_tables = None
         self._arena_zero = False                 # True while the [row, category] flow accumulators are known to be all zero
         self.param_flows = None
         self._dev = {}
@@ -360,7 +370,13 @@ class InputLayer(Layer, nn.Module):
                              s_pfids=_dev_i32(self.s_pfids, device), source_nids=_dev_i32(self.source_nids, device),
                              node_cats=_dev_i32(self.node_cats, device))
         self._setup_shadow(device)
+        self._teacher_tables = None
         return self
+
+    def _leaf_tables(self) -> LeafTables:
+        if self._teacher_tables is None:
+            self._teacher_tables = LeafTables(self._vectors, self._shadow["C"] if self._shadow is not None else 0, self.device)
+        return self._teacher_tables
 
     def _init_parameters(self, perturbation: float):
         """Copy (or draw) the parameters of every untied vector, in layer order (layer/input_layer.py:1131-1143)."""
@@ -394,7 +410,7 @@ class InputLayer(Layer, nn.Module):
             raise NotImplementedError("input layers run on CUDA only (no CPU path)")
 
     def forward(self, data: torch.Tensor, node_mars: torch.Tensor, params=None, missing_mask=None, **kwargs):
-        """``data`` is ``[num_vars, B]`` (variables outermost), integer."""
+        """``data`` is ``[num_vars, B]`` (variables outermost), integer, or the prepared slots of a teacher."""
         _unsupported(params=params is not None, missing_mask=missing_mask is not None)
         self._require_cuda()
         node_mars, = _rows(node_mars)
@@ -423,16 +439,21 @@ class InputLayer(Layer, nn.Module):
                 sh["logp"] = torch.empty(sh["R"] * sh["C"], dtype=torch.float32, device=self.device)
             if stale:                                       # parameters changed: transpose and take logarithms once
                 _lib.call("pcx_input_cat_shadow", sh["logp"], self.params.data, sh["R"], sh["C"])
+            if isinstance(data, Entries):
+                return self._leaf_tables().forward(node_mars, sh["logp"], data, turned_stride=sh["R"])
             _lib.call("pcx_input_cat_fwd_t", node_mars, sh["logp"], data, data.element_size(), self._dev["vids"],
                       sh["prow"], sh["R"], sh["C"], self.num_nodes, self._output_ind_range[0], B)
             return
+        if isinstance(data, Entries):
+            return self._leaf_tables().forward(node_mars, self.params.data, data)
         _lib.call("pcx_input_cat_fwd", node_mars, self.params.data, data, data.element_size(),
                   self._dev["vids"], self._dev["s_pids"], self._dev["node_cats"], self.max_cats,
                   self.num_nodes, self._output_ind_range[0], B)
 
     def backward(self, data: torch.Tensor, node_flows: torch.Tensor, node_mars: torch.Tensor, params=None,
                  logspace_flows: bool = False, missing_mask=None, **kwargs):
-        """Adds the (linear) flow of every (node, sample) to the flow of the observed category."""
+        """Adds the (linear) flow of every (node, sample) to the flow of the observed category, or, in proportion to their
+        weights, to the flows of a teacher's categories."""
         _unsupported(params=params is not None, missing_mask=missing_mask is not None)
         self._require_cuda()
         if self._param_flows is None:
@@ -458,10 +479,14 @@ class InputLayer(Layer, nn.Module):
             if sh["flows"] is None:
                 sh["flows"] = torch.zeros(sh["R"] * sh["C"], dtype=torch.float32, device=self.device)
                 sh["touched"] = torch.zeros(sh["C"], dtype=torch.int32, device=self.device)
+            if isinstance(data, Entries):
+                return self._leaf_tables().backward(sh["flows"], node_flows, data, logspace_flows, sh["R"], sh["touched"])
             _lib.call("pcx_input_cat_bwd_t", sh["flows"], sh["touched"], node_flows, data, data.element_size(), self._dev["vids"],
                       sh["prow"], sh["R"], sh["C"], self.num_nodes, self._output_ind_range[0], B,
                       int(bool(logspace_flows)))
             return
+        if isinstance(data, Entries):
+            return self._leaf_tables().backward(self._param_flows, node_flows, data, logspace_flows)
         _lib.call("pcx_input_cat_bwd", self._param_flows, node_flows, data, data.element_size(),
                   self._dev["vids"], self._dev["s_pfids"], self._dev["node_cats"], self.max_cats,
                   self.num_nodes, self._output_ind_range[0], B, int(bool(logspace_flows)))

@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 from typing import List, NamedTuple, Optional, Tuple
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -72,6 +73,78 @@ def _prepare(teacher: TopLogits, width: int, out: Optional[torch.Tensor] = None)
         _lib.call("pcx_teacher_prep", out, ids, int(ids.dtype == torch.int64), *ids.stride(), x, _TYPES[x.dtype], *x.stride(),
                   None if norm is None else norm.detach(), nb, nv, B, T, K, width, float(teacher.temperature))
     return out
+
+
+class Entries:
+    """A prepared batch of teacher's slots, in the place of a circuit's ``[V, W]`` categories."""
+    __slots__ = ("tensor", "width", "slots")
+
+    def __init__(self, tensor: torch.Tensor):
+        self.tensor = tensor
+        _, self.width, self.slots, _ = tensor.shape
+
+    def data_ptr(self):
+        """What a captured pass goes by: where the slots are, and how many."""
+        return (self.tensor.data_ptr(), *self.tensor.shape)
+
+
+class LeafTables:
+    """The leaf vectors of an input layer as the teacher's kernels walk them: vectors, groups that share a table (in the
+    order of their first vector), and the variables of each group."""
+
+    def __init__(self, vectors, cats_per_row: int, device):
+        """``vectors``: (variable, nodes, categories, first row of the value buffers, first parameter, first flow or None for a
+        tied vector) of every leaf vector."""
+        segs, groups, sets, by_table = [], [], {}, {}
+        for v in vectors:
+            by_table.setdefault(v[4], []).append(v)
+        flow_col = 0
+        for table, members in by_table.items():
+            M, C = members[0][1:3]
+            col = table // cats_per_row if cats_per_row else 0
+            at = sets.setdefault(tuple(v[0] for v in members), len(sets))
+            groups.append((at, M, C, col, next(v[5] for v in members if v[5] is not None), flow_col))
+            for var, _, _, row0, _, _ in members:
+                segs.append((var, M, C, col, row0, table, flow_col))
+                flow_col += -(-M // 4) * 4
+        self.cols_by_four = all(s[3] % 4 == 0 for s in segs)
+        seg = np.zeros(len(segs), dtype=[("a", np.int32, 4), ("b", np.int64, 3)])
+        seg["a"], seg["b"] = [s[:4] for s in segs], [s[4:] for s in segs]
+        grp = np.zeros(len(groups), dtype=[("a", np.int32, 4), ("b", np.int64, 2)])
+        grp["a"], grp["b"] = [g[:4] for g in groups], [g[4:] for g in groups]
+        first = np.cumsum([0] + [len(v) for v in sets]).astype(np.int32)
+        on = lambda a: torch.from_numpy(a.view(np.uint8).copy()).to(device)
+        self._held = [on(seg), on(grp), on(first), on(np.concatenate([np.asarray(v, np.int32) for v in sets]))]
+        self.sizes = dict(flow_cols=flow_col, nodes=max(s[1] for s in segs), cats=max(s[2] for s in segs), n_segs=len(segs),
+                          n_groups=len(groups), n_sets=len(sets), max_vars=max(len(v) for v in sets), total_vars=int(first[-1]))
+
+    def geo(self, entries: Entries) -> _Geo:
+        return _Geo(*[t.data_ptr() for t in self._held], width=entries.width, slots=entries.slots, **self.sizes)
+
+    def _named(self, entries: Entries) -> int:
+        """Slots that look one table up."""
+        return self.sizes["max_vars"] * entries.width * entries.slots
+
+    def forward(self, node_mars: torch.Tensor, params: torch.Tensor, entries: Entries, turned_stride: int = 0):
+        """``params``: probabilities of the tables, or (``turned_stride``) their transposed logarithms."""
+        geo = self.geo(entries)
+        if turned_stride:
+            form = 3 if self.cols_by_four and turned_stride % 4 == 0 else 1
+        else:
+            form = 2 if (self._named(entries) * 8 >= geo.cats and
+                         _lib.load().pcx_teacher_staged_nodes(geo.cats, geo.nodes) > 0) else 0
+        _lib.call("pcx_teacher_fwd", node_mars, params, entries.tensor, ctypes.addressof(geo), form, turned_stride,
+                  int(turned_stride == 0))
+
+    def backward(self, flows: torch.Tensor, node_flows: torch.Tensor, entries: Entries, logspace: bool, turned_stride: int = 0,
+                 touched: Optional[torch.Tensor] = None):
+        """Adds to the accumulators of the tables, or (``turned_stride``) to transposed ones."""
+        geo = self.geo(entries)
+        runs = int(self._named(entries) * 16 < geo.cats)
+        scratch = torch.empty(_lib.load().pcx_teacher_bwd_scratch_bytes(ctypes.addressof(geo), runs), dtype=torch.uint8,
+                              device=flows.device)
+        _lib.call("pcx_teacher_bwd", flows, touched, scratch, node_flows, entries.tensor, ctypes.addressof(geo),
+                  2 if turned_stride else 1, runs, turned_stride, int(logspace))
 
 
 class _Expected(torch.autograd.Function):

@@ -32,6 +32,7 @@ from .compiler import _IdDict, compile_cum_par_flows, compile_par_update, create
 from .layers import InputLayer, LayerGroup, ParamPacker, ProdLayer, SumLayer, _alg_of, _fill, _scale, _unsupported
 from .column import ColumnProgram, Unsupported
 from .flows import FlowArena
+from .lm import Entries, TopLogits, _prepare
 from .nodes import as_bitset
 
 NEG_INF = float("-inf")
@@ -371,7 +372,7 @@ class TensorCircuit(nn.Module):
         self._fusing_dev = [(start, n, torch.tensor(accs, dtype=torch.int64, device=device))
                             for start, n, accs in self._tied_sum_groups]
         self._nm = self._em = self._nf = self._ef = self.param_flows = None
-        self._data_buf = self._root_view = self._root_w = self._cum_buf = None
+        self._data_buf = self._token_buf = self._teacher_buf = self._root_view = self._root_w = self._cum_buf = None
         if device.type == "cuda":
             self._mask_parentless_in_device_tables()
         self._setup_fusion()
@@ -571,6 +572,8 @@ class TensorCircuit(nn.Module):
     def _prepare_inputs(self, inputs: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The batch as ``[V, W]`` int32 (variables outermost, batch padded with category 0), the layout every leaf
         kernel reads.  ``out`` is written when it fits."""
+        if isinstance(inputs, TopLogits):
+            return self._prepare_teacher(inputs, out)
         assert inputs.dim() == 2 and inputs.size(1) >= self.num_vars
         if inputs.is_floating_point():
             raise TypeError("categorical inputs must be an integer tensor")
@@ -582,6 +585,22 @@ class TensorCircuit(nn.Module):
         if out is None or out.size(0) != V or out.size(1) != W:
             out = torch.empty(V, W, dtype=torch.int32, device=self.device)
         _lib.call("pcx_load_inputs", out, x, x.element_size(), B, V, x.stride(0), x.stride(1), W)
+        return out
+
+    def _prepare_teacher(self, teacher: TopLogits, out: Optional[Entries] = None) -> Entries:
+        """The slots of a teacher, variables outermost, batch padded with empty slots."""
+        teacher._check()
+        if teacher.ids.dim() != 3 or teacher.ids.size(1) < self.num_vars or teacher.ids.size(2) < 1:
+            raise ValueError(f"the teacher's ids must be [B, {self.num_vars}, K] with at least one slot")
+        B, K = teacher.ids.size(0), teacher.ids.size(2)
+        W = -(-B // self._PAD) * self._PAD
+        if W * K * self.num_vars >= 2 ** 30:
+            raise ValueError("more than 2^30 slots in a batch")
+        move = lambda t: t if t is None else t[:, :self.num_vars].to(self.device, non_blocking=True)
+        shape = (self.num_vars, W, K, 2)
+        if out is None or tuple(out.tensor.shape) != shape:
+            out = Entries(torch.empty(shape, dtype=torch.int32, device=self.device))
+        _prepare(teacher._replace(ids=move(teacher.ids), logits=move(teacher.logits), log_norm=move(teacher.log_norm)), W, out.tensor)
         return out
 
     def _run_inner(self, key, fn):
@@ -802,7 +821,11 @@ class TensorCircuit(nn.Module):
     @_in_own_mode
     def forward(self, inputs: torch.Tensor, input_layer_fn=None, cache=None, return_cache: bool = False,
                 propagation_alg: Optional[str] = None, pflow_temperature: float = 1.0, **kwargs):
-        """Per-sample log-likelihoods ``[B, num_roots]`` of ``inputs`` (``[B, num_vars]``, integer)."""
+        """Per-sample log-likelihoods ``[B, num_roots]`` of ``inputs`` (``[B, num_vars]``, integer).
+
+        With a :class:`~pyjuice_b200.lm.TopLogits` (ids and logits ``[B, num_vars, K]``) the leaves see a teacher: a leaf's
+        value is its log-probability expected under the teacher's weights of that variable, a variable without slots is
+        marginalised, and the backward pass spreads a leaf's flow over the teacher's categories."""
         self._require_cuda()
         if kwargs or input_layer_fn is not None or cache is not None or return_cache or pflow_temperature != 1.0:
             _unsupported(input_layer_fn=input_layer_fn is not None, cache=cache is not None, return_cache=return_cache,
@@ -810,10 +833,16 @@ class TensorCircuit(nn.Module):
                          missing_mask=kwargs.get("missing_mask") is not None)
         origin_inputs = inputs
         with torch.no_grad():
-            B = inputs.size(0)
+            if isinstance(inputs, TopLogits):
+                data = self._teacher_buf = self._prepare_teacher(inputs, self._teacher_buf)
+                B = inputs.ids.size(0)
+            else:
+                data, B = None, inputs.size(0)
             self._ensure_buffers(B)
             W = self._nm.size(1)
-            data = self._data_buf = self._prepare_inputs(inputs, out=self._data_buf)
+            if data is None:
+                data = self._token_buf = self._prepare_inputs(inputs, out=self._token_buf)
+            self._data_buf = data
             self._last_inputs = origin_inputs
             if W > 0:                           # (an empty batch has nothing to launch)
                 self._forward_launches(data, W)
@@ -1061,7 +1090,7 @@ class TensorCircuit(nn.Module):
             if own:
                 data = self._data_buf
             else:
-                assert inputs.dim() == 2 and inputs.size(0) == B
+                assert (inputs.ids if isinstance(inputs, TopLogits) else inputs).size(0) == B
                 data = self._prepare_inputs(inputs)
             self._ensure_buffers(B, backward=True)
             ls = int(bool(logspace_flows))
