@@ -10,6 +10,7 @@ from .nodes import distributions
 from .model import TensorCircuit, compile
 from .io import save, load
 from .layers import InputLayer, ProdLayer, SumLayer, LayerGroup
+from . import decoding
 
 __version__ = "0.1.0"
 

@@ -818,6 +818,28 @@ class TensorCircuit(nn.Module):
             if stale:
                 layer._mark_shadow()
 
+    def _values_of_inner(self, leaves, B: int, inputs: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Log-values of the root nodes, ``[num_roots, W]`` (a view of the value buffer), for B columns whose input vectors
+        hold given log-values: ``leaves`` lists (vector, ``[nodes, B]``); the other vectors look at ``inputs``."""
+        self._require_cuda()
+        with torch.no_grad(), _lib.use_sum_mode(self.sum_mode):
+            self._ensure_buffers(B)
+            W = self._nm.size(1)
+            if inputs is not None:
+                data = self._data_buf = self._token_buf = self._prepare_inputs(inputs, out=self._token_buf)
+                for layer in self.input_layer_group:
+                    layer.forward(data, self._nm)
+            for ns, values in leaves:
+                s, e = ns._output_ind_range
+                self._nm[s:e, :B].copy_(values)
+            plan = self._column_plan()
+            if _lib.sum_mode() != 0 and self._packer.stale(self._sum_params, plan):
+                self._packer.prepare(plan)
+                self._packer.launch(self.params.data, plan)
+                self._packer.mark(self._sum_params, plan)
+            self._run_inner(("fv", W, self._launch_cfg(), self._param_ptrs()), self._forward_inner)
+            return self._nm[self._root_node_range[0]:self._root_node_range[1]]
+
     @_in_own_mode
     def forward(self, inputs: torch.Tensor, input_layer_fn=None, cache=None, return_cache: bool = False,
                 propagation_alg: Optional[str] = None, pflow_temperature: float = 1.0, **kwargs):
