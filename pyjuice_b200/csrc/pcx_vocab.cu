@@ -16,19 +16,16 @@
 
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kTile = kThreads * 16;     // logits of a tile: 16 per thread
-constexpr int kMaxTop = 128;                                                      // entries of a list
-constexpr int kFew = 512;                                                         // candidates ranked by counting at once
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxTop = 128;                        // entries of a list
+constexpr int kRoom = 4096;                         // candidates a CTA holds besides its list
+constexpr int kFew = 512;                           // candidates ranked by counting at once
+constexpr int kMaxSplits = 32;                      // parts of a row: their lists fit kRoom
 
 typedef unsigned long long u64;
 
-// What a CTA leaves for the join: the sorted keys of its list, then the maximum and the sum of its part.
+// What a CTA leaves for the join: the sorted keys of its list, the maximum of its part and the sum of exp((x - m) / T).
 struct Part { float m; int count; double s; };
-
-template <typename T> __device__ __forceinline__ float to_f32(T x);
-template <> __device__ __forceinline__ float to_f32(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 
 // Unsigned integers in the order of the floats; one zero (-0 counts as 0).
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -46,6 +43,48 @@ __device__ __forceinline__ double unordered(u64 k) {
     return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
 }
 __device__ __forceinline__ u64 key_of(float x, uint32_t place) { return ((u64)ordered(x) << 32) | (uint32_t)~place; }
+__device__ __forceinline__ float value_of(u64 key) { return unordered((uint32_t)(key >> 32)); }
+__device__ __forceinline__ uint32_t place_of(u64 key) { return ~(uint32_t)key; }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16 bytes of logits: their maximum (NaN skipped) and the logits one by one.
+template <typename T> struct Pack;
+template <> struct Pack<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ float max(const uint4& v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    }
+    static __device__ __forceinline__ float at(const uint4& v, int i) { return __uint_as_float((&v.x)[i]); }
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ float max(const uint4& v) {
+        const __nv_bfloat162* h = (const __nv_bfloat162*)&v;
+        const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ float at(const uint4& v, int i) {
+        const uint32_t w = (&v.x)[i >> 1];
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
+    }
+};
+template <> struct Pack<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ float max(const uint4& v) {
+        const __half2* h = (const __half2*)&v;
+        const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    static __device__ __forceinline__ float at(const uint4& v, int i) {
+        const __half2 h = ((const __half2*)&v)[i >> 1];
+        return i & 1 ? __high2float(h) : __low2float(h);
+    }
+};
 
 struct RowArgs {
     const void* logits;
@@ -70,7 +109,7 @@ __device__ __forceinline__ double log_norm(float m, double s, double inv_t) {
 }
 
 struct Shared {
-    u64 keys[kTile + kMaxTop];     // the list (sorted, first), behind it the candidates of a tile
+    u64 keys[kRoom + kMaxTop];     // the list (sorted, first), behind it the candidates of a tile
     u64 list[kMaxTop];
     float red_m[kWarps];
     double red_s[kWarps];
@@ -78,42 +117,53 @@ struct Shared {
     int count;
 };
 
+__device__ __forceinline__ int block_sum(int mine, int* total) {       // every thread gets the sum
+    mine = __reduce_add_sync(~0u, mine);
+    __syncthreads();
+    if (threadIdx.x == 0) *total = 0;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0 && mine != 0) atomicAdd(total, mine);
+    __syncthreads();
+    return *total;
+}
+
+// The largest threshold t, by bisection, with least <= #(keys >= t) <= most, or (keys are unique, so only when `most` <
+// `least`) the smallest count above; `count(t)` gives a thread's share.
+template <typename F>
+__device__ __forceinline__ u64 bisect(int least, int most, int* total, F count) {
+    u64 lo = 0, hi = ~0ull;
+    while (lo < hi) {
+        const u64 mid = lo + ((hi - lo) >> 1) + ((hi - lo) & 1);
+        const int c = block_sum(count(mid), total);
+        if (c >= least) {
+            lo = mid;
+            if (c <= most) break;
+        } else {
+            hi = mid - 1;
+        }
+    }
+    __syncthreads();
+    return lo;
+}
+
 // Keeps the n largest of the `total` unique keys in sh.keys, sorted, at its front.  Returns how many there are.
 __device__ int prune(Shared& sh, int total, int n) {
     const int tid = threadIdx.x;
     if (total > kFew) {
-        // bisect over the key's bits until no more than kFew keys (and at least n) are above the threshold
-        u64 lo = 0, hi = ~0ull;
-        while (true) {
-            const u64 mid = lo + ((hi - lo) >> 1) + ((hi - lo) & 1);
-            int mine = 0;
-            for (int i = tid; i < total; i += kThreads) mine += sh.keys[i] >= mid;
-            for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
-            if (tid == 0) sh.count = 0;
-            __syncthreads();
-            if ((tid & 31) == 0) atomicAdd(&sh.count, mine);
-            __syncthreads();
-            const int c = sh.count;
-            __syncthreads();
-            if (c >= n) { lo = mid; if (c <= kFew) break; }
-            else hi = mid - 1;
-            if (lo >= hi) break;
-        }
-        // compaction through registers: a thread's keys are read before any is overwritten
-        u64 own[(kTile + kMaxTop + kThreads - 1) / kThreads];
-#pragma unroll
-        for (int j = 0; j < (kTile + kMaxTop + kThreads - 1) / kThreads; ++j) {
-            const int i = tid + j * kThreads;
-            own[j] = i < total ? sh.keys[i] : 0;
-        }
+        const u64 t = bisect(n, kFew, &sh.count, [&](u64 mid) {
+            int c = 0;
+            for (int i = tid; i < total; i += kThreads) c += sh.keys[i] >= mid;
+            return c;
+        });
+        // compaction, a block of keys after the other: those of a block are read before any is overwritten
         if (tid == 0) sh.count = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < (kTile + kMaxTop + kThreads - 1) / kThreads; ++j)
-            if (own[j] != 0 && own[j] >= lo) sh.keys[atomicAdd(&sh.count, 1)] = own[j];
+        for (int i0 = 0; i0 < total; i0 += kThreads) {
+            const u64 own = i0 + tid < total ? sh.keys[i0 + tid] : 0;
+            __syncthreads();
+            if (own >= t && own != 0) sh.keys[atomicAdd(&sh.count, 1)] = own;
+        }
         __syncthreads();
         total = sh.count;
-        __syncthreads();
     }
     const int kept = min(total, n);
     for (int i = tid; i < total; i += kThreads) {
@@ -128,55 +178,110 @@ __device__ int prune(Shared& sh, int total, int n) {
     return kept;
 }
 
+// Statistics of a block: maximum and sum of all threads' (m, s), to every thread.
+__device__ __forceinline__ void block_stats(Shared& sh, float m, double s, double inv_t, float& M, double& S) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    M = m;
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    if (lane == 0) sh.red_m[warp] = M;
+    __syncthreads();
+    M = sh.red_m[0];
+    for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh.red_m[w]);
+    S = m > PCX_NEG_INF && M < CUDART_INF_F ? s * exp((double)(m - M) * inv_t) : 0.0;
+    for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(~0u, S, o);
+    if (lane == 0) sh.red_s[warp] = S;
+    __syncthreads();
+    S = 0.0;
+    for (int w = 0; w < kWarps; ++w) S += sh.red_s[w];
+}
+
+// An answer of top logits, or a part of one.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__device__ __forceinline__ void leave(const RowArgs& a, const Shared& sh, int64_t row, int have, float M, double S) {
+    const int tid = threadIdx.x;
+    if (a.ids == nullptr) {
+        if (tid == 0) a.parts[blockIdx.x] = Part{M, have, S};
+        for (int i = tid; i < have; i += kThreads) a.keys[(int64_t)blockIdx.x * a.n + i] = sh.keys[i];
+        return;
+    }
+    if (tid == 0) a.norms[row] = (float)log_norm(M, S, a.inv_t);
+    for (int i = tid; i < a.n; i += kThreads) {
+        const u64 k = i < have ? sh.keys[i] : 0;
+        a.ids[row * a.n + i] = i < have ? (int64_t)place_of(k) : -1;
+        ((T*)a.values)[row * a.n + i] = i < have ? (T)value_of(k) : (T)PCX_NEG_INF;
+    }
+}
+
+// G groups of 16 bytes a thread and tile.
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads, G > 4 ? 3 : 4)
 top_rows_kernel(RowArgs a) {
-    constexpr int VE = 16 / (int)sizeof(T), G = 16 / VE;
+    constexpr int VE = Pack<T>::N;
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / a.splits;
     const int part = blockIdx.x % a.splits;
-    float m = PCX_NEG_INF, s = 0.0f;
+    // The terms of a sum are 2^(x * scale - r) with r = m * scale rounded once: one fused operation each, and all of them
+    // relative to the same r.  What r is off is put right when the sum is read.
+    float m = PCX_NEG_INF, r = PCX_NEG_INF, s = 0.0f;
     int have = 0;
     bool skip = a.finished != nullptr && a.finished[row] != 0;
     if (a.scores != nullptr) skip |= !(a.scores[row] > PCX_NEG_INF);
     if (!skip) {
         const T* x = (const T*)a.logits + (row / a.inner) * a.stride0 + (row % a.inner) * a.stride1;
-        // groups of 16 bytes that begin on 16-byte boundaries; the first and the last may reach over the row's ends
+        // groups begin on 16-byte boundaries; the first and the last may reach over the row's ends
         const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
         const int groups = (int)(((int64_t)off + a.vocab + VE - 1) / VE);
         const int per = (groups + a.splits - 1) / a.splits;
         const int g0 = part * per, g1 = min(groups, g0 + per);
         float bound = PCX_NEG_INF;             // value of the last entry of a full list
         for (int g = g0; g < g1; g += kThreads * G) {
-            T v[G][VE];
+            uint4 v[G];
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 const int gi = g + j * kThreads + tid;
                 const int e = gi * VE - off;
                 if (gi < g1 && e >= 0 && e + VE <= a.vocab) {
-                    *(uint4*)v[j] = __ldg((const uint4*)(x + e));
+                    v[j] = __ldcs((const uint4*)(x + e));
                 } else {
+                    T edge[VE];
 #pragma unroll
                     for (int i = 0; i < VE; ++i)
-                        v[j][i] = gi < g1 && e + i >= 0 && e + i < a.vocab ? x[e + i] : (T)PCX_NEG_INF;
+                        edge[i] = gi < g1 && e + i >= 0 && e + i < a.vocab ? x[e + i] : (T)PCX_NEG_INF;
+                    v[j] = *(const uint4*)edge;
                 }
             }
             float top = PCX_NEG_INF;
 #pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < VE; ++i) top = fmaxf(top, to_f32(v[j][i]));       // (skips NaN)
+            for (int j = 0; j < G; ++j) top = fmaxf(top, Pack<T>::max(v[j]));
             if (top > m) {
-                s *= exp2f((m - top) * a.scale);
+                const float nr = top * a.scale;
+                const bool plain = fabsf(r) < CUDART_INF_F && fabsf(nr) < CUDART_INF_F;
+                s = m > PCX_NEG_INF ? s * exp2_fast(plain ? r - nr : (m - top) * a.scale) : 0.0f;
                 m = top;
+                r = nr;
             }
             if (m > PCX_NEG_INF) {
+                float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
                 for (int j = 0; j < G; ++j)
 #pragma unroll
-                    for (int i = 0; i < VE; ++i)
-                        s += exp2f((fmaxf(to_f32(v[j][i]), PCX_NEG_INF) - m) * a.scale);
+                    for (int i = 0; i < VE; i += 2) {
+                        s0 += exp2_fast(fmaf(Pack<T>::at(v[j], i), a.scale, -r));
+                        s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
+                    }
+                s0 += s1;
+                if (!(s0 < CUDART_INF_F) || !(fabsf(r) < CUDART_INF_F)) {        // NaN, infinities, or |m| near the largest number
+                    s0 = 0.0f;
+#pragma unroll 1
+                    for (int i = 0; i < G * VE; ++i) {
+                        const int gi = g + i / VE * kThreads + tid, e = gi * VE - off + i % VE;
+                        if (gi >= g1 || e < 0 || e >= a.vocab) continue;
+                        const float f = fmaxf((float)x[e], PCX_NEG_INF);
+                        s0 += exp2_fast(f == m ? 0.0f : fabsf(r) < CUDART_INF_F ? fmaf(f, a.scale, -r) : (f - m) * a.scale);
+                    }
+                }
+                s += s0;
             }
             if (!__syncthreads_or(top > bound)) continue;
             // A lower bound of the tile's n-th largest logit: every warp's (n / warps)-th largest thread maximum, the
@@ -192,142 +297,173 @@ top_rows_kernel(RowArgs a) {
                 }
             const int nth = (a.n + kWarps - 1) / kWarps - 1;
             if (lane == nth) sh.warp_t[warp] = k;
-            if (tid == 0) sh.count = have;
             __syncthreads();
             uint32_t t = sh.warp_t[0];
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) t = min(t, sh.warp_t[w]);
             const float least = unordered(t);
+            // every logit that may be among the n largest so far, read again (its group is among the few that hold one);
+            // `from`: a key below which none is wanted
+            uint32_t hot = 0;
             if (top > bound && top >= least) {
 #pragma unroll
-                for (int j = 0; j < G; ++j)
+                for (int j = 0; j < G; ++j) {
+                    const float gm = Pack<T>::max(v[j]);
+                    hot |= (uint32_t)(gm > bound && gm >= least) << j;
+                }
+            }
+            auto each = [&](u64 from, auto&& found) {
+                for (uint32_t left = hot; left != 0; left &= left - 1) {
+                    const int e = (g + (__ffs(left) - 1) * kThreads + tid) * VE - off;
 #pragma unroll
                     for (int i = 0; i < VE; ++i) {
-                        const float f = to_f32(v[j][i]);
-                        if (f > bound && f >= least)
-                            sh.keys[atomicAdd(&sh.count, 1)] =
-                                key_of(f, (uint32_t)((g + j * kThreads + tid) * VE - off + i));
+                        if (e + i < 0 || e + i >= a.vocab) continue;
+                        const float f = (float)x[e + i];
+                        if (f > bound && f >= least) {
+                            const u64 key = key_of(f, (uint32_t)(e + i));
+                            if (key >= from) found(key);
+                        }
                     }
+                }
+            };
+            auto collect = [&](u64 from) {
+                if (tid == 0) sh.count = have;
+                __syncthreads();
+                each(from, [&](u64 key) {
+                    const int at = atomicAdd(&sh.count, 1);
+                    if (at < kRoom + kMaxTop) sh.keys[at] = key;
+                });
+                __syncthreads();
+                const int total = sh.count;
+                __syncthreads();
+                return total;
+            };
+            int total = collect(0);
+            if (total > kRoom + kMaxTop) {
+                // too many (ordered or equal logits): the exact n-th largest, whatever it takes
+                const u64 from = bisect(a.n, kRoom, &sh.count, [&](u64 mid) {
+                    int c = 0;
+                    each(mid, [&](u64) { ++c; });
+                    return c;
+                });
+                total = collect(from);
             }
-            __syncthreads();
-            const int total = sh.count;
-            __syncthreads();
             have = prune(sh, total, a.n);
-            if (have == a.n) bound = unordered((uint32_t)(sh.keys[a.n - 1] >> 32));
+            if (have == a.n) bound = value_of(sh.keys[a.n - 1]);
         }
     }
-    // the part's maximum and sum
-    float M = m;
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    if (lane == 0) sh.red_m[warp] = M;
-    __syncthreads();
-    M = sh.red_m[0];
-    for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh.red_m[w]);
-    double S = m > PCX_NEG_INF && M < CUDART_INF_F ? (double)s * exp((double)(m - M) * a.inv_t) : 0.0;
-    for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(~0u, S, o);
-    if (lane == 0) sh.red_s[warp] = S;
-    __syncthreads();
-    if (a.ids != nullptr) {
-        if (tid == 0 && a.norms != nullptr) {
-            S = 0.0;
-            for (int w = 0; w < kWarps; ++w) S += sh.red_s[w];
-            a.norms[row] = (float)log_norm(M, S, a.inv_t);
-        }
-        for (int i = tid; i < a.n; i += kThreads) {
-            const u64 k = i < have ? sh.keys[i] : 0;
-            a.ids[row * a.n + i] = i < have ? (int64_t)(uint32_t)~(uint32_t)k : -1;
-            ((T*)a.values)[row * a.n + i] = i < have ? (T)unordered((uint32_t)(k >> 32)) : (T)PCX_NEG_INF;
-        }
-        return;
-    }
-    if (tid == 0) {
-        S = 0.0;
-        for (int w = 0; w < kWarps; ++w) S += sh.red_s[w];
-        a.parts[blockIdx.x] = Part{M, have, S};
-    }
-    for (int i = tid; i < have; i += kThreads) a.keys[(int64_t)blockIdx.x * a.n + i] = sh.keys[i];
+    float M;
+    double S;
+    const double off_by = fabsf(r) < CUDART_INF_F ? (double)r - (double)m * (double)a.scale : 0.0;
+    block_stats(sh, m, m > PCX_NEG_INF ? (double)s * exp2(off_by) : 0.0, a.inv_t, M, S);
+    leave<T>(a, sh, row, have, M, S);
 }
 
 // ---- the join --------------------------------------------------------------------------------------------------------
 
-struct JoinArgs {
-    const u64* keys;
-    const Part* parts;
-    const float* scores;           // null: logits themselves are compared (top logits)
+// The parts of a row become one: in place of the row's answer (top logits) or as its only part (beams).
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+join_parts_kernel(RowArgs a, const u64* keys, const Part* parts) {
+    __shared__ Shared sh;
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    float m = PCX_NEG_INF;
+    double s = 0.0;
+    if (tid < a.splits) {
+        m = parts[row * a.splits + tid].m;
+        s = parts[row * a.splits + tid].s;
+    }
+    for (int i = tid; i < a.splits * a.n; i += kThreads)
+        if (i % a.n < parts[row * a.splits + i / a.n].count)
+            sh.keys[atomicAdd(&sh.count, 1)] = keys[row * a.splits * a.n + i];
+    __syncthreads();
+    const int total = sh.count;
+    __syncthreads();
+    const int have = prune(sh, total, a.n);
+    float M;
+    double S;
+    block_stats(sh, m, s, a.inv_t, M, S);
+    leave<T>(a, sh, row, have, M, S);
+}
+
+struct BeamArgs {
+    const u64* keys;               // [batch * beams][n]
+    const Part* parts;             // [batch * beams]
+    const float* scores;
     const uint8_t* finished;
-    float* out_scores;             // beams
-    int64_t* ids;                  // beams: tokens
-    int64_t* parents;              // beams
-    void* values;                  // top logits, in their type
-    float* norms;                  // top logits
-    int rows, splits, n, vocab, pad_id, normalize, elsize;       // rows: beams of an answer
-    double inv_t;
+    float* out_scores;
+    int64_t *tokens, *parents;
+    int beams, n, vocab, pad_id, normalize;
 };
 
-constexpr int kJoinTile = 2048;                     // candidates looked at together
-struct JoinShared {
-    u64 score[kJoinTile + kMaxTop];
-    uint32_t place[kJoinTile + kMaxTop];            // beam * vocab + token: a lower one first among equal scores
+constexpr int kBeamTile = 2048;                     // candidates looked at together
+struct BeamShared {
+    u64 score[kBeamTile + kMaxTop];
+    uint32_t place[kBeamTile + kMaxTop];            // beam * vocab + token: a lower one first among equal scores
     u64 list_s[kMaxTop];
     uint32_t list_p[kMaxTop];
+    double base[kMaxTop];                           // what a beam's logits are raised by
     int count;
 };
 
-__device__ __forceinline__ void store_value(void* out, int elsize, int64_t i, float x) {
-    if (elsize == 4) ((float*)out)[i] = x;
-    else if (elsize == 2) ((__nv_bfloat16*)out)[i] = __float2bfloat16(x);
-    else ((__half*)out)[i] = __float2half(x);       // elsize 3 stands for fp16
-}
-
+// One CTA per sequence.
 __global__ void __launch_bounds__(kThreads)
-join_kernel(JoinArgs a) {
-    __shared__ JoinShared sh;
-    extern __shared__ double base[];                // [rows] what a row's logits are raised by
+join_beams_kernel(BeamArgs a) {
+    __shared__ BeamShared sh;
     const int tid = threadIdx.x;
-    const int64_t first = (int64_t)blockIdx.x * a.rows;
-    for (int r = tid; r < a.rows; r += kThreads) {
-        const Part* p = a.parts + (first + r) * a.splits;
-        float M = PCX_NEG_INF;
-        for (int i = 0; i < a.splits; ++i) M = fmaxf(M, p[i].m);
-        double S = 0.0;
-        for (int i = 0; i < a.splits; ++i)
-            if (p[i].m > PCX_NEG_INF && M < CUDART_INF_F) S += p[i].s * exp((double)(p[i].m - M) * a.inv_t);
-        const double norm = log_norm(M, S, a.inv_t);
-        if (a.norms != nullptr) a.norms[first + r] = (float)norm;
-        base[r] = a.scores == nullptr ? 0.0 : (double)a.scores[first + r] - (a.normalize ? norm : 0.0);
-    }
+    const int64_t first = (int64_t)blockIdx.x * a.beams;
     if (tid == 0) sh.count = 0;
     __syncthreads();
-    const int64_t slots = (int64_t)a.rows * a.splits * a.n;
-    int have = 0;
-    if (a.finished != nullptr) {                    // a finished beam has one continuation, at its own score
-        for (int r = tid; r < a.rows; r += kThreads)
-            if (a.finished[first + r] != 0) {
-                const float sc = a.scores[first + r];
-                if (sc > PCX_NEG_INF) {
-                    const int at = atomicAdd(&sh.count, 1);
-                    sh.score[at] = ordered((double)sc);
-                    sh.place[at] = (uint32_t)r * a.vocab + a.pad_id;
-                }
-            }
-        __syncthreads();
+    for (int b = tid; b < a.beams; b += kThreads) {
+        const Part p = a.parts[first + b];
+        const float sc = a.scores[first + b];
+        sh.base[b] = (double)sc - (a.normalize ? log_norm(p.m, p.s, 1.0) : 0.0);
+        if (a.finished != nullptr && a.finished[first + b] != 0 && sc > PCX_NEG_INF) {
+            const int at = atomicAdd(&sh.count, 1); // a finished beam has one continuation, at its own score
+            sh.score[at] = ordered((double)sc);
+            sh.place[at] = (uint32_t)b * a.vocab + a.pad_id;
+        }
     }
-    for (int64_t at = 0; at < slots || at == 0; at += kJoinTile - kMaxTop) {
-        for (int i = tid; i < kJoinTile - kMaxTop; i += kThreads) {
-            const int64_t slot = at + i;
-            if (slot >= slots) continue;
-            const int list = (int)(slot / a.n), entry = (int)(slot % a.n);
-            if (entry >= a.parts[first * a.splits + list].count) continue;
-            const u64 k = a.keys[(first * a.splits + list) * a.n + entry];
-            const int r = list / a.splits;
-            const double score = base[r] + (double)unordered((uint32_t)(k >> 32));
+    __syncthreads();
+    const int slots = a.beams * a.n;
+    int have = 0;
+    for (int at = 0; at < slots; at += kBeamTile - kMaxTop) {
+        for (int i = tid; i < kBeamTile - kMaxTop && at + i < slots; i += kThreads) {
+            const int b = (at + i) / a.n, entry = (at + i) % a.n;
+            if (entry >= a.parts[first + b].count) continue;
+            const u64 k = a.keys[first * a.n + at + i];
+            const double score = sh.base[b] + (double)value_of(k);
             if (!(score > -CUDART_INF)) continue;   // NaN: a row without a normaliser
             const int to = atomicAdd(&sh.count, 1);
             sh.score[to] = ordered(score);
-            sh.place[to] = (uint32_t)r * a.vocab + ~(uint32_t)k;
+            sh.place[to] = (uint32_t)b * a.vocab + place_of(k);
         }
         __syncthreads();
-        const int total = sh.count;
+        int total = sh.count;
+        __syncthreads();
+        if (total > kFew) {
+            const u64 t = bisect(a.n, kFew, &sh.count, [&](u64 mid) {
+                int c = 0;
+                for (int i = tid; i < total; i += kThreads) c += sh.score[i] >= mid;
+                return c;
+            });
+            if (tid == 0) sh.count = 0;
+            for (int i0 = 0; i0 < total; i0 += kThreads) {
+                const u64 own = i0 + tid < total ? sh.score[i0 + tid] : 0;
+                const uint32_t place = i0 + tid < total ? sh.place[i0 + tid] : 0;
+                __syncthreads();
+                if (own >= t && own != 0) {
+                    const int to = atomicAdd(&sh.count, 1);
+                    sh.score[to] = own;
+                    sh.place[to] = place;
+                }
+            }
+            __syncthreads();
+            total = sh.count;
+        }
         for (int i = tid; i < total; i += kThreads) {
             const u64 s = sh.score[i];
             const uint32_t p = sh.place[i];
@@ -348,14 +484,9 @@ join_kernel(JoinArgs a) {
         const int64_t to = (int64_t)blockIdx.x * a.n + i;
         const bool is = i < have;
         const uint32_t p = is ? sh.place[i] : 0;
-        if (a.parents == nullptr) {
-            a.ids[to] = is ? (int64_t)p : -1;
-            store_value(a.values, a.elsize, to, is ? (float)unordered(sh.score[i]) : PCX_NEG_INF);
-        } else {
-            a.ids[to] = is ? (int64_t)(p % (uint32_t)a.vocab) : -1;
-            a.parents[to] = is ? (int64_t)(p / (uint32_t)a.vocab) : 0;
-            a.out_scores[to] = is ? (float)unordered(sh.score[i]) : PCX_NEG_INF;
-        }
+        a.tokens[to] = is ? (int64_t)(p % (uint32_t)a.vocab) : -1;
+        a.parents[to] = is ? (int64_t)(p / (uint32_t)a.vocab) : 0;
+        a.out_scores[to] = is ? (float)unordered(sh.score[i]) : PCX_NEG_INF;
     }
 }
 
@@ -400,66 +531,86 @@ int sm_count() {
     return counts[d];
 }
 
-int launch_rows(const RowArgs& a, int dtype, int64_t rows, cudaStream_t stream) {
+template <typename T>
+void launch_rows(const RowArgs& a, int64_t rows, cudaStream_t stream) {
     const unsigned grid = (unsigned)(rows * a.splits);
-    switch (dtype) {
-        case 0: top_rows_kernel<float><<<grid, kThreads, 0, stream>>>(a); break;
-        case 1: top_rows_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(a); break;
-        case 2: top_rows_kernel<__half><<<grid, kThreads, 0, stream>>>(a); break;
-        default: return -1;
+    const int64_t groups = a.vocab / Pack<T>::N / a.splits;
+    if (groups > 3 * kThreads) top_rows_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
+    else top_rows_kernel<T, 2><<<grid, kThreads, 0, stream>>>(a);
+}
+
+// The lists of all rows, one part each when this returns: in the answer's place, or in `keys` and `parts`.
+template <typename T>
+int select_rows(RowArgs a, void* scratch, int64_t rows, cudaStream_t stream) {
+    const int64_t lists = rows * a.splits;
+    u64* keys = (u64*)scratch;
+    Part* parts = (Part*)(keys + lists * a.n);
+    u64* joined_keys = (u64*)(parts + lists);
+    Part* joined_parts = (Part*)(joined_keys + rows * a.n);
+    RowArgs rows_args = a;
+    rows_args.keys = keys;
+    rows_args.parts = parts;
+    if (a.splits == 1) {
+        if (a.ids == nullptr) { rows_args.keys = joined_keys; rows_args.parts = joined_parts; }
+        launch_rows<T>(rows_args, rows, stream);
+        PCX_LAUNCH_CHECK();
+        return 0;
     }
+    rows_args.ids = nullptr;
+    launch_rows<T>(rows_args, rows, stream);
+    PCX_LAUNCH_CHECK();
+    a.keys = joined_keys;
+    a.parts = joined_parts;
+    join_parts_kernel<T><<<(unsigned)rows, kThreads, 0, stream>>>(a, keys, parts);
     PCX_LAUNCH_CHECK();
     return 0;
+}
+int select_rows(const RowArgs& a, int dtype, void* scratch, int64_t rows, cudaStream_t stream) {
+    switch (dtype) {
+        case 0: return select_rows<float>(a, scratch, rows, stream);
+        case 1: return select_rows<__nv_bfloat16>(a, scratch, rows, stream);
+        case 2: return select_rows<__half>(a, scratch, rows, stream);
+        default: return -1;
+    }
 }
 
 }  // namespace
 
 extern "C" {
 
-// CTAs per row: enough to give every SM four, none of less than one tile.
+// CTAs per row: enough to give every SM four, none of less than 4096 logits.
 int pcx_vocab_splits(int64_t rows, int64_t vocab) {
     if (rows <= 0 || vocab <= 0) return 1;
     const int64_t want = pcx_cdiv((int64_t)sm_count() * 4, rows);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(want, pcx_cdiv(vocab, kTile)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, pcx_cdiv(vocab, 4096), kMaxSplits}));
 }
 
 int64_t pcx_vocab_scratch_bytes(int64_t rows, int splits, int n) {
-    return rows * splits * ((int64_t)n * 8 + (int64_t)sizeof(Part));
+    return rows * (splits + 1) * ((int64_t)n * 8 + (int64_t)sizeof(Part));
 }
 
 int pcx_top_logits(int64_t* ids, void* values, float* norms, void* scratch, const void* logits, int dtype, int64_t rows,
                    int vocab, int64_t row_stride, int n, int splits, double temperature, void* stream) {
     if (rows <= 0 || n <= 0) return 0;
-    if (n > kMaxTop || vocab <= 0 || splits < 1 || rows * splits > 0x7fffffff) return -1;
+    if (n > kMaxTop || vocab <= 0 || splits < 1 || splits > kMaxSplits || rows * splits > 0x7fffffff) return -1;
     RowArgs a{};
     a.logits = logits;
-    a.stride0 = 0;
     a.stride1 = row_stride;
     a.inner = 0x7fffffff;
     a.vocab = vocab; a.n = n; a.splits = splits;
     a.inv_t = 1.0 / temperature;
     a.scale = (float)(1.4426950408889634 / temperature);
-    if (splits == 1) { a.ids = ids; a.values = values; a.norms = norms; }
-    a.keys = (u64*)scratch;
-    a.parts = (Part*)((char*)scratch + rows * splits * n * 8);
-    const int rc = launch_rows(a, dtype, rows, (cudaStream_t)stream);
-    if (rc != 0 || splits == 1) return rc;
-    JoinArgs j{};
-    j.keys = a.keys; j.parts = a.parts;
-    j.ids = ids; j.values = values; j.norms = norms;
-    j.rows = 1; j.splits = splits; j.n = n; j.vocab = vocab; j.inv_t = a.inv_t;
-    j.elsize = dtype == 0 ? 4 : dtype == 1 ? 2 : 3;
-    join_kernel<<<(unsigned)rows, kThreads, 8, (cudaStream_t)stream>>>(j);
-    PCX_LAUNCH_CHECK();
-    return 0;
+    a.ids = ids; a.values = values; a.norms = norms;
+    return select_rows(a, dtype, scratch, rows, (cudaStream_t)stream);
 }
 
 int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* scratch, const void* logits, int dtype,
                     const float* scores, const uint8_t* finished, int64_t batch, int beams, int vocab, int64_t stride_batch,
                     int64_t stride_beam, int n, int pad_id, int normalize, int splits, void* stream) {
     if (batch <= 0 || n <= 0) return 0;
-    if (n > kMaxTop || vocab <= 0 || beams <= 0 || beams > kMaxTop || splits < 1 || (int64_t)beams * vocab > 0x7fffffff ||
-        batch * beams * splits > 0x7fffffff)
+    const int64_t rows = batch * beams;
+    if (n > kMaxTop || vocab <= 0 || beams <= 0 || beams > kMaxTop || splits < 1 || splits > kMaxSplits ||
+        (int64_t)beams * vocab > 0x7fffffff || rows * splits > 0x7fffffff)
         return -1;
     RowArgs a{};
     a.logits = logits; a.scores = scores; a.finished = finished;
@@ -467,16 +618,15 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
     a.inner = beams; a.vocab = vocab; a.n = n; a.splits = splits;
     a.inv_t = 1.0;
     a.scale = 1.4426950408889634f;
-    const int64_t rows = batch * beams;
-    a.keys = (u64*)scratch;
-    a.parts = (Part*)((char*)scratch + rows * splits * a.n * 8);
-    const int rc = launch_rows(a, dtype, rows, (cudaStream_t)stream);
+    const int rc = select_rows(a, dtype, scratch, rows, (cudaStream_t)stream);
     if (rc != 0) return rc;
-    JoinArgs j{};
-    j.keys = a.keys; j.parts = a.parts; j.scores = scores; j.finished = finished;
-    j.out_scores = out_scores; j.ids = tokens; j.parents = parents;
-    j.rows = beams; j.splits = splits; j.n = n; j.vocab = vocab; j.pad_id = pad_id; j.normalize = normalize; j.inv_t = 1.0;
-    join_kernel<<<(unsigned)batch, kThreads, beams * 8, (cudaStream_t)stream>>>(j);
+    BeamArgs j{};
+    j.keys = (const u64*)((const char*)scratch + rows * splits * ((int64_t)n * 8 + (int64_t)sizeof(Part)));
+    j.parts = (const Part*)(j.keys + rows * n);
+    j.scores = scores; j.finished = finished;
+    j.out_scores = out_scores; j.tokens = tokens; j.parents = parents;
+    j.beams = beams; j.n = n; j.vocab = vocab; j.pad_id = pad_id; j.normalize = normalize;
+    join_beams_kernel<<<(unsigned)batch, kThreads, 0, (cudaStream_t)stream>>>(j);
     PCX_LAUNCH_CHECK();
     return 0;
 }
