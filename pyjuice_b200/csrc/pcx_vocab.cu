@@ -86,6 +86,17 @@ template <> struct Pack<__half> {
     }
 };
 
+// The 16 bytes of elements e ... of a row; -inf beyond its ends.
+template <typename T>
+__device__ __forceinline__ uint4 load_group(const T* x, int e, int vocab) {
+    constexpr int VE = Pack<T>::N;
+    if (e >= 0 && e + VE <= vocab) return __ldcs((const uint4*)(x + e));
+    T edge[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) edge[i] = e + i >= 0 && e + i < vocab ? x[e + i] : (T)PCX_NEG_INF;
+    return *(const uint4*)edge;
+}
+
 struct RowArgs {
     const void* logits;
     const float* scores;           // beams: [rows], a row whose score is -inf or NaN is skipped; null = none
@@ -109,7 +120,7 @@ __device__ __forceinline__ double log_norm(float m, double s, double inv_t) {
 }
 
 struct Shared {
-    u64 keys[kRoom + kMaxTop];     // the list (sorted, first), behind it the candidates of a tile
+    alignas(16) u64 keys[kRoom + kMaxTop];     // the list (sorted, first), behind it the candidates of a tile
     u64 list[kMaxTop];
     float red_m[kWarps];
     double red_s[kWarps];
@@ -169,7 +180,11 @@ __device__ int prune(Shared& sh, int total, int n) {
     for (int i = tid; i < total; i += kThreads) {
         const u64 k = sh.keys[i];
         int rank = 0;
-        for (int j = 0; j < total; ++j) rank += sh.keys[j] > k;
+        for (int j = 0; j < (total & ~1); j += 2) {
+            const ulonglong2 o = *(const ulonglong2*)(sh.keys + j);
+            rank += (o.x > k) + (o.y > k);
+        }
+        if (total & 1) rank += sh.keys[total - 1] > k;
         if (rank < n) sh.list[rank] = k;
     }
     __syncthreads();
@@ -178,21 +193,19 @@ __device__ int prune(Shared& sh, int total, int n) {
     return kept;
 }
 
-// Statistics of a block: maximum and sum of all threads' (m, s), to every thread.
+// Statistics of a block: maximum and sum of all warps' (m, s), to every thread.
 __device__ __forceinline__ void block_stats(Shared& sh, float m, double s, double inv_t, float& M, double& S) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    M = m;
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    if (lane == 0) sh.red_m[warp] = M;
+    if (lane == 0) { sh.red_m[warp] = m; sh.red_s[warp] = s; }
     __syncthreads();
     M = sh.red_m[0];
+#pragma unroll
     for (int w = 1; w < kWarps; ++w) M = fmaxf(M, sh.red_m[w]);
-    S = m > PCX_NEG_INF && M < CUDART_INF_F ? s * exp((double)(m - M) * inv_t) : 0.0;
-    for (int o = 16; o; o >>= 1) S += __shfl_xor_sync(~0u, S, o);
-    if (lane == 0) sh.red_s[warp] = S;
-    __syncthreads();
     S = 0.0;
-    for (int w = 0; w < kWarps; ++w) S += sh.red_s[w];
+    if (threadIdx.x == 0 && M > PCX_NEG_INF && M < CUDART_INF_F)
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+            if (sh.red_m[w] > PCX_NEG_INF) S += sh.red_s[w] * exp((double)(sh.red_m[w] - M) * inv_t);
 }
 
 // An answer of top logits, or a part of one.
@@ -240,20 +253,14 @@ top_rows_kernel(RowArgs a) {
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 const int gi = g + j * kThreads + tid;
-                const int e = gi * VE - off;
-                if (gi < g1 && e >= 0 && e + VE <= a.vocab) {
-                    v[j] = __ldcs((const uint4*)(x + e));
-                } else {
-                    T edge[VE];
-#pragma unroll
-                    for (int i = 0; i < VE; ++i)
-                        edge[i] = gi < g1 && e + i >= 0 && e + i < a.vocab ? x[e + i] : (T)PCX_NEG_INF;
-                    v[j] = *(const uint4*)edge;
-                }
+                v[j] = load_group<T>(x, gi < g1 ? gi * VE - off : -VE, a.vocab);
             }
-            float top = PCX_NEG_INF;
+            float top = PCX_NEG_INF, group_top[G];
 #pragma unroll
-            for (int j = 0; j < G; ++j) top = fmaxf(top, Pack<T>::max(v[j]));
+            for (int j = 0; j < G; ++j) {
+                group_top[j] = Pack<T>::max(v[j]);
+                top = fmaxf(top, group_top[j]);
+            }
             if (top > m) {
                 const float nr = top * a.scale;
                 const bool plain = fabsf(r) < CUDART_INF_F && fabsf(nr) < CUDART_INF_F;
@@ -283,42 +290,42 @@ top_rows_kernel(RowArgs a) {
                 }
                 s += s0;
             }
-            if (!__syncthreads_or(top > bound)) continue;
-            // A lower bound of the tile's n-th largest logit: every warp's (n / warps)-th largest thread maximum, the
-            // smallest of them (at least n threads hold one that large)
-            uint32_t k = ordered(top);
+            const int over = __syncthreads_count(top > bound);
+            if (over == 0) continue;
+            float least = PCX_NEG_INF;
+            if (over > 2 * a.n) {
+                // A lower bound of the tile's n-th largest logit: every warp's (n / warps)-th largest thread maximum, the
+                // smallest of them (at least n threads hold one that large)
+                uint32_t k = ordered(top);
 #pragma unroll
-            for (int size = 2; size <= 32; size <<= 1)
+                for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-                for (int o = size >> 1; o; o >>= 1) {
-                    const uint32_t other = __shfl_xor_sync(~0u, k, o);
-                    const bool up = ((lane & size) == 0) == ((lane & o) == 0);       // larger first
-                    k = up ? max(k, other) : min(k, other);
-                }
-            const int nth = (a.n + kWarps - 1) / kWarps - 1;
-            if (lane == nth) sh.warp_t[warp] = k;
-            __syncthreads();
-            uint32_t t = sh.warp_t[0];
+                    for (int o = size >> 1; o; o >>= 1) {
+                        const uint32_t other = __shfl_xor_sync(~0u, k, o);
+                        const bool up = ((lane & size) == 0) == ((lane & o) == 0);       // larger first
+                        k = up ? max(k, other) : min(k, other);
+                    }
+                if (lane == (a.n + kWarps - 1) / kWarps - 1) sh.warp_t[warp] = k;
+                __syncthreads();
+                uint32_t t = sh.warp_t[0];
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) t = min(t, sh.warp_t[w]);
-            const float least = unordered(t);
+                for (int w = 1; w < kWarps; ++w) t = min(t, sh.warp_t[w]);
+                least = unordered(t);
+            }
             // every logit that may be among the n largest so far, read again (its group is among the few that hold one);
             // `from`: a key below which none is wanted
             uint32_t hot = 0;
             if (top > bound && top >= least) {
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    const float gm = Pack<T>::max(v[j]);
-                    hot |= (uint32_t)(gm > bound && gm >= least) << j;
-                }
+                for (int j = 0; j < G; ++j) hot |= (uint32_t)(group_top[j] > bound && group_top[j] >= least) << j;
             }
             auto each = [&](u64 from, auto&& found) {
                 for (uint32_t left = hot; left != 0; left &= left - 1) {
                     const int e = (g + (__ffs(left) - 1) * kThreads + tid) * VE - off;
+                    const uint4 w = load_group<T>(x, e, a.vocab);
 #pragma unroll
                     for (int i = 0; i < VE; ++i) {
-                        if (e + i < 0 || e + i >= a.vocab) continue;
-                        const float f = (float)x[e + i];
+                        const float f = Pack<T>::at(w, i);
                         if (f > bound && f >= least) {
                             const u64 key = key_of(f, (uint32_t)(e + i));
                             if (key >= from) found(key);
@@ -352,10 +359,19 @@ top_rows_kernel(RowArgs a) {
             if (have == a.n) bound = value_of(sh.keys[a.n - 1]);
         }
     }
+    // a warp's statistics in fp32 ...
+    float wm = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(~0u, wm, o));
+    const float wr = wm * a.scale;
+    const bool plain = fabsf(wr) < CUDART_INF_F;
+    s = m > PCX_NEG_INF ? s * exp2_fast(plain && fabsf(r) < CUDART_INF_F ? r - wr : (m - wm) * a.scale) : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    // ... and those of the warps in 64 bits
     float M;
     double S;
-    const double off_by = fabsf(r) < CUDART_INF_F ? (double)r - (double)m * (double)a.scale : 0.0;
-    block_stats(sh, m, m > PCX_NEG_INF ? (double)s * exp2(off_by) : 0.0, a.inv_t, M, S);
+    block_stats(sh, wm, plain ? (double)s * (1.0 + (double)fmaf(-wm, a.scale, wr) * 0.6931471805599453) : (double)s, a.inv_t, M, S);
     leave<T>(a, sh, row, have, M, S);
 }
 
@@ -372,9 +388,15 @@ join_parts_kernel(RowArgs a, const u64* keys, const Part* parts) {
     __syncthreads();
     float m = PCX_NEG_INF;
     double s = 0.0;
-    if (tid < a.splits) {
-        m = parts[row * a.splits + tid].m;
-        s = parts[row * a.splits + tid].s;
+    if (tid < 32) {                                 // (kMaxSplits parts at most)
+        if (tid < a.splits) { m = parts[row * a.splits + tid].m; s = parts[row * a.splits + tid].s; }
+        float wm = m;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(~0u, wm, o));
+        s = m > PCX_NEG_INF && wm < CUDART_INF_F ? s * exp((double)(m - wm) * a.inv_t) : 0.0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+        m = wm;
     }
     for (int i = tid; i < a.splits * a.n; i += kThreads)
         if (i % a.n < parts[row * a.splits + i / a.n].count)
@@ -444,8 +466,9 @@ join_beams_kernel(BeamArgs a) {
         __syncthreads();
         int total = sh.count;
         __syncthreads();
-        if (total > kFew) {
-            const u64 t = bisect(a.n, kFew, &sh.count, [&](u64 mid) {
+        const int few = max(64, 2 * a.n);
+        if (total > few) {
+            const u64 t = bisect(a.n, few, &sh.count, [&](u64 mid) {
                 int c = 0;
                 for (int i = tid; i < total; i += kThreads) c += sh.score[i] >= mid;
                 return c;
@@ -470,7 +493,7 @@ join_beams_kernel(BeamArgs a) {
             int rank = 0;
             for (int j = 0; j < total; ++j) {
                 const u64 o = sh.score[j];
-                rank += o > s || (o == s && sh.place[j] < p);
+                rank += (int)(o > s) | ((int)(o == s) & (int)(sh.place[j] < p));
             }
             if (rank < a.n) { sh.list_s[rank] = s; sh.list_p[rank] = p; }
         }
