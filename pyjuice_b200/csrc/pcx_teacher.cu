@@ -72,8 +72,10 @@ struct PrepArgs {
     double inv_t64;
 };
 
-// One warp per position.
+// One warp per position; up to 4 slots a lane stay in registers, more are read again.  Slots that say something come first, in
+// their order: what reads them stops at the first empty one.
 __global__ void __launch_bounds__(kTh) teacher_prep_kernel(PrepArgs a) {
+    constexpr int HELD = 4;
     const int64_t at = (int64_t)blockIdx.x * kW + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (at >= (int64_t)a.V * a.W) return;
@@ -84,41 +86,50 @@ __global__ void __launch_bounds__(kTh) teacher_prep_kernel(PrepArgs a) {
         return;
     }
     auto slot = [&](int k, int& id, float& x) {
+        id = -1;
+        x = PCX_NEG_INF;
+        if (k >= a.K) return;
         const int64_t i = b * a.ib + v * a.iv + k * a.ik;
         const int64_t wide = a.wide_ids ? ((const int64_t*)a.ids)[i] : (int64_t)((const int32_t*)a.ids)[i];
-        x = load_logit(a.logits, a.dtype, b * a.lb + v * a.lv + k * a.lk);
-        if (wide < 0 || !(x > PCX_NEG_INF)) { id = -1; x = PCX_NEG_INF; }
-        else id = (int)min(wide, (int64_t)0x7fffffff);
+        const float y = load_logit(a.logits, a.dtype, b * a.lb + v * a.lv + k * a.lk);
+        if (wide >= 0 && y > PCX_NEG_INF) { id = (int)min(wide, (int64_t)0x7fffffff); x = y; }
     };
-    float m = PCX_NEG_INF;
-    for (int k = lane; k < a.K; k += 32) {
-        int id; float x;
-        slot(k, id, x);
-        m = fmaxf(m, x);
-    }
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    int ids[HELD];
+    float xs[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) slot(lane + 32 * i, ids[i], xs[i]);
+    auto each = [&](auto&& f) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i)
+            if (32 * i < a.K) f(ids[i], xs[i]);
+        for (int k0 = 32 * HELD; k0 < a.K; k0 += 32) {
+            int id; float x;
+            slot(k0 + lane, id, x);
+            f(id, x);
+        }
+    };
     const float norm = a.norms != nullptr ? a.norms[b * a.nb + v * a.nv] : CUDART_INF_F;
     const bool given = fabsf(norm) < CUDART_INF_F;
+    float m = PCX_NEG_INF, sum = 0.0f;
+    each([&](int, float x) { m = fmaxf(m, x); });
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     auto raw = [&](float x) {
         if (x == PCX_NEG_INF) return 0.0f;
         if (given) return expf((float)((double)x * a.inv_t64 - (double)norm));
         return x == m ? 1.0f : expf((x - m) * a.inv_t);          // (+inf logits share the weight)
     };
-    float sum = 0.0f;
     if (!given) {
-        for (int k = lane; k < a.K; k += 32) {
-            int id; float x;
-            slot(k, id, x);
-            sum += raw(x);
-        }
+        each([&](int, float x) { sum += raw(x); });
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     }
-    for (int k = lane; k < a.K; k += 32) {
-        int id; float x;
-        slot(k, id, x);
+    int count = 0;
+    each([&](int id, float x) {
         const float q = given ? raw(x) : sum > 0.0f ? raw(x) / sum : 0.0f;
-        out[k] = make_int2(q > 0.0f ? id : -1, __float_as_int(q));
-    }
+        const unsigned says = __ballot_sync(~0u, id >= 0 && q > 0.0f);
+        if (id >= 0 && q > 0.0f) out[count + __popc(says & ((1u << lane) - 1))] = make_int2(id, __float_as_int(q));
+        count += __popc(says);
+    });
+    for (int k = count + lane; k < a.K; k += 32) out[k] = make_int2(-1, 0);
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -131,29 +142,33 @@ struct FwdArgs {
     int take_log, m_tiles, per_b;
 };
 
-// Few slots, or tables of a single node: the table is read where it lies.  Eight lanes share an output.
+// Few slots, or tables of a single node: the table is read where it lies.  Eight lanes share an output; the outputs of the
+// same nodes at all positions run side by side, since their reads meet in the same parts of the table.
 __global__ void __launch_bounds__(kTh) teacher_fwd_direct_kernel(FwdArgs a) {
-    const int s = blockIdx.x / a.m_tiles;
+    const int64_t task = (int64_t)blockIdx.x * (kTh / 8) + (threadIdx.x >> 3);
+    const int W = a.g.W, s = (int)(task / W % a.g.n_segs), b = (int)(task % W);
+    const int m = (int)(task / W / a.g.n_segs);
+    if (m >= a.g.M) return;
     const Seg seg = seg_of(a.g, s);
-    const int64_t o = (int64_t)(blockIdx.x % a.m_tiles) * (kTh / 8) + (threadIdx.x >> 3);
-    if (o >= (int64_t)seg.M * a.g.W) return;
+    if (m >= seg.M) return;
     const int sub = threadIdx.x & 7;
-    const int m = (int)(o / a.g.W), b = (int)(o % a.g.W);
     const float* row = a.table + seg.table + (int64_t)m * seg.C;
-    const int2* e = a.ent + ((int64_t)seg.var * a.g.W + b) * a.g.K;
+    const int2* e = a.ent + ((int64_t)seg.var * W + b) * a.g.K;
     float acc = 0.0f;
-#pragma unroll 4
-    for (int k = sub; k < a.g.K; k += 8) {
-        const int2 x = __ldg(e + k);
-        if (x.x >= 0) {
-            float v = x.x < seg.C ? __ldg(row + x.x) : a.take_log ? 0.0f : PCX_NEG_INF;
-            if (a.take_log) v = logf(v);
-            acc = fmaf(__int_as_float(x.y), v, acc);
-        }
+    for (int k0 = 0; k0 < a.g.K; k0 += 64) {
+        int2 x[8];
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = k0 + 8 * i + sub < a.g.K ? __ldg(e + k0 + 8 * i + sub) : make_int2(-1, 0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = x[i].x >= 0 && x[i].x < seg.C ? __ldg(row + x[i].x) : a.take_log ? 0.0f : PCX_NEG_INF;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (x[i].x >= 0) acc = fmaf(__int_as_float(x[i].y), a.take_log ? logf(v[i]) : v[i], acc);
     }
     const unsigned mask = 0xffu << (threadIdx.x & 24);
     for (int off = 4; off; off >>= 1) acc += __shfl_xor_sync(mask, acc, off);
-    if (sub == 0) a.out[(seg.row0 + m) * a.g.W + b] = acc;
+    if (sub == 0) a.out[(seg.row0 + m) * W + b] = acc;
 }
 
 // NM * 32 nodes of one vector; a warp takes one position at a time, its lanes the nodes.  SRC 0: the turned table, four
@@ -165,13 +180,15 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_kernel(FwdArgs a) {
     float* tile = sm;                                  // [MT][33]
     float* part = sm + MT * 33;                        // [C][MT + 1]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const Seg seg = seg_of(a.g, blockIdx.x / a.m_tiles);
-    const int m0 = (blockIdx.x % a.m_tiles) * MT;
+    // (turned tables: the same nodes of all positions run side by side, so that their part of the table stays in L2)
+    const Seg seg = seg_of(a.g, SRC == 2 ? blockIdx.x / a.m_tiles : blockIdx.x % a.g.n_segs);
+    const int m0 = (SRC == 2 ? blockIdx.x % a.m_tiles : blockIdx.x / a.g.n_segs) * MT;
     if (m0 >= seg.M) return;
     const int W = a.g.W, K = a.g.K;
     if constexpr (SRC == 2) {
         for (int m = warp; m < MT; m += kW) {
             const float* row = a.table + seg.table + (int64_t)(m0 + m) * seg.C;
+#pragma unroll 4
             for (int c = lane; c < seg.C; c += 32) {
                 float v = m0 + m < seg.M ? row[c] : 1.0f;
                 if (a.take_log) v = logf(v);
@@ -188,30 +205,36 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_kernel(FwdArgs a) {
             if (b >= b_end) break;
             const int2* e = a.ent + ((int64_t)seg.var * W + b) * K;
             float acc[NM] = {};
+            bool beyond = false;                       // a category that the table does not have
+            for (int k0 = 0; k0 < K; k0 += 32) {
+                const int id = k0 + lane < K ? __ldg(e + k0 + lane).x : -1;
+                const int n = __popc(__ballot_sync(~0u, id >= 0));
+                beyond |= __any_sync(~0u, id >= seg.C);
 #pragma unroll 8
-            for (int k = 0; k < K; ++k) {
-                const int2 x = __ldg(e + k);
-                if (x.x < 0) continue;
-                const float q = __int_as_float(x.y);
-                if (x.x >= seg.C) {
+                for (int k = k0; k < k0 + n; ++k) {
+                    const int2 x = __ldg(e + k);
+                    const int c = min(x.x, seg.C - 1);
+                    const float q = __int_as_float(x.y);
+                    if constexpr (SRC == 0) {
+                        if (m0 + lane * 4 < seg.M) {
+                            const float4 v = __ldg((const float4*)(base + (int64_t)c * a.R) + lane);
+                            acc[0] = fmaf(q, v.x, acc[0]); acc[1] = fmaf(q, v.y, acc[1]);
+                            acc[2] = fmaf(q, v.z, acc[2]); acc[3] = fmaf(q, v.w, acc[3]);
+                        }
+                    } else if constexpr (SRC == 1) {
 #pragma unroll
-                    for (int i = 0; i < NM; ++i) acc[i] = PCX_NEG_INF;
-                    continue;
-                }
-                if constexpr (SRC == 0) {
-                    if (m0 + lane * 4 < seg.M) {
-                        const float4 v = __ldg((const float4*)(base + (int64_t)x.x * a.R) + lane);
-                        acc[0] = fmaf(q, v.x, acc[0]); acc[1] = fmaf(q, v.y, acc[1]);
-                        acc[2] = fmaf(q, v.z, acc[2]); acc[3] = fmaf(q, v.w, acc[3]);
+                        for (int i = 0; i < NM; ++i)
+                            if (m0 + lane + 32 * i < seg.M) acc[i] = fmaf(q, __ldg(base + (int64_t)c * a.R + lane + 32 * i), acc[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < NM; ++i) acc[i] = fmaf(q, part[c * (MT + 1) + lane + 32 * i], acc[i]);
                     }
-                } else if constexpr (SRC == 1) {
-#pragma unroll
-                    for (int i = 0; i < NM; ++i)
-                        if (m0 + lane + 32 * i < seg.M) acc[i] = fmaf(q, __ldg(base + (int64_t)x.x * a.R + lane + 32 * i), acc[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < NM; ++i) acc[i] = fmaf(q, part[x.x * (MT + 1) + lane + 32 * i], acc[i]);
                 }
+                if (n < 32) break;
+            }
+            if (beyond) {
+#pragma unroll
+                for (int i = 0; i < NM; ++i) acc[i] = PCX_NEG_INF;
             }
 #pragma unroll
             for (int i = 0; i < NM; ++i) tile[(SRC == 0 ? lane * 4 + i : lane + 32 * i) * 33 + warp * 4 + j] = acc[i];
@@ -224,52 +247,96 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_kernel(FwdArgs a) {
 }
 
 // ---- turning -----------------------------------------------------------------------------------------------------------
-// [R][C] -> [C][stride], of logarithms if asked.
+// 64 x 64 tiles; a thread reads and writes four neighbours at a time where rows allow it (VEC).
+constexpr int kTurn = 64;
+
+// out[c][r] = value(r, c) for r < n_r, c < n_c of a tile, 0 for n_r <= r < pad_r.  `in` and `out` point at the tile.
+template <bool VEC_IN, bool VEC_OUT, typename F>
+__device__ __forceinline__ void turn_tile(float (*tile)[kTurn + 1], const float* in, int64_t in_stride, int n_r, int n_c, float* out,
+                                          int64_t out_stride, int pad_r, F value) {
+    const int q = (threadIdx.x & 15) * 4, y = threadIdx.x >> 4;
+    float4 v[kTurn / 16];
+#pragma unroll
+    for (int i = 0; i < kTurn / 16; ++i) {
+        const int r = y + 16 * i;
+        const float* p = in + r * in_stride + q;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n_r) {
+            if (VEC_IN && q + 4 <= n_c) v[i] = *(const float4*)p;
+            else {
+                if (q < n_c) v[i].x = p[0];
+                if (q + 1 < n_c) v[i].y = p[1];
+                if (q + 2 < n_c) v[i].z = p[2];
+                if (q + 3 < n_c) v[i].w = p[3];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kTurn / 16; ++i) {
+        const int r = y + 16 * i;
+        tile[r][q] = v[i].x; tile[r][q + 1] = v[i].y; tile[r][q + 2] = v[i].z; tile[r][q + 3] = v[i].w;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kTurn / 16; ++i) {
+        const int c = y + 16 * i;
+        if (c >= n_c || q >= pad_r) continue;
+        float o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = q + k < n_r ? value(tile[q + k][c]) : 0.0f;
+        float* p = out + c * out_stride + q;
+        if (VEC_OUT && q + 4 <= pad_r) *(float4*)p = make_float4(o[0], o[1], o[2], o[3]);
+        else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (q + k < pad_r) p[k] = o[k];
+        }
+    }
+}
+
+// [R][C] -> [C][stride].
+template <bool VEC_IN, bool VEC_OUT>
 __global__ void __launch_bounds__(kTh) teacher_turn_kernel(float* __restrict__ out, const float* __restrict__ in, int64_t R, int C,
                                                           int64_t stride, int64_t r_tiles) {
-    __shared__ float tile[32][33];
-    const int64_t r0 = (int64_t)(blockIdx.x % r_tiles) * 32;
-    const int c0 = (int)(blockIdx.x / r_tiles) * 32;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int k = ty; k < 32; k += kW) tile[k][tx] = r0 + k < R && c0 + tx < C ? in[(r0 + k) * C + c0 + tx] : 0.0f;
-    __syncthreads();
-    for (int k = ty; k < 32; k += kW)
-        if (c0 + k < C && r0 + tx < stride) out[(c0 + k) * stride + r0 + tx] = tile[tx][k];
+    __shared__ float tile[kTurn][kTurn + 1];
+    const int64_t r0 = (int64_t)(blockIdx.x % r_tiles) * kTurn;
+    const int c0 = (int)(blockIdx.x / r_tiles) * kTurn;
+    turn_tile<VEC_IN, VEC_OUT>(tile, in + r0 * C + c0, C, (int)max((int64_t)0, min((int64_t)kTurn, R - r0)), min(kTurn, C - c0),
+                               out + c0 * stride + r0, stride, (int)min((int64_t)kTurn, stride - r0), [](float v) { return v; });
 }
 
 // Flows [node][sample] -> [sample][node] of every vector, exponentials if they are logarithms; padding nodes are 0.
+template <bool VEC_IN>
 __global__ void __launch_bounds__(kTh) teacher_turn_flows_kernel(float* __restrict__ out, const float* __restrict__ flows, Geo g,
                                                                 int m_tiles, int logspace) {
-    __shared__ float tile[32][33];
+    __shared__ float tile[kTurn][kTurn + 1];
     const Seg seg = seg_of(g, blockIdx.x / m_tiles);
-    const int m0 = (blockIdx.x % m_tiles) * 32, b0 = blockIdx.y * 32, mp = pad4(seg.M);
+    const int m0 = (blockIdx.x % m_tiles) * kTurn, b0 = blockIdx.y * kTurn, mp = pad4(seg.M);
     if (m0 >= seg.M) return;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int k = ty; k < 32; k += kW) {
-        float v = 0.0f;
-        if (m0 + k < seg.M && b0 + tx < g.W) {
-            v = flows[(seg.row0 + m0 + k) * g.W + b0 + tx];
-            if (logspace) v = expf(v);
-        }
-        tile[k][tx] = v;
-    }
-    __syncthreads();
-    for (int k = ty; k < 32; k += kW)
-        if (b0 + k < g.W && m0 + tx < mp) out[seg.gcol * g.W + (int64_t)(b0 + k) * mp + m0 + tx] = tile[tx][k];
+    turn_tile<VEC_IN, true>(tile, flows + (seg.row0 + m0) * g.W + b0, g.W, min(kTurn, seg.M - m0), min(kTurn, g.W - b0),
+                            out + seg.gcol * g.W + (int64_t)b0 * mp + m0, mp, min(kTurn, mp - m0),
+                            [&](float v) { return logspace ? expf(v) : v; });
 }
 
 // ---- sorting the slots by category -------------------------------------------------------------------------------------
 // Per set of variables: keys (category; C for empty slots) with the slot's place (position in the set * W + sample) and
 // weight, in the order of categories, the slots of a category in their own order.
-constexpr int kSmallSort = 4096, kSortTile = 4096, kDigits = 256, kMaxCats = 1000000;
+// Radix passes of at most 10 bits: the digit counts of the warps (and tiles), their running sums in the order of digits,
+// then every slot moves to its place; slots of one digit keep their order.
+constexpr int kSmallSort = 4096, kSortRounds = 8, kSortTile = kTh * kSortRounds, kMaxCats = 1000000;
 
 struct SortArgs {
     Geo g;
     const int2* ent;
     int32_t* keys;                 // sorted
     int2* slots;                   // sorted: place, weight
-    int32_t *key_a, *key_b, *idx_a, *idx_b, *hist;
-    int C, tiles, shift;
+    int32_t* first;                // [n_sets][C + 1], or null
+    const int32_t* key_in;         // what a pass over tiles reads (null: the entries) ...
+    const int2* slot_in;
+    int32_t* key_out;              // ... and writes
+    int2* slot_out;
+    int32_t *hist, *totals;        // [n_sets][digits][tiles], [n_sets][digits]
+    int C, tiles, shift, bits;
 };
 
 __device__ __forceinline__ int2 set_entry(const Geo& g, const int2* ent, int first, int j) {
@@ -278,118 +345,187 @@ __device__ __forceinline__ int2 set_entry(const Geo& g, const int2* ent, int fir
 }
 __device__ __forceinline__ int key_of_entry(int2 e, int C) { return e.x < 0 || e.x >= C ? C : e.x; }
 
-__global__ void __launch_bounds__(1024) teacher_sort_small_kernel(SortArgs a, int P) {
-    extern __shared__ uint32_t comp[];
-    const int u = blockIdx.x, first = set_begin(a.g, u), N = set_size(a.g, u) * a.g.W * a.g.K;
-    for (int j = threadIdx.x; j < P; j += blockDim.x)
-        comp[j] = j < N ? ((uint32_t)key_of_entry(set_entry(a.g, a.ent, first, j), a.C) << 12) | (uint32_t)j : ~0u;
+// Running sum over the threads of a block (before this thread's own).
+__device__ __forceinline__ int scan_before(int v, int* warp_sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_warps = blockDim.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, x, o); if (lane >= o) x += y; }
+    if (lane == 31) warp_sum[warp] = x;
     __syncthreads();
-    for (int size = 2; size <= P; size <<= 1)
-        for (int step = size >> 1; step; step >>= 1) {
-            for (int i = threadIdx.x; i < P / 2; i += blockDim.x) {
-                const int x = 2 * i - (i & (step - 1)), y = x + step;
-                const uint32_t p = comp[x], q = comp[y];
-                if ((p > q) == ((x & size) == 0)) { comp[x] = q; comp[y] = p; }
-            }
+    int before = x - v;
+    for (int w = 0; w < n_warps; ++w) before += w < warp ? warp_sum[w] : 0;
+    __syncthreads();
+    return before;
+}
+
+// A set of at most 4096 slots: one CTA, 128 slots a warp; a slot is its key and, in the low 12 bits, its number.
+__global__ void __launch_bounds__(1024) teacher_sort_small_kernel(SortArgs a) {
+    extern __shared__ uint32_t sm_sort[];
+    const int n_warps = blockDim.x >> 5, cap = n_warps * 128, D = 1 << a.bits;
+    uint32_t* here = sm_sort;
+    uint32_t* there = here + cap;
+    uint16_t* count = (uint16_t*)(there + cap);        // [n_warps][D]
+    __shared__ int warp_sum[32];
+    const int u = blockIdx.x, first = set_begin(a.g, u), N = set_size(a.g, u) * a.g.W * a.g.K;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int j = tid; j < cap; j += blockDim.x)
+        here[j] = j < N ? ((uint32_t)key_of_entry(set_entry(a.g, a.ent, first, j), a.C) << 12) | (uint32_t)j : ~0u;
+    for (int shift = 12; (a.C >> (shift - 12)) != 0; shift += a.bits) {
+        for (int i = tid; i < n_warps * D / 2; i += blockDim.x) ((uint32_t*)count)[i] = 0;
+        __syncthreads();
+        uint32_t v[4];
+        int rank[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            v[r] = here[warp * 128 + r * 32 + lane];
+            const int d = v[r] == ~0u ? -1 : (int)((v[r] >> shift) & (D - 1));
+            const unsigned same = __match_any_sync(~0u, d);
+            rank[r] = d < 0 ? 0 : count[warp * D + d] + __popc(same & ((1u << lane) - 1));
+            __syncwarp();
+            if (d >= 0 && lane == __ffs(same) - 1) count[warp * D + d] += __popc(same);
+            __syncwarp();
+        }
+        __syncthreads();
+        int run = 0;                                   // digits before those of this round
+        for (int d0 = 0; d0 < D; d0 += blockDim.x) {
+            const int d = d0 + tid;
+            int total = 0;
+            if (d < D)
+                for (int w = 0; w < n_warps; ++w) { const int c = count[w * D + d]; count[w * D + d] = (uint16_t)total; total += c; }
+            const int before = run + scan_before(total, warp_sum);
+            if (d < D)
+                for (int w = 0; w < n_warps; ++w) count[w * D + d] += (uint16_t)before;
+            if (tid == blockDim.x - 1) warp_sum[0] = before + total;
+            __syncthreads();
+            run = warp_sum[0];
             __syncthreads();
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (v[r] != ~0u) there[count[warp * D + ((v[r] >> shift) & (D - 1))] + rank[r]] = v[r];
+        __syncthreads();
+        for (int j = N + tid; j < cap; j += blockDim.x) there[j] = ~0u;
+        uint32_t* t = here; here = there; there = t;
+        __syncthreads();
+    }
     const int64_t base = (int64_t)first * a.g.W * a.g.K;
-    for (int j = threadIdx.x; j < N; j += blockDim.x) {
-        const int at = comp[j] & 4095;
-        a.keys[base + j] = (int)(comp[j] >> 12);
+    for (int j = tid; j < N; j += blockDim.x) {
+        const int at = here[j] & 4095;
+        a.keys[base + j] = (int)(here[j] >> 12);
         a.slots[base + j] = make_int2(at / a.g.K, set_entry(a.g, a.ent, first, at).y);
     }
+    if (a.first != nullptr)
+        for (int c = tid; c <= a.C; c += blockDim.x) {
+            int lo = 0, hi = N;                        // the first slot with a key of at least c
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if ((int)(here[mid] >> 12) < c) lo = mid + 1; else hi = mid;
+            }
+            a.first[(int64_t)u * (a.C + 1) + c] = lo;
+        }
 }
 
-// One pass of a stable radix sort over 8 bits: digit counts of every tile, their running sums, the move.
+template <bool FIRST>
+__device__ __forceinline__ int sort_key(const SortArgs& a, int first, int64_t base, int j) {
+    return FIRST ? key_of_entry(set_entry(a.g, a.ent, first, j), a.C) : a.key_in[base + j];
+}
+
 template <bool FIRST>
 __global__ void __launch_bounds__(kTh) teacher_hist_kernel(SortArgs a) {
-    __shared__ int count[kDigits];
-    const int u = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+    __shared__ int count[1024];
+    const int u = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles, D = 1 << a.bits;
     const int first = set_begin(a.g, u), N = set_size(a.g, u) * a.g.W * a.g.K;
     const int64_t base = (int64_t)first * a.g.W * a.g.K;
-    for (int d = threadIdx.x; d < kDigits; d += kTh) count[d] = 0;
+    for (int d = threadIdx.x; d < D; d += kTh) count[d] = 0;
     __syncthreads();
-    for (int j = tile * kSortTile + threadIdx.x; j < min(N, (tile + 1) * kSortTile); j += kTh) {
-        const int k = FIRST ? key_of_entry(set_entry(a.g, a.ent, first, j), a.C) : a.key_a[base + j];
-        atomicAdd(&count[(k >> a.shift) & (kDigits - 1)], 1);
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+        const int j = tile * kSortTile + r * kTh + threadIdx.x;
+        if (j < N) atomicAdd(&count[(sort_key<FIRST>(a, first, base, j) >> a.shift) & (D - 1)], 1);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kTh) a.hist[((int64_t)u * kDigits + d) * a.tiles + tile] = count[d];
+    for (int d = threadIdx.x; d < D; d += kTh) a.hist[((int64_t)u * D + d) * a.tiles + tile] = count[d];
 }
 
-__global__ void __launch_bounds__(1024) teacher_scan_kernel(int32_t* hist, int n) {
-    __shared__ int warp_sum[32];
-    int32_t* h = hist + (int64_t)blockIdx.x * n;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// One warp per set and digit: running sums over the tiles, and the digit's total.
+__global__ void __launch_bounds__(kTh) teacher_scan_kernel(int32_t* hist, int32_t* totals, int64_t n, int tiles) {
+    const int64_t at = (int64_t)blockIdx.x * kW + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (at >= n) return;
+    int32_t* h = hist + at * tiles;
     int carry = 0;
-    for (int i0 = 0; i0 < n; i0 += 1024) {
-        const int i = i0 + threadIdx.x;
-        const int v = i < n ? h[i] : 0;
+    for (int i0 = 0; i0 < tiles; i0 += 32) {
+        const int v = i0 + lane < tiles ? h[i0 + lane] : 0;
         int x = v;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, x, o); if (lane >= o) x += y; }
-        if (lane == 31) warp_sum[warp] = x;
-        __syncthreads();
-        if (warp == 0) {
-            int w = warp_sum[lane];
-            for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, w, o); if (lane >= o) w += y; }
-            warp_sum[lane] = w;
-        }
-        __syncthreads();
-        const int before = carry + (warp > 0 ? warp_sum[warp - 1] : 0) + x - v;
-        carry += warp_sum[31];
-        if (i < n) h[i] = before;
-        __syncthreads();
+        if (i0 + lane < tiles) h[i0 + lane] = carry + x - v;
+        carry += __shfl_sync(~0u, x, 31);
     }
+    if (lane == 0) totals[at] = carry;
 }
 
-template <bool FIRST, bool LAST>
+template <bool FIRST>
 __global__ void __launch_bounds__(kTh) teacher_move_kernel(SortArgs a) {
-    __shared__ int count[kW][kDigits];
-    const int u = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+    extern __shared__ int sm_move[];                   // [kW][D]
+    __shared__ int warp_sum[32];
+    const int u = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles, D = 1 << a.bits;
     const int first = set_begin(a.g, u), N = set_size(a.g, u) * a.g.W * a.g.K;
     if (tile * kSortTile >= N) return;
     const int64_t base = (int64_t)first * a.g.W * a.g.K;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int ROUNDS = kSortTile / kTh;
-    for (int i = threadIdx.x; i < kW * kDigits; i += kTh) (&count[0][0])[i] = 0;
-    __syncthreads();
-    const int j0 = tile * kSortTile + warp * (kSortTile / kW);
-    int key[ROUNDS];
+    int* count = sm_move + warp * D;
+    for (int i = threadIdx.x; i < kW * D; i += kTh) sm_move[i] = 0;
+    const int j0 = tile * kSortTile + warp * (32 * kSortRounds) + lane;
+    int key[kSortRounds], rank[kSortRounds];
+    int2 slot[kSortRounds];
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const int j = j0 + r * 32 + lane;
+    for (int r = 0; r < kSortRounds; ++r) {
+        const int j = j0 + r * 32;
         key[r] = -1;
         if (j < N) {
-            key[r] = FIRST ? key_of_entry(set_entry(a.g, a.ent, first, j), a.C) : a.key_a[base + j];
-            atomicAdd(&count[warp][(key[r] >> a.shift) & (kDigits - 1)], 1);
+            if constexpr (FIRST) {
+                const int2 e = set_entry(a.g, a.ent, first, j);
+                key[r] = key_of_entry(e, a.C);
+                slot[r] = make_int2(j / a.g.K, e.y);
+            } else {
+                key[r] = a.key_in[base + j];
+                slot[r] = a.slot_in[base + j];
+            }
         }
-    }
-    __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += kTh) {
-        int at = a.hist[((int64_t)u * kDigits + d) * a.tiles + tile];
-        for (int w = 0; w < kW; ++w) { const int c = count[w][d]; count[w][d] = at; at += c; }
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < ROUNDS; ++r) {
-        const int j = j0 + r * 32 + lane;
-        const int d = key[r] < 0 ? kDigits : (key[r] >> a.shift) & (kDigits - 1);
+    for (int r = 0; r < kSortRounds; ++r) {
+        const int d = key[r] < 0 ? -1 : (key[r] >> a.shift) & (D - 1);
         const unsigned same = __match_any_sync(~0u, d);
-        int to = 0;
-        if (key[r] >= 0) to = count[warp][d] + __popc(same & ((1u << lane) - 1));
+        rank[r] = d < 0 ? 0 : count[d] + __popc(same & ((1u << lane) - 1));
         __syncwarp();
-        if (key[r] >= 0 && lane == __ffs(same) - 1) count[warp][d] += __popc(same);
+        if (d >= 0 && lane == __ffs(same) - 1) count[d] += __popc(same);
         __syncwarp();
-        if (key[r] < 0) continue;
-        const int idx = FIRST ? j : a.idx_a[base + j];
-        if constexpr (LAST) {
-            a.keys[base + to] = key[r];
-            a.slots[base + to] = make_int2(idx / a.g.K, set_entry(a.g, a.ent, first, idx).y);
-        } else {
-            a.key_b[base + to] = key[r];
-            a.idx_b[base + to] = idx;
+    }
+    __syncthreads();
+    int run = 0;
+    for (int d0 = 0; d0 < D; d0 += kTh) {
+        const int d = d0 + threadIdx.x;
+        const int total = d < D ? a.totals[(int64_t)u * D + d] : 0;
+        const int before = run + scan_before(total, warp_sum);
+        if (d < D) {
+            int at = before + a.hist[((int64_t)u * D + d) * a.tiles + tile];
+            for (int w = 0; w < kW; ++w) { const int c = sm_move[w * D + d]; sm_move[w * D + d] = at; at += c; }
         }
+        if (threadIdx.x == kTh - 1) warp_sum[0] = before + total;
+        __syncthreads();
+        run = warp_sum[0];
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+        if (key[r] < 0) continue;
+        const int64_t to = base + count[(key[r] >> a.shift) & (D - 1)] + rank[r];
+        a.key_out[to] = key[r];
+        a.slot_out[to] = slot[r];
     }
 }
 
@@ -532,10 +668,10 @@ int64_t align(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // What the backward pass keeps in its scratch.
 struct Layout {
-    int64_t flows, keys, slots, first, key_a, key_b, idx_a, idx_b, hist, total;
+    int64_t flows, keys, slots, first, key_b, slot_b, hist, totals, total;
     int64_t n_max;                 // slots of the largest set
     bool small;
-    int tiles;
+    int tiles, bits, passes;
 };
 Layout layout(const PcxTeacherGeo* p, bool runs) {
     Layout l{};
@@ -543,6 +679,10 @@ Layout layout(const PcxTeacherGeo* p, bool runs) {
     l.n_max = (int64_t)p->max_vars * p->width * p->slots;
     l.small = l.n_max <= kSmallSort;
     l.tiles = (int)pcx_cdiv(std::max<int64_t>(l.n_max, 1), kSortTile);
+    int bits = 1;
+    while ((p->cats >> bits) != 0) ++bits;
+    l.passes = (int)pcx_cdiv(bits, l.small ? 9 : 10);
+    l.bits = (int)pcx_cdiv(bits, l.passes);
     int64_t at = 0;
     auto take = [&](int64_t bytes) { const int64_t here = at; at += align(bytes); return here; };
     l.flows = take(p->flow_cols * p->width * 4);
@@ -550,8 +690,9 @@ Layout layout(const PcxTeacherGeo* p, bool runs) {
     l.slots = take(E * 8);
     l.first = take(runs ? 0 : (int64_t)p->n_sets * (p->cats + 1) * 4);
     if (!l.small) {
-        l.key_a = take(E * 4); l.key_b = take(E * 4); l.idx_a = take(E * 4); l.idx_b = take(E * 4);
-        l.hist = take((int64_t)p->n_sets * kDigits * l.tiles * 4);
+        l.key_b = take(E * 4); l.slot_b = take(E * 8);
+        l.hist = take(((int64_t)p->n_sets << l.bits) * l.tiles * 4);
+        l.totals = take(((int64_t)p->n_sets << l.bits) * 4);
     }
     l.total = at;
     return l;
@@ -581,9 +722,15 @@ int pcx_teacher_prep(void* entries, const void* ids, int wide_ids, int64_t ids_b
 
 int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int64_t stride, void* stream) {
     if (rows <= 0 || cats <= 0) return 0;
-    const int64_t r_tiles = pcx_cdiv(stride, 32), blocks = r_tiles * pcx_cdiv(cats, 32);
+    const int64_t r_tiles = pcx_cdiv(stride, kTurn), blocks = r_tiles * pcx_cdiv(cats, kTurn);
     if (blocks > 0x7fffffff) return -1;
-    teacher_turn_kernel<<<(unsigned)blocks, kTh, 0, (cudaStream_t)stream>>>(out, table, rows, cats, stride, r_tiles);
+    const bool in4 = cats % 4 == 0 && (uintptr_t)table % 16 == 0, out4 = stride % 4 == 0 && (uintptr_t)out % 16 == 0;
+    const unsigned grid = (unsigned)blocks;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (in4 && out4) teacher_turn_kernel<true, true><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
+    else if (out4) teacher_turn_kernel<false, true><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
+    else if (in4) teacher_turn_kernel<true, false><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
+    else teacher_turn_kernel<false, false><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
     PCX_LAUNCH_CHECK();
     return 0;
 }
@@ -605,10 +752,9 @@ int pcx_teacher_fwd(float* out, const float* table, const void* entries, const P
     a.out = out; a.table = table; a.ent = (const int2*)entries; a.R = turned_stride; a.take_log = take_log;
     cudaStream_t st = (cudaStream_t)stream;
     if (form == 0) {
-        const int64_t blocks = pcx_cdiv((int64_t)geo->nodes * geo->width, kTh / 8);
-        if (blocks * geo->n_segs > 0x7fffffff) return -1;
-        a.m_tiles = (int)blocks;
-        teacher_fwd_direct_kernel<<<(unsigned)(blocks * geo->n_segs), kTh, 0, st>>>(a);
+        const int64_t blocks = pcx_cdiv((int64_t)geo->nodes * geo->width * geo->n_segs, kTh / 8);
+        if (blocks > 0x7fffffff) return -1;
+        teacher_fwd_direct_kernel<<<(unsigned)blocks, kTh, 0, st>>>(a);
         PCX_LAUNCH_CHECK();
         return 0;
     }
@@ -655,43 +801,49 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     char* base = (char*)scratch;
     float* turned = (float*)(base + l.flows);
     {
-        const int m_tiles = (int)pcx_cdiv(geo->nodes, 32);
-        if ((int64_t)m_tiles * geo->n_segs > 0x7fffffff || pcx_cdiv(geo->width, 32) > 65535) return -1;
-        teacher_turn_flows_kernel<<<dim3((unsigned)(m_tiles * geo->n_segs), (unsigned)pcx_cdiv(geo->width, 32)), kTh, 0, st>>>(
-            turned, flows, g, m_tiles, logspace);
+        const int m_tiles = (int)pcx_cdiv(geo->nodes, kTurn);
+        if ((int64_t)m_tiles * geo->n_segs > 0x7fffffff || pcx_cdiv(geo->width, kTurn) > 65535) return -1;
+        const dim3 grid((unsigned)(m_tiles * geo->n_segs), (unsigned)pcx_cdiv(geo->width, kTurn));
+        if (geo->width % 4 == 0 && (uintptr_t)flows % 16 == 0) teacher_turn_flows_kernel<true><<<grid, kTh, 0, st>>>(turned, flows, g, m_tiles, logspace);
+        else teacher_turn_flows_kernel<false><<<grid, kTh, 0, st>>>(turned, flows, g, m_tiles, logspace);
         PCX_LAUNCH_CHECK();
     }
     SortArgs s{};
-    s.g = g; s.ent = (const int2*)entries; s.C = geo->cats;
+    s.g = g; s.ent = (const int2*)entries; s.C = geo->cats; s.bits = l.bits;
     s.keys = (int32_t*)(base + l.keys); s.slots = (int2*)(base + l.slots);
     if (l.small) {
-        int P = 2;
-        while (P < l.n_max) P <<= 1;
-        teacher_sort_small_kernel<<<geo->n_sets, std::min(1024, std::max(32, P / 2)), P * 4, st>>>(s, P);
+        s.first = runs ? nullptr : (int32_t*)(base + l.first);
+        const int warps = (int)std::max<int64_t>(1, pcx_cdiv(l.n_max, 128));
+        const int bytes = warps * (2 * 128 * 4 + (2 << l.bits));
+        static PcxOnce done;
+        if (!done) {
+            const cudaError_t e = cudaFuncSetAttribute((const void*)teacher_sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);
+            if (e != cudaSuccess) return (int)e;
+            done = true;
+        }
+        teacher_sort_small_kernel<<<geo->n_sets, warps * 32, bytes, st>>>(s);
         PCX_LAUNCH_CHECK();
     } else {
-        s.key_a = (int32_t*)(base + l.key_a); s.key_b = (int32_t*)(base + l.key_b);
-        s.idx_a = (int32_t*)(base + l.idx_a); s.idx_b = (int32_t*)(base + l.idx_b);
-        s.hist = (int32_t*)(base + l.hist);
+        s.hist = (int32_t*)(base + l.hist); s.totals = (int32_t*)(base + l.totals);
         s.tiles = l.tiles;
-        if ((int64_t)l.tiles * geo->n_sets > 0x7fffffff || (int64_t)l.tiles * kDigits > 0x7fffffff) return -1;
+        const int64_t digits = (int64_t)geo->n_sets << l.bits;
+        if ((int64_t)l.tiles * geo->n_sets > 0x7fffffff || pcx_cdiv(digits, kW) > 0x7fffffff) return -1;
         const unsigned grid = (unsigned)(l.tiles * geo->n_sets);
-        int bits = 1;
-        while ((geo->cats >> bits) != 0) ++bits;
-        for (int shift = 0; shift < bits; shift += 8) {
-            const bool first = shift == 0, last = shift + 8 >= bits;
-            s.shift = shift;
-            if (first) teacher_hist_kernel<true><<<grid, kTh, 0, st>>>(s); else teacher_hist_kernel<false><<<grid, kTh, 0, st>>>(s);
+        // the last of an odd number of passes ends in place; of an even number, the first goes to the other buffer too
+        int32_t* key_to[2] = {s.keys, (int32_t*)(base + l.key_b)};
+        int2* slot_to[2] = {s.slots, (int2*)(base + l.slot_b)};
+        for (int pass = 0; pass < l.passes; ++pass) {
+            const int to = (l.passes - 1 - pass) & 1;
+            s.shift = pass * l.bits;
+            s.key_in = key_to[to ^ 1]; s.slot_in = slot_to[to ^ 1];
+            s.key_out = key_to[to]; s.slot_out = slot_to[to];
+            if (pass == 0) teacher_hist_kernel<true><<<grid, kTh, 0, st>>>(s); else teacher_hist_kernel<false><<<grid, kTh, 0, st>>>(s);
             PCX_LAUNCH_CHECK();
-            teacher_scan_kernel<<<geo->n_sets, 1024, 0, st>>>(s.hist, kDigits * l.tiles);
+            teacher_scan_kernel<<<(unsigned)pcx_cdiv(digits, kW), kTh, 0, st>>>(s.hist, s.totals, digits, l.tiles);
             PCX_LAUNCH_CHECK();
-            if (first && last) teacher_move_kernel<true, true><<<grid, kTh, 0, st>>>(s);
-            else if (first) teacher_move_kernel<true, false><<<grid, kTh, 0, st>>>(s);
-            else if (last) teacher_move_kernel<false, true><<<grid, kTh, 0, st>>>(s);
-            else teacher_move_kernel<false, false><<<grid, kTh, 0, st>>>(s);
+            if (pass == 0) teacher_move_kernel<true><<<grid, kTh, (kW << l.bits) * 4, st>>>(s);
+            else teacher_move_kernel<false><<<grid, kTh, (kW << l.bits) * 4, st>>>(s);
             PCX_LAUNCH_CHECK();
-            std::swap(s.key_a, s.key_b);
-            std::swap(s.idx_a, s.idx_b);
         }
     }
     BwdArgs a{};
@@ -704,7 +856,7 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
         PCX_LAUNCH_CHECK();
         return 0;
     }
-    {
+    if (!l.small) {
         const int64_t blocks = pcx_cdiv(l.n_max + 1, kTh);
         if (blocks * geo->n_sets > 0x7fffffff) return -1;
         teacher_first_kernel<<<(unsigned)(blocks * geo->n_sets), kTh, 0, st>>>((int32_t*)(base + l.first), s.keys, g, geo->cats, (int)blocks);
