@@ -171,77 +171,157 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_direct_kernel(FwdArgs a) {
     if (sub == 0) a.out[(seg.row0 + m) * W + b] = acc;
 }
 
-// NM * 32 nodes of one vector; a warp takes one position at a time, its lanes the nodes.  SRC 0: the turned table, four
-// neighbouring nodes per lane; 1: the turned table, any alignment; 2: the table's part in shared memory.
-template <int SRC, int NM>
-__global__ void __launch_bounds__(kTh) teacher_fwd_kernel(FwdArgs a) {
-    constexpr int MT = 32 * NM;
-    extern __shared__ float sm[];
-    float* tile = sm;                                  // [MT][33]
-    float* part = sm + MT * 33;                        // [C][MT + 1]
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // (turned tables: the same nodes of all positions run side by side, so that their part of the table stays in L2)
-    const Seg seg = seg_of(a.g, SRC == 2 ? blockIdx.x / a.m_tiles : blockIdx.x % a.g.n_segs);
-    const int m0 = (SRC == 2 ? blockIdx.x % a.m_tiles : blockIdx.x / a.g.n_segs) * MT;
-    if (m0 >= seg.M) return;
-    const int W = a.g.W, K = a.g.K;
-    if constexpr (SRC == 2) {
-        for (int m = warp; m < MT; m += kW) {
-            const float* row = a.table + seg.table + (int64_t)(m0 + m) * seg.C;
-#pragma unroll 4
-            for (int c = lane; c < seg.C; c += 32) {
-                float v = m0 + m < seg.M ? row[c] : 1.0f;
-                if (a.take_log) v = logf(v);
-                part[c * (MT + 1) + m] = v;
-            }
+// How a lane's NV values lie among the nodes of a tile: four neighbours at a time, or 32 apart.
+template <bool VEC>
+__device__ __forceinline__ int node_of(int lane, int i) { return VEC ? (i / 4) * 128 + lane * 4 + i % 4 : i * 32 + lane; }
+
+// The entries of four positions beside one another: their loads and lookups do not wait for one another.
+template <int NV, typename F>
+__device__ __forceinline__ void four_rows(const int2* const (&e)[4], int K, int C, float (&acc)[4][NV], F add) {
+    const int lane = threadIdx.x & 31;
+    bool beyond[4] = {};                               // a category that the table does not have
+    for (int k0 = 0; k0 < K; k0 += 32) {
+        int n[4], most = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int id = e[j] != nullptr && k0 + lane < K ? __ldg(&e[j][k0 + lane].x) : -1;
+            n[j] = __popc(__ballot_sync(~0u, id >= 0));
+            if (__any_sync(~0u, id >= C)) { beyond[j] = true; n[j] = 0; }
+            most = max(most, n[j]);
         }
-        __syncthreads();
+        for (int k = 0; k < most; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (k < n[j]) {
+                    const int2 x = __ldg(e[j] + k0 + k);
+                    add(x.x, __int_as_float(x.y), acc[j]);
+                }
+        if (most < 32 && !(beyond[0] | beyond[1] | beyond[2] | beyond[3])) break;
     }
-    const float* base = a.table + seg.col + m0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (beyond[j])
+#pragma unroll
+            for (int i = 0; i < NV; ++i) acc[j][i] = PCX_NEG_INF;
+}
+
+// A warp's results [NV * 32 nodes][32 positions] of all positions of a block go through shared memory to rows of positions.
+template <int NV>
+__device__ __forceinline__ void store_rows(const float* tile, float* out, int m_left, int b_left, int W) {
+    const int lane = threadIdx.x & 31;
+    for (int m = threadIdx.x >> 5; m < min(32 * NV, m_left); m += kW)
+        if (lane < b_left) out[(int64_t)m * W + lane] = tile[m * 33 + lane];
+}
+
+// Turned table: a warp takes one position at a time, its lanes NV nodes each.  The same nodes of all positions run side by
+// side, so that their part of the table stays in L2.
+template <bool VEC, int NV>
+__global__ void __launch_bounds__(kTh) teacher_fwd_turned_kernel(FwdArgs a) {
+    constexpr int MT = 32 * NV;
+    extern __shared__ float tile[];                    // [MT][33]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Seg seg = seg_of(a.g, blockIdx.x % a.g.n_segs);
+    const int m0 = blockIdx.x / a.g.n_segs * MT;
+    if (m0 >= seg.M) return;
+    const int W = a.g.W, K = a.g.K, R = (int)a.R;
+    const float* at[VEC ? NV / 4 : NV];                // lanes without a node look at the vector's first
+#pragma unroll
+    for (int i = 0; i < (VEC ? NV / 4 : NV); ++i) {
+        const int m = m0 + node_of<VEC>(lane, VEC ? 4 * i : i);
+        at[i] = a.table + seg.col + (m < seg.M ? m : 0);
+    }
     const int b_end = min(W, (int)(blockIdx.y + 1) * a.per_b);
     for (int b0 = blockIdx.y * a.per_b; b0 < b_end; b0 += 32) {
         for (int j = 0; j < 4; ++j) {
             const int b = b0 + warp * 4 + j;
             if (b >= b_end) break;
             const int2* e = a.ent + ((int64_t)seg.var * W + b) * K;
-            float acc[NM] = {};
-            bool beyond = false;                       // a category that the table does not have
+            float acc[NV] = {};
             for (int k0 = 0; k0 < K; k0 += 32) {
-                const int id = k0 + lane < K ? __ldg(e + k0 + lane).x : -1;
+                const int id = k0 + lane < K ? __ldg(&e[k0 + lane].x) : -1;
                 const int n = __popc(__ballot_sync(~0u, id >= 0));
-                beyond |= __any_sync(~0u, id >= seg.C);
-#pragma unroll 8
-                for (int k = k0; k < k0 + n; ++k) {
-                    const int2 x = __ldg(e + k);
-                    const int c = min(x.x, seg.C - 1);
-                    const float q = __int_as_float(x.y);
-                    if constexpr (SRC == 0) {
-                        if (m0 + lane * 4 < seg.M) {
-                            const float4 v = __ldg((const float4*)(base + (int64_t)c * a.R) + lane);
-                            acc[0] = fmaf(q, v.x, acc[0]); acc[1] = fmaf(q, v.y, acc[1]);
-                            acc[2] = fmaf(q, v.z, acc[2]); acc[3] = fmaf(q, v.w, acc[3]);
-                        }
-                    } else if constexpr (SRC == 1) {
+                if (__any_sync(~0u, id >= seg.C)) {
 #pragma unroll
-                        for (int i = 0; i < NM; ++i)
-                            if (m0 + lane + 32 * i < seg.M) acc[i] = fmaf(q, __ldg(base + (int64_t)c * a.R + lane + 32 * i), acc[i]);
+                    for (int i = 0; i < NV; ++i) acc[i] = PCX_NEG_INF;
+                    break;
+                }
+#pragma unroll 8
+                for (int k = 0; k < n; ++k) {
+                    const int2 x = __ldg(e + k0 + k);
+                    const float q = __int_as_float(x.y);
+                    const int64_t off = (int64_t)x.x * R;
+                    if constexpr (VEC) {
+#pragma unroll
+                        for (int i = 0; i < NV / 4; ++i) {
+                            const float4 v = __ldg((const float4*)(at[i] + off));
+                            acc[4 * i] = fmaf(q, v.x, acc[4 * i]); acc[4 * i + 1] = fmaf(q, v.y, acc[4 * i + 1]);
+                            acc[4 * i + 2] = fmaf(q, v.z, acc[4 * i + 2]); acc[4 * i + 3] = fmaf(q, v.w, acc[4 * i + 3]);
+                        }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < NM; ++i) acc[i] = fmaf(q, part[c * (MT + 1) + lane + 32 * i], acc[i]);
+                        for (int i = 0; i < NV; ++i) acc[i] = fmaf(q, __ldg(at[i] + off), acc[i]);
                     }
                 }
                 if (n < 32) break;
             }
-            if (beyond) {
 #pragma unroll
-                for (int i = 0; i < NM; ++i) acc[i] = PCX_NEG_INF;
-            }
-#pragma unroll
-            for (int i = 0; i < NM; ++i) tile[(SRC == 0 ? lane * 4 + i : lane + 32 * i) * 33 + warp * 4 + j] = acc[i];
+            for (int i = 0; i < NV; ++i) tile[node_of<VEC>(lane, i) * 33 + warp * 4 + j] = acc[i];
         }
         __syncthreads();
-        for (int m = warp; m < MT; m += kW)
-            if (m0 + m < seg.M && b0 + lane < b_end) a.out[(seg.row0 + m0 + m) * W + b0 + lane] = tile[m * 33 + lane];
+        store_rows<NV>(tile, a.out + (seg.row0 + m0) * W + b0, seg.M - m0, b_end - b0, W);
+        __syncthreads();
+    }
+}
+
+// A table of its own: NV * 32 nodes of it go through shared memory, the nodes of a category side by side.
+template <int NV>
+__global__ void __launch_bounds__(kTh) teacher_fwd_staged_kernel(FwdArgs a) {
+    constexpr int MT = 32 * NV;
+    extern __shared__ float tile[];                    // [MT][33], then the table's part [C][MT + 1]
+    float* part = tile + MT * 33;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Seg seg = seg_of(a.g, blockIdx.x / a.m_tiles);
+    const int m0 = blockIdx.x % a.m_tiles * MT;
+    if (m0 >= seg.M) return;
+    const int W = a.g.W, K = a.g.K, C = seg.C;
+    for (int c = lane; c < C; c += 64) {
+        constexpr int PER = MT / kW;                   // a warp's nodes, two categories a lane at a time
+        const float* row = a.table + seg.table + (int64_t)(m0 + warp * PER) * C + c;
+        float v[2][PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const bool in = m0 + warp * PER + i < seg.M;
+            v[0][i] = in ? __ldg(row + (int64_t)i * C) : 1.0f;
+            v[1][i] = in && c + 32 < C ? __ldg(row + (int64_t)i * C + 32) : 1.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            float* to = part + c * (MT + 1) + warp * PER + i;
+            to[0] = a.take_log ? logf(v[0][i]) : v[0][i];
+            if (c + 32 < C) to[32 * (MT + 1)] = a.take_log ? logf(v[1][i]) : v[1][i];
+        }
+    }
+    __syncthreads();
+    const int b_end = min(W, (int)(blockIdx.y + 1) * a.per_b);
+    for (int b0 = blockIdx.y * a.per_b; b0 < b_end; b0 += 32) {
+        const int2* e[4];
+        float acc[4][NV] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int b = b0 + warp * 4 + j;
+            e[j] = b < b_end ? a.ent + ((int64_t)seg.var * W + b) * K : nullptr;
+        }
+        four_rows<NV>(e, K, C, acc, [&](int c, float q, float (&s)[NV]) {
+            const float* v = part + c * (MT + 1) + lane;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) s[i] = fmaf(q, v[32 * i], s[i]);
+        });
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) tile[(32 * i + lane) * 33 + warp * 4 + j] = acc[j][i];
+        __syncthreads();
+        store_rows<NV>(tile, a.out + (seg.row0 + m0) * W + b0, seg.M - m0, b_end - b0, W);
         __syncthreads();
     }
 }
@@ -550,83 +630,108 @@ struct BwdArgs {
     const int2* slots;
     const int32_t* first;
     int64_t R;
-    int C, mode, c_tiles, m_tiles; // mode 0: written, all of it; 1: added; 2: added to the turned table
+    int C, mode, c_tiles, m_tiles, c_tile;             // mode 0: written, all of it; 1: added; 2: added to the turned table
 };
 
-constexpr int kHeavy = 128;        // slots of a category that all warps of a CTA share
-
-// 32 categories x 128 nodes of one group.  A warp sums a category's slots in their order, lanes over the nodes; a category
-// with many slots is split over the CTA's warps, whose parts are added in order.
+// c_tile (at most 32) categories x NV * 32 nodes of one group.  The slots of the tile's categories, side by side after the sort,
+// are dealt out to the warps in equal parts; a warp walks its part in order, lanes over the nodes, and closes a category's
+// sum where the next begins.  A category that an earlier warp began is added to that warp's sum afterwards, in order.
+template <int NV>
 __global__ void __launch_bounds__(kTh) teacher_bwd_kernel(BwdArgs a) {
-    __shared__ float acc[32][129];
-    __shared__ float part[kW][128];
+    constexpr int MT = 32 * NV, AHEAD = NV > 4 ? 4 : 8;
+    extern __shared__ float acc[];                     // [c_tile][MT + 1], then [kW][MT]
     __shared__ int from[33];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int64_t at = blockIdx.x;
-    const int c0 = (int)(at % a.c_tiles) * 32;
+    const int c0 = (int)(at % a.c_tiles) * a.c_tile;
     at /= a.c_tiles;
-    const int m0 = (int)(at % a.m_tiles) * 128;
+    const int m0 = (int)(at % a.m_tiles) * MT;
     const Grp grp = grp_of(a.g, (int)(at / a.m_tiles));
     if (m0 >= grp.M || c0 >= grp.C) return;
-    const int nc = min(32, grp.C - c0);
+    const int nc = min(a.c_tile, grp.C - c0), nm = min(MT, grp.M - m0);
+    float* part = acc + a.c_tile * (MT + 1);
     if (tid <= nc) from[tid] = a.first[(int64_t)grp.set * (a.C + 1) + c0 + tid];
     __syncthreads();
-    const bool none = from[0] == from[nc];
-    if (none && a.mode != 0) return;
-    const int mp = pad4(grp.M);
-    const float* flows = a.flows + grp.gbase * a.g.W + m0 + lane * 4;
-    const int2* slots = a.slots + (int64_t)set_begin(a.g, grp.set) * a.g.W * a.g.K;
-    const bool in = m0 + lane * 4 < mp;
-    auto sum = [&](int lo, int hi) {
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (in) {
-#pragma unroll 8
-            for (int j = lo; j < hi; ++j) {
-                const int2 e = __ldg(slots + j);
-                const float q = __int_as_float(e.y);
-                const float4 v = __ldg((const float4*)(flows + (int64_t)e.x * mp));
-                s.x = fmaf(q, v.x, s.x); s.y = fmaf(q, v.y, s.y); s.z = fmaf(q, v.z, s.z); s.w = fmaf(q, v.w, s.w);
+    const int begin = from[0], end = from[nc];
+    if (begin == end && a.mode != 0) return;
+    if (begin < end) {
+        const int mp = pad4(grp.M);
+        const int64_t base = (int64_t)set_begin(a.g, grp.set) * a.g.W * a.g.K;
+        const int2* slots = a.slots + base;
+        const int32_t* keys = a.keys + base;
+        const float* v_at[NV / 4];                     // lanes without a node look at the group's first
+#pragma unroll
+        for (int i = 0; i < NV / 4; ++i) {
+            const int m = m0 + i * 128 + lane * 4;
+            v_at[i] = a.flows + grp.gbase * a.g.W + (m < mp ? m : 0);
+        }
+        const int per = (end - begin + kW - 1) / kW;
+        const int lo = min(end, begin + warp * per), hi = min(end, lo + per);
+        if (lo < hi) {
+            float s[NV] = {};
+            int cur = keys[lo];
+            float* to = lo > from[cur - c0] ? part + warp * MT : acc + (cur - c0) * (MT + 1);
+            auto close = [&]() {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) { to[node_of<true>(lane, i)] = s[i]; s[i] = 0.0f; }
+            };
+            for (int j0 = lo; j0 < hi; j0 += AHEAD) {
+                int c[AHEAD];
+                float q[AHEAD];
+                float4 v[AHEAD][NV / 4];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int j = min(j0 + i, hi - 1);
+                    const int2 e = __ldg(slots + j);
+                    c[i] = __ldg(keys + j);
+                    q[i] = __int_as_float(e.y);
+#pragma unroll
+                    for (int k = 0; k < NV / 4; ++k) v[i][k] = __ldg((const float4*)(v_at[k] + (int64_t)e.x * mp));
+                }
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    if (j0 + i >= hi) break;
+                    if (c[i] != cur) {
+                        close();
+                        cur = c[i];
+                        to = acc + (cur - c0) * (MT + 1);
+                    }
+#pragma unroll
+                    for (int k = 0; k < NV / 4; ++k) {
+                        s[4 * k] = fmaf(q[i], v[i][k].x, s[4 * k]); s[4 * k + 1] = fmaf(q[i], v[i][k].y, s[4 * k + 1]);
+                        s[4 * k + 2] = fmaf(q[i], v[i][k].z, s[4 * k + 2]); s[4 * k + 3] = fmaf(q[i], v[i][k].w, s[4 * k + 3]);
+                    }
+                }
             }
+            close();
         }
-        return s;
-    };
-    if (!none) {
-        for (int cc = warp; cc < nc; cc += kW) {
-            const int lo = from[cc], hi = from[cc + 1];
-            if (hi - lo > kHeavy) continue;
-            const float4 s = sum(lo, hi);
-            acc[cc][lane * 4] = s.x; acc[cc][lane * 4 + 1] = s.y; acc[cc][lane * 4 + 2] = s.z; acc[cc][lane * 4 + 3] = s.w;
-        }
-        for (int cc = 0; cc < nc; ++cc) {
-            const int lo = from[cc], hi = from[cc + 1];
-            if (hi - lo <= kHeavy) continue;
-            const int per = (hi - lo + kW - 1) / kW;
-            const float4 s = sum(lo + warp * per, min(hi, lo + (warp + 1) * per));
-            *(float4*)&part[warp][lane * 4] = s;
-            __syncthreads();
-            if (tid < 128) {
-                float t = part[0][tid];
-                for (int w = 1; w < kW; ++w) t += part[w][tid];
-                acc[cc][tid] = t;
+        __syncthreads();
+        if (per > 0 && tid < MT)
+            for (int w = 1; w < kW; ++w) {
+                const int l = begin + w * per;
+                if (l >= end) break;
+                const int c = keys[l] - c0;
+                if (l > from[c]) acc[c * (MT + 1) + tid] += part[w * MT + tid];
             }
-            __syncthreads();
-        }
         __syncthreads();
     }
     if (a.mode == 2) {
         for (int cc = warp; cc < nc; cc += kW) {
             if (from[cc] == from[cc + 1]) continue;
             float* row = a.out + (int64_t)(c0 + cc) * a.R + grp.col + m0;
-            for (int m = lane; m < 128 && m0 + m < grp.M; m += 32) row[m] += acc[cc][m];
+            for (int m = lane; m < nm; m += 32) row[m] += acc[cc * (MT + 1) + m];
             if (lane == 0) a.touched[c0 + cc] = 1;
         }
         return;
     }
-    for (int m = warp; m < 128 && m0 + m < grp.M; m += kW) {
-        if (lane >= nc) continue;
-        float* p = a.out + grp.out + (int64_t)(m0 + m) * grp.C + c0 + lane;
-        if (a.mode == 0) *p = none ? 0.0f : acc[lane][m];
-        else if (from[lane] != from[lane + 1]) *p += acc[lane][m];
+    const int n_lanes = a.c_tile, rows = kTh / n_lanes;       // lanes side by side over the categories
+    const int cc = tid % n_lanes;
+    if (cc >= nc) return;
+    const bool has = from[cc] != from[cc + 1];
+    float* p = a.out + grp.out + (int64_t)m0 * grp.C + c0 + cc;
+    for (int m = tid / n_lanes; m < nm; m += rows) {
+        if (a.mode == 0) p[(int64_t)m * grp.C] = has ? acc[cc * (MT + 1) + m] : 0.0f;
+        else if (has) p[(int64_t)m * grp.C] += acc[cc * (MT + 1) + m];
     }
 }
 
@@ -758,33 +863,36 @@ int pcx_teacher_fwd(float* out, const float* table, const void* entries, const P
         PCX_LAUNCH_CHECK();
         return 0;
     }
-    int mt = 128;
-    if (form == 2 && (mt = pcx_teacher_staged_nodes(geo->cats, geo->nodes)) == 0) return -1;
+    // nodes per CTA: as many as there are, 128 or 256, of a turned table
+    const int mt = form == 2 ? pcx_teacher_staged_nodes(geo->cats, geo->nodes) : geo->nodes > 128 && form == 3 ? 256 : 128;
+    if (mt == 0) return -1;
     a.m_tiles = (int)pcx_cdiv(geo->nodes, mt);
-    if ((int64_t)a.m_tiles * geo->n_segs > 0x7fffffff) return -1;
-    // positions per CTA: all of them where the table has to be staged first, unless few CTAs would be left
     const int64_t tiles = (int64_t)a.m_tiles * geo->n_segs;
+    if (tiles > 0x7fffffff || turned_stride > 0x7fffffff) return -1;
+    // positions per CTA: all of them where the table has to be staged first, unless few CTAs would be left
     const int64_t splits = std::max<int64_t>(1, std::min(pcx_cdiv(geo->width, 32), form == 2 ? pcx_cdiv(148, tiles) : (int64_t)65535));
     a.per_b = (int)(pcx_cdiv(pcx_cdiv(geo->width, splits), 32) * 32);
     const dim3 grid((unsigned)tiles, (unsigned)pcx_cdiv(geo->width, a.per_b));
     const int tile_bytes = mt * 33 * 4;
     if (form == 1) {
-        teacher_fwd_kernel<1, 4><<<grid, kTh, tile_bytes, st>>>(a);
+        teacher_fwd_turned_kernel<false, 4><<<grid, kTh, tile_bytes, st>>>(a);
+    } else if (form == 3 && mt == 128) {
+        teacher_fwd_turned_kernel<true, 4><<<grid, kTh, tile_bytes, st>>>(a);
     } else if (form == 3) {
-        teacher_fwd_kernel<0, 4><<<grid, kTh, tile_bytes, st>>>(a);
+        teacher_fwd_turned_kernel<true, 8><<<grid, kTh, tile_bytes, st>>>(a);
     } else {
         const int bytes = tile_bytes + geo->cats * (mt + 1) * 4;
         static PcxOnce done;
         if (!done) {
-            for (const void* k : {(const void*)teacher_fwd_kernel<2, 4>, (const void*)teacher_fwd_kernel<2, 2>, (const void*)teacher_fwd_kernel<2, 1>}) {
+            for (const void* k : {(const void*)teacher_fwd_staged_kernel<4>, (const void*)teacher_fwd_staged_kernel<2>, (const void*)teacher_fwd_staged_kernel<1>}) {
                 const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
                 if (e != cudaSuccess) return (int)e;
             }
             done = true;
         }
-        if (mt == 128) teacher_fwd_kernel<2, 4><<<grid, kTh, bytes, st>>>(a);
-        else if (mt == 64) teacher_fwd_kernel<2, 2><<<grid, kTh, bytes, st>>>(a);
-        else teacher_fwd_kernel<2, 1><<<grid, kTh, bytes, st>>>(a);
+        if (mt == 128) teacher_fwd_staged_kernel<4><<<grid, kTh, bytes, st>>>(a);
+        else if (mt == 64) teacher_fwd_staged_kernel<2><<<grid, kTh, bytes, st>>>(a);
+        else teacher_fwd_staged_kernel<1><<<grid, kTh, bytes, st>>>(a);
     }
     PCX_LAUNCH_CHECK();
     return 0;
@@ -863,11 +971,18 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
         PCX_LAUNCH_CHECK();
     }
     a.first = (const int32_t*)(base + l.first);
-    a.c_tiles = (int)pcx_cdiv(geo->cats, 32);
-    a.m_tiles = (int)pcx_cdiv(geo->nodes, 128);
-    const int64_t blocks = (int64_t)a.c_tiles * a.m_tiles * geo->n_groups;
-    if (blocks > 0x7fffffff) return -1;
-    teacher_bwd_kernel<<<(unsigned)blocks, kTh, 0, st>>>(a);
+    // nodes and categories per CTA: as many as leave every SM four CTAs
+    int mt = geo->nodes > 128 ? 256 : 128;
+    a.c_tile = 32;
+    auto ctas = [&]() { return pcx_cdiv(geo->cats, a.c_tile) * pcx_cdiv(geo->nodes, mt) * geo->n_groups; };
+    while (a.c_tile > 8 && ctas() < 148 * 4) a.c_tile /= 2;
+    if (ctas() < 148 * 4) mt = 128;
+    a.c_tiles = (int)pcx_cdiv(geo->cats, a.c_tile);
+    a.m_tiles = (int)pcx_cdiv(geo->nodes, mt);
+    if (ctas() > 0x7fffffff) return -1;
+    const int bytes = (a.c_tile * (mt + 1) + kW * mt) * 4;
+    if (mt == 256) teacher_bwd_kernel<8><<<(unsigned)ctas(), kTh, bytes, st>>>(a);
+    else teacher_bwd_kernel<4><<<(unsigned)ctas(), kTh, bytes, st>>>(a);
     PCX_LAUNCH_CHECK();
     return 0;
 }
