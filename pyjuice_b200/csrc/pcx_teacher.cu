@@ -13,6 +13,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -72,23 +73,20 @@ struct PrepArgs {
     double inv_t64;
 };
 
-// One warp per position; up to 4 slots a lane stay in registers, more are read again.  Slots that say something come first, in
-// their order: what reads them stops at the first empty one.
+// L lanes per position, four slots a lane in registers (more are read again).  Slots that say something come first, in their
+// order: what reads them stops at the first empty one.
+template <int L>
 __global__ void __launch_bounds__(kTh) teacher_prep_kernel(PrepArgs a) {
     constexpr int HELD = 4;
-    const int64_t at = (int64_t)blockIdx.x * kW + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (at >= (int64_t)a.V * a.W) return;
-    const int v = (int)(at / a.W), b = (int)(at % a.W);
+    const int64_t at = (int64_t)blockIdx.x * (kTh / L) + threadIdx.x / L;
+    const int lane = threadIdx.x % L;
+    const bool here = at < (int64_t)a.V * a.W;         // (all lanes take part in the shuffles)
+    const int v = (int)(at / a.W), b = here ? (int)(at % a.W) : a.B;
     int2* out = a.ent + at * a.K;
-    if (b >= a.B) {                                    // padding columns
-        for (int k = lane; k < a.K; k += 32) out[k] = make_int2(-1, 0);
-        return;
-    }
     auto slot = [&](int k, int& id, float& x) {
         id = -1;
         x = PCX_NEG_INF;
-        if (k >= a.K) return;
+        if (k >= a.K || b >= a.B) return;              // (padding columns are empty)
         const int64_t i = b * a.ib + v * a.iv + k * a.ik;
         const int64_t wide = a.wide_ids ? ((const int64_t*)a.ids)[i] : (int64_t)((const int32_t*)a.ids)[i];
         const float y = load_logit(a.logits, a.dtype, b * a.lb + v * a.lv + k * a.lk);
@@ -97,39 +95,41 @@ __global__ void __launch_bounds__(kTh) teacher_prep_kernel(PrepArgs a) {
     int ids[HELD];
     float xs[HELD];
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) slot(lane + 32 * i, ids[i], xs[i]);
+    for (int i = 0; i < HELD; ++i) slot(lane + L * i, ids[i], xs[i]);
     auto each = [&](auto&& f) {
 #pragma unroll
         for (int i = 0; i < HELD; ++i)
-            if (32 * i < a.K) f(ids[i], xs[i]);
-        for (int k0 = 32 * HELD; k0 < a.K; k0 += 32) {
+            if (L * i < a.K) f(ids[i], xs[i]);
+        for (int k0 = L * HELD; k0 < a.K; k0 += L) {
             int id; float x;
             slot(k0 + lane, id, x);
             f(id, x);
         }
     };
-    const float norm = a.norms != nullptr ? a.norms[b * a.nb + v * a.nv] : CUDART_INF_F;
+    const float norm = a.norms != nullptr && b < a.B ? a.norms[b * a.nb + v * a.nv] : CUDART_INF_F;
     const bool given = fabsf(norm) < CUDART_INF_F;
     float m = PCX_NEG_INF, sum = 0.0f;
     each([&](int, float x) { m = fmaxf(m, x); });
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
     auto raw = [&](float x) {
         if (x == PCX_NEG_INF) return 0.0f;
         if (given) return expf((float)((double)x * a.inv_t64 - (double)norm));
         return x == m ? 1.0f : expf((x - m) * a.inv_t);          // (+inf logits share the weight)
     };
-    if (!given) {
-        each([&](int, float x) { sum += raw(x); });
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    }
+    each([&](int, float x) { sum += raw(x); });
+#pragma unroll
+    for (int o = L / 2; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     int count = 0;
+    const int first_lane = threadIdx.x % 32 - lane;
     each([&](int id, float x) {
         const float q = given ? raw(x) : sum > 0.0f ? raw(x) / sum : 0.0f;
-        const unsigned says = __ballot_sync(~0u, id >= 0 && q > 0.0f);
+        const unsigned says = (__ballot_sync(~0u, id >= 0 && q > 0.0f) >> first_lane) & (L == 32 ? ~0u : (1u << (L & 31)) - 1);
         if (id >= 0 && q > 0.0f) out[count + __popc(says & ((1u << lane) - 1))] = make_int2(id, __float_as_int(q));
         count += __popc(says);
     });
-    for (int k = count + lane; k < a.K; k += 32) out[k] = make_int2(-1, 0);
+    if (here)
+        for (int k = count + lane; k < a.K; k += L) out[k] = make_int2(-1, 0);
 }
 
 // ---- forward -----------------------------------------------------------------------------------------------------------
@@ -171,39 +171,18 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_direct_kernel(FwdArgs a) {
     if (sub == 0) a.out[(seg.row0 + m) * W + b] = acc;
 }
 
+// Row `i` of `stride` bytes from `base`: one multiply-add.
+template <typename T>
+__device__ __forceinline__ const T* row_at(const char* base, int i, uint32_t stride) {
+    return (const T*)(base + (uint64_t)(uint32_t)i * stride);
+}
+__device__ __forceinline__ void fma4(float q, const float4& v, float* s) {
+    s[0] = fmaf(q, v.x, s[0]); s[1] = fmaf(q, v.y, s[1]); s[2] = fmaf(q, v.z, s[2]); s[3] = fmaf(q, v.w, s[3]);
+}
+
 // How a lane's NV values lie among the nodes of a tile: four neighbours at a time, or 32 apart.
 template <bool VEC>
 __device__ __forceinline__ int node_of(int lane, int i) { return VEC ? (i / 4) * 128 + lane * 4 + i % 4 : i * 32 + lane; }
-
-// The entries of four positions beside one another: their loads and lookups do not wait for one another.
-template <int NV, typename F>
-__device__ __forceinline__ void four_rows(const int2* const (&e)[4], int K, int C, float (&acc)[4][NV], F add) {
-    const int lane = threadIdx.x & 31;
-    bool beyond[4] = {};                               // a category that the table does not have
-    for (int k0 = 0; k0 < K; k0 += 32) {
-        int n[4], most = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int id = e[j] != nullptr && k0 + lane < K ? __ldg(&e[j][k0 + lane].x) : -1;
-            n[j] = __popc(__ballot_sync(~0u, id >= 0));
-            if (__any_sync(~0u, id >= C)) { beyond[j] = true; n[j] = 0; }
-            most = max(most, n[j]);
-        }
-        for (int k = 0; k < most; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (k < n[j]) {
-                    const int2 x = __ldg(e[j] + k0 + k);
-                    add(x.x, __int_as_float(x.y), acc[j]);
-                }
-        if (most < 32 && !(beyond[0] | beyond[1] | beyond[2] | beyond[3])) break;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (beyond[j])
-#pragma unroll
-            for (int i = 0; i < NV; ++i) acc[j][i] = PCX_NEG_INF;
-}
 
 // A warp's results [NV * 32 nodes][32 positions] of all positions of a block go through shared memory to rows of positions.
 template <int NV>
@@ -216,19 +195,21 @@ __device__ __forceinline__ void store_rows(const float* tile, float* out, int m_
 // Turned table: a warp takes one position at a time, its lanes NV nodes each.  The same nodes of all positions run side by
 // side, so that their part of the table stays in L2.
 template <bool VEC, int NV>
-__global__ void __launch_bounds__(kTh) teacher_fwd_turned_kernel(FwdArgs a) {
+__global__ void __launch_bounds__(kTh, 4) teacher_fwd_turned_kernel(FwdArgs a) {
     constexpr int MT = 32 * NV;
     extern __shared__ float tile[];                    // [MT][33]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Seg seg = seg_of(a.g, blockIdx.x % a.g.n_segs);
     const int m0 = blockIdx.x / a.g.n_segs * MT;
     if (m0 >= seg.M) return;
-    const int W = a.g.W, K = a.g.K, R = (int)a.R;
-    const float* at[VEC ? NV / 4 : NV];                // lanes without a node look at the vector's first
+    const int W = a.g.W, K = a.g.K;
+    constexpr int LOADS = VEC ? NV / 4 : NV;
+    const uint32_t stride = (uint32_t)a.R * 4;
+    const char* at[LOADS];                             // lanes without a node look at the vector's first
 #pragma unroll
-    for (int i = 0; i < (VEC ? NV / 4 : NV); ++i) {
+    for (int i = 0; i < LOADS; ++i) {
         const int m = m0 + node_of<VEC>(lane, VEC ? 4 * i : i);
-        at[i] = a.table + seg.col + (m < seg.M ? m : 0);
+        at[i] = (const char*)(a.table + seg.col + (m < seg.M ? m : 0));
     }
     const int b_end = min(W, (int)(blockIdx.y + 1) * a.per_b);
     for (int b0 = blockIdx.y * a.per_b; b0 < b_end; b0 += 32) {
@@ -238,30 +219,42 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_turned_kernel(FwdArgs a) {
             const int2* e = a.ent + ((int64_t)seg.var * W + b) * K;
             float acc[NV] = {};
             for (int k0 = 0; k0 < K; k0 += 32) {
-                const int id = k0 + lane < K ? __ldg(&e[k0 + lane].x) : -1;
-                const int n = __popc(__ballot_sync(~0u, id >= 0));
-                if (__any_sync(~0u, id >= seg.C)) {
+                const int2 own = k0 + lane < K ? __ldg(e + k0 + lane) : make_int2(-1, 0);
+                const int n = __popc(__ballot_sync(~0u, own.x >= 0));
+                if (__any_sync(~0u, own.x >= seg.C)) { // a category that the table does not have
 #pragma unroll
                     for (int i = 0; i < NV; ++i) acc[i] = PCX_NEG_INF;
                     break;
                 }
-#pragma unroll 8
-                for (int k = 0; k < n; ++k) {
-                    const int2 x = __ldg(e + k0 + k);
-                    const float q = __int_as_float(x.y);
-                    const int64_t off = (int64_t)x.x * R;
-                    if constexpr (VEC) {
+                constexpr int AHEAD = VEC ? 32 / NV : 4;
+                auto some = [&](int k, auto whole) {   // the next AHEAD slots, or what is left of them
+                    float q[AHEAD];
+                    float4 v[AHEAD][LOADS];
 #pragma unroll
-                        for (int i = 0; i < NV / 4; ++i) {
-                            const float4 v = __ldg((const float4*)(at[i] + off));
-                            acc[4 * i] = fmaf(q, v.x, acc[4 * i]); acc[4 * i + 1] = fmaf(q, v.y, acc[4 * i + 1]);
-                            acc[4 * i + 2] = fmaf(q, v.z, acc[4 * i + 2]); acc[4 * i + 3] = fmaf(q, v.w, acc[4 * i + 3]);
+                    for (int h = 0; h < AHEAD; ++h) {
+                        const int c = __shfl_sync(~0u, own.x, k + h);
+                        q[h] = __int_as_float(__shfl_sync(~0u, own.y, k + h));
+                        if (whole.value || k + h < n) {
+#pragma unroll
+                            for (int i = 0; i < LOADS; ++i) {
+                                if constexpr (VEC) v[h][i] = __ldg(row_at<float4>(at[i], c, stride));
+                                else v[h][i].x = __ldg(row_at<float>(at[i], c, stride));
+                            }
                         }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < NV; ++i) acc[i] = fmaf(q, __ldg(at[i] + off), acc[i]);
                     }
-                }
+#pragma unroll
+                    for (int h = 0; h < AHEAD; ++h) {
+                        if (!whole.value && k + h >= n) break;
+#pragma unroll
+                        for (int i = 0; i < LOADS; ++i) {
+                            if constexpr (VEC) fma4(q[h], v[h][i], acc + 4 * i);
+                            else acc[i] = fmaf(q[h], v[h][i].x, acc[i]);
+                        }
+                    }
+                };
+                int k = 0;
+                for (; k + AHEAD <= n; k += AHEAD) some(k, std::true_type());
+                if (k < n) some(k, std::false_type());
                 if (n < 32) break;
             }
 #pragma unroll
@@ -274,16 +267,26 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_turned_kernel(FwdArgs a) {
 }
 
 // A table of its own: NV * 32 nodes of it go through shared memory, the nodes of a category side by side.
-template <int NV>
+template <int NV, bool LOG>
 __global__ void __launch_bounds__(kTh) teacher_fwd_staged_kernel(FwdArgs a) {
     constexpr int MT = 32 * NV;
-    extern __shared__ float tile[];                    // [MT][33], then the table's part [C][MT + 1]
+    extern __shared__ float tile[];                    // [MT][33], then the table's part [C][MT + 1] and a row of zeros
     float* part = tile + MT * 33;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Seg seg = seg_of(a.g, blockIdx.x / a.m_tiles);
     const int m0 = blockIdx.x % a.m_tiles * MT;
     if (m0 >= seg.M) return;
     const int W = a.g.W, K = a.g.K, C = seg.C;
+    const int b_begin = blockIdx.y * a.per_b, b_end = min(W, b_begin + a.per_b);
+    int2 next[4];                                      // the first 32 slots of this warp's next four positions
+    auto fetch = [&](int b0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int b = b0 + warp * 4 + j;
+            next[j] = b < b_end && lane < K ? __ldg(a.ent + ((int64_t)seg.var * W + b) * K + lane) : make_int2(-1, 0);
+        }
+    };
+    fetch(b_begin);
     for (int c = lane; c < C; c += 64) {
         constexpr int PER = MT / kW;                   // a warp's nodes, two categories a lane at a time
         const float* row = a.table + seg.table + (int64_t)(m0 + warp * PER) * C + c;
@@ -297,29 +300,46 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_staged_kernel(FwdArgs a) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             float* to = part + c * (MT + 1) + warp * PER + i;
-            to[0] = a.take_log ? logf(v[0][i]) : v[0][i];
-            if (c + 32 < C) to[32 * (MT + 1)] = a.take_log ? logf(v[1][i]) : v[1][i];
+            to[0] = LOG ? logf(v[0][i]) : v[0][i];
+            if (c + 32 < C) to[32 * (MT + 1)] = LOG ? logf(v[1][i]) : v[1][i];
         }
     }
+    if (threadIdx.x < MT) part[C * (MT + 1) + threadIdx.x] = 0.0f;
     __syncthreads();
-    const int b_end = min(W, (int)(blockIdx.y + 1) * a.per_b);
-    for (int b0 = blockIdx.y * a.per_b; b0 < b_end; b0 += 32) {
-        const int2* e[4];
-        float acc[4][NV] = {};
+    for (int b0 = b_begin; b0 < b_end; b0 += 32) {
+        int2 now[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) now[j] = next[j];
+        fetch(b0 + 32);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int b = b0 + warp * 4 + j;
-            e[j] = b < b_end ? a.ent + ((int64_t)seg.var * W + b) * K : nullptr;
+            if (b >= b_end) break;
+            const int2* e = a.ent + ((int64_t)seg.var * W + b) * K;
+            float acc[NV] = {};
+            for (int k0 = 0; k0 < K; k0 += 32) {
+                const int2 own = k0 == 0 ? now[j] : k0 + lane < K ? __ldg(e + k0 + lane) : make_int2(-1, 0);
+                const int n = __popc(__ballot_sync(~0u, own.x >= 0));
+                if (__any_sync(~0u, own.x >= C)) {     // a category that the table does not have
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) acc[i] = PCX_NEG_INF;
+                    break;
+                }
+                const int row = (own.x < 0 ? C : own.x) * (MT + 1);          // empty slots look at the row of zeros
+                const float weight = __int_as_float(own.y);
+                for (int k = 0; k < n; k += 4)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const float* v = part + __shfl_sync(~0u, row, k + h) + lane;
+                        const float q = __shfl_sync(~0u, weight, k + h);
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) acc[i] = fmaf(q, v[32 * i], acc[i]);
+                    }
+                if (n < 32) break;
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) tile[(32 * i + lane) * 33 + warp * 4 + j] = acc[i];
         }
-        four_rows<NV>(e, K, C, acc, [&](int c, float q, float (&s)[NV]) {
-            const float* v = part + c * (MT + 1) + lane;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) s[i] = fmaf(q, v[32 * i], s[i]);
-        });
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < NV; ++i) tile[(32 * i + lane) * 33 + warp * 4 + j] = acc[j][i];
         __syncthreads();
         store_rows<NV>(tile, a.out + (seg.row0 + m0) * W + b0, seg.M - m0, b_end - b0, W);
         __syncthreads();
@@ -633,14 +653,16 @@ struct BwdArgs {
     int C, mode, c_tiles, m_tiles, c_tile;             // mode 0: written, all of it; 1: added; 2: added to the turned table
 };
 
-// c_tile (at most 32) categories x NV * 32 nodes of one group.  The slots of the tile's categories, side by side after the sort,
+constexpr int kMaxTile = 64;       // categories of a tile
+
+// c_tile categories x NV * 32 nodes of one group.  The slots of the tile's categories, side by side after the sort,
 // are dealt out to the warps in equal parts; a warp walks its part in order, lanes over the nodes, and closes a category's
 // sum where the next begins.  A category that an earlier warp began is added to that warp's sum afterwards, in order.
 template <int NV>
-__global__ void __launch_bounds__(kTh) teacher_bwd_kernel(BwdArgs a) {
-    constexpr int MT = 32 * NV, AHEAD = NV > 4 ? 4 : 8;
+__global__ void __launch_bounds__(kTh, 3) teacher_bwd_kernel(BwdArgs a) {
+    constexpr int MT = 32 * NV, AHEAD = 4;
     extern __shared__ float acc[];                     // [c_tile][MT + 1], then [kW][MT]
-    __shared__ int from[33];
+    __shared__ int from[kMaxTile + 1], carry[kW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int64_t at = blockIdx.x;
     const int c0 = (int)(at % a.c_tiles) * a.c_tile;
@@ -659,60 +681,67 @@ __global__ void __launch_bounds__(kTh) teacher_bwd_kernel(BwdArgs a) {
         const int64_t base = (int64_t)set_begin(a.g, grp.set) * a.g.W * a.g.K;
         const int2* slots = a.slots + base;
         const int32_t* keys = a.keys + base;
-        const float* v_at[NV / 4];                     // lanes without a node look at the group's first
+        const uint32_t stride = (uint32_t)mp * 4;
+        const char* flow_at[NV / 4];                   // lanes without a node look at the group's first
 #pragma unroll
         for (int i = 0; i < NV / 4; ++i) {
             const int m = m0 + i * 128 + lane * 4;
-            v_at[i] = a.flows + grp.gbase * a.g.W + (m < mp ? m : 0);
+            flow_at[i] = (const char*)(a.flows + grp.gbase * a.g.W + (m < mp ? m : 0));
         }
         const int per = (end - begin + kW - 1) / kW;
         const int lo = min(end, begin + warp * per), hi = min(end, lo + per);
+        if (lane == 0) carry[warp] = -1;
         if (lo < hi) {
             float s[NV] = {};
-            int cur = keys[lo];
-            float* to = lo > from[cur - c0] ? part + warp * MT : acc + (cur - c0) * (MT + 1);
+            int cur = keys[lo] - c0;
+            const bool later = lo > from[cur];
+            if (later && lane == 0) carry[warp] = cur;
+            float* to = later ? part + warp * MT : acc + cur * (MT + 1);
             auto close = [&]() {
 #pragma unroll
                 for (int i = 0; i < NV; ++i) { to[node_of<true>(lane, i)] = s[i]; s[i] = 0.0f; }
             };
-            for (int j0 = lo; j0 < hi; j0 += AHEAD) {
-                int c[AHEAD];
-                float q[AHEAD];
-                float4 v[AHEAD][NV / 4];
+            for (int j0 = lo; j0 < hi; j0 += 32) {
+                const int n = min(32, hi - j0);
+                const int2 own = lane < n ? __ldg(slots + j0 + lane) : make_int2(0, 0);
+                const int key = lane < n ? __ldg(keys + j0 + lane) - c0 : -1;
+                int before = __shfl_up_sync(~0u, key, 1);
+                if (lane == 0) before = cur;
+                const unsigned opens = __ballot_sync(~0u, lane < n && key != before);
+                auto some = [&](int k, auto whole) {   // the next AHEAD slots, or what is left of them
+                    float q[AHEAD];
+                    float4 v[AHEAD][NV / 4];
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int j = min(j0 + i, hi - 1);
-                    const int2 e = __ldg(slots + j);
-                    c[i] = __ldg(keys + j);
-                    q[i] = __int_as_float(e.y);
+                    for (int h = 0; h < AHEAD; ++h) {
+                        const int place = __shfl_sync(~0u, own.x, k + h);
+                        q[h] = __int_as_float(__shfl_sync(~0u, own.y, k + h));
+                        if (whole.value || k + h < n) {
 #pragma unroll
-                    for (int k = 0; k < NV / 4; ++k) v[i][k] = __ldg((const float4*)(v_at[k] + (int64_t)e.x * mp));
-                }
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    if (j0 + i >= hi) break;
-                    if (c[i] != cur) {
-                        close();
-                        cur = c[i];
-                        to = acc + (cur - c0) * (MT + 1);
+                            for (int i = 0; i < NV / 4; ++i) v[h][i] = __ldg(row_at<float4>(flow_at[i], place, stride));
+                        }
                     }
 #pragma unroll
-                    for (int k = 0; k < NV / 4; ++k) {
-                        s[4 * k] = fmaf(q[i], v[i][k].x, s[4 * k]); s[4 * k + 1] = fmaf(q[i], v[i][k].y, s[4 * k + 1]);
-                        s[4 * k + 2] = fmaf(q[i], v[i][k].z, s[4 * k + 2]); s[4 * k + 3] = fmaf(q[i], v[i][k].w, s[4 * k + 3]);
+                    for (int h = 0; h < AHEAD; ++h) {
+                        if (!whole.value && k + h >= n) break;
+                        if (opens >> (k + h) & 1) {
+                            close();
+                            to = acc + __shfl_sync(~0u, key, k + h) * (MT + 1);
+                        }
+#pragma unroll
+                        for (int i = 0; i < NV / 4; ++i) fma4(q[h], v[h][i], s + 4 * i);
                     }
-                }
+                };
+                int k = 0;
+                for (; k + AHEAD <= n; k += AHEAD) some(k, std::true_type());
+                if (k < n) some(k, std::false_type());
+                cur = __shfl_sync(~0u, key, n - 1);
             }
             close();
         }
         __syncthreads();
-        if (per > 0 && tid < MT)
-            for (int w = 1; w < kW; ++w) {
-                const int l = begin + w * per;
-                if (l >= end) break;
-                const int c = keys[l] - c0;
-                if (l > from[c]) acc[c * (MT + 1) + tid] += part[w * MT + tid];
-            }
+        if (tid < MT)
+            for (int w = 1; w < kW; ++w)
+                if (carry[w] >= 0) acc[carry[w] * (MT + 1) + tid] += part[w * MT + tid];
         __syncthreads();
     }
     if (a.mode == 2) {
@@ -724,14 +753,27 @@ __global__ void __launch_bounds__(kTh) teacher_bwd_kernel(BwdArgs a) {
         }
         return;
     }
-    const int n_lanes = a.c_tile, rows = kTh / n_lanes;       // lanes side by side over the categories
-    const int cc = tid % n_lanes;
+    float* out = a.out + grp.out + (int64_t)m0 * grp.C + c0;
+    if (a.mode == 0 && grp.C % 4 == 0 && ((uintptr_t)out & 15) == 0) {       // four categories a thread
+        const int n_lanes = a.c_tile / 4, cc = tid % n_lanes * 4;
+        if (cc >= nc) return;
+        bool has[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) has[i] = from[cc + i] != from[cc + i + 1];
+        for (int m = tid / n_lanes; m < nm; m += kTh / n_lanes) {
+            const float* v = acc + cc * (MT + 1) + m;
+            *(float4*)(out + (int64_t)m * grp.C + cc) = make_float4(has[0] ? v[0] : 0.0f, has[1] ? v[MT + 1] : 0.0f,
+                                                                   has[2] ? v[2 * (MT + 1)] : 0.0f, has[3] ? v[3 * (MT + 1)] : 0.0f);
+        }
+        return;
+    }
+    const int n_lanes = a.c_tile, cc = tid % n_lanes;  // lanes side by side over the categories
     if (cc >= nc) return;
     const bool has = from[cc] != from[cc + 1];
-    float* p = a.out + grp.out + (int64_t)m0 * grp.C + c0 + cc;
-    for (int m = tid / n_lanes; m < nm; m += rows) {
-        if (a.mode == 0) p[(int64_t)m * grp.C] = has ? acc[cc * (MT + 1) + m] : 0.0f;
-        else if (has) p[(int64_t)m * grp.C] += acc[cc * (MT + 1) + m];
+    for (int m = tid / n_lanes; m < nm; m += kTh / n_lanes) {
+        float* p = out + (int64_t)m * grp.C + cc;
+        if (a.mode == 0) *p = has ? acc[cc * (MT + 1) + m] : 0.0f;
+        else if (has) *p += acc[cc * (MT + 1) + m];
     }
 }
 
@@ -816,11 +858,15 @@ int pcx_teacher_prep(void* entries, const void* ids, int wide_ids, int64_t ids_b
                      int dtype, int64_t logits_b, int64_t logits_v, int64_t logits_k, const float* norms, int64_t norms_b,
                      int64_t norms_v, int batch, int vars, int slots, int width, double temperature, void* stream) {
     if (vars <= 0 || width <= 0 || slots <= 0) return 0;
-    const int64_t blocks = pcx_cdiv((int64_t)vars * width, kW);
+    const int lanes = slots <= 32 ? 8 : slots <= 64 ? 16 : 32;
+    const int64_t blocks = pcx_cdiv((int64_t)vars * width, kTh / lanes);
     if (blocks > 0x7fffffff || dtype < 0 || dtype > 2) return -1;
     PrepArgs a{(int2*)entries, ids, logits, norms, ids_b, ids_v, ids_k, logits_b, logits_v, logits_k, norms_b, norms_v, wide_ids,
                dtype, batch, width, vars, slots, (float)(1.0 / temperature), 1.0 / temperature};
-    teacher_prep_kernel<<<(unsigned)blocks, kTh, 0, (cudaStream_t)stream>>>(a);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (lanes == 8) teacher_prep_kernel<8><<<(unsigned)blocks, kTh, 0, st>>>(a);
+    else if (lanes == 16) teacher_prep_kernel<16><<<(unsigned)blocks, kTh, 0, st>>>(a);
+    else teacher_prep_kernel<32><<<(unsigned)blocks, kTh, 0, st>>>(a);
     PCX_LAUNCH_CHECK();
     return 0;
 }
@@ -844,7 +890,7 @@ int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int
 int pcx_teacher_staged_nodes(int cats, int nodes) {
     for (int nm = 4; nm; nm >>= 1) {
         if (nm > 1 && nodes <= 16 * nm) continue;
-        if ((int64_t)4 * (32 * nm * 33 + (int64_t)cats * (32 * nm + 1)) <= (nm > 1 ? 110 : 220) * 1024) return 32 * nm;
+        if ((int64_t)4 * (32 * nm * 33 + (int64_t)(cats + 1) * (32 * nm + 1)) <= (nm > 1 ? 110 : 220) * 1024) return 32 * nm;
     }
     return 0;
 }
@@ -868,7 +914,7 @@ int pcx_teacher_fwd(float* out, const float* table, const void* entries, const P
     if (mt == 0) return -1;
     a.m_tiles = (int)pcx_cdiv(geo->nodes, mt);
     const int64_t tiles = (int64_t)a.m_tiles * geo->n_segs;
-    if (tiles > 0x7fffffff || turned_stride > 0x7fffffff) return -1;
+    if (tiles > 0x7fffffff || turned_stride >= 1 << 30) return -1;
     // positions per CTA: all of them where the table has to be staged first, unless few CTAs would be left
     const int64_t splits = std::max<int64_t>(1, std::min(pcx_cdiv(geo->width, 32), form == 2 ? pcx_cdiv(148, tiles) : (int64_t)65535));
     a.per_b = (int)(pcx_cdiv(pcx_cdiv(geo->width, splits), 32) * 32);
@@ -881,18 +927,24 @@ int pcx_teacher_fwd(float* out, const float* table, const void* entries, const P
     } else if (form == 3) {
         teacher_fwd_turned_kernel<true, 8><<<grid, kTh, tile_bytes, st>>>(a);
     } else {
-        const int bytes = tile_bytes + geo->cats * (mt + 1) * 4;
+        const int bytes = tile_bytes + (geo->cats + 1) * (mt + 1) * 4;
         static PcxOnce done;
         if (!done) {
-            for (const void* k : {(const void*)teacher_fwd_staged_kernel<4>, (const void*)teacher_fwd_staged_kernel<2>, (const void*)teacher_fwd_staged_kernel<1>}) {
+            for (const void* k : {(const void*)teacher_fwd_staged_kernel<4, false>, (const void*)teacher_fwd_staged_kernel<2, false>,
+                                  (const void*)teacher_fwd_staged_kernel<1, false>, (const void*)teacher_fwd_staged_kernel<4, true>,
+                                  (const void*)teacher_fwd_staged_kernel<2, true>, (const void*)teacher_fwd_staged_kernel<1, true>}) {
                 const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
                 if (e != cudaSuccess) return (int)e;
             }
             done = true;
         }
-        if (mt == 128) teacher_fwd_staged_kernel<4><<<grid, kTh, bytes, st>>>(a);
-        else if (mt == 64) teacher_fwd_staged_kernel<2><<<grid, kTh, bytes, st>>>(a);
-        else teacher_fwd_staged_kernel<1><<<grid, kTh, bytes, st>>>(a);
+        auto launch = [&](auto nv) {
+            if (take_log) teacher_fwd_staged_kernel<nv.value, true><<<grid, kTh, bytes, st>>>(a);
+            else teacher_fwd_staged_kernel<nv.value, false><<<grid, kTh, bytes, st>>>(a);
+        };
+        if (mt == 128) launch(std::integral_constant<int, 4>());
+        else if (mt == 64) launch(std::integral_constant<int, 2>());
+        else launch(std::integral_constant<int, 1>());
     }
     PCX_LAUNCH_CHECK();
     return 0;
@@ -973,7 +1025,7 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     a.first = (const int32_t*)(base + l.first);
     // nodes and categories per CTA: as many as leave every SM four CTAs
     int mt = geo->nodes > 128 ? 256 : 128;
-    a.c_tile = 32;
+    a.c_tile = kMaxTile;
     auto ctas = [&]() { return pcx_cdiv(geo->cats, a.c_tile) * pcx_cdiv(geo->nodes, mt) * geo->n_groups; };
     while (a.c_tile > 8 && ctas() < 148 * 4) a.c_tile /= 2;
     if (ctas() < 148 * 4) mt = 128;
@@ -981,6 +1033,14 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     a.m_tiles = (int)pcx_cdiv(geo->nodes, mt);
     if (ctas() > 0x7fffffff) return -1;
     const int bytes = (a.c_tile * (mt + 1) + kW * mt) * 4;
+    static PcxOnce done;
+    if (!done) {
+        for (const void* k : {(const void*)teacher_bwd_kernel<4>, (const void*)teacher_bwd_kernel<8>}) {
+            const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 76 * 1024);
+            if (e != cudaSuccess) return (int)e;
+        }
+        done = true;
+    }
     if (mt == 256) teacher_bwd_kernel<8><<<(unsigned)ctas(), kTh, bytes, st>>>(a);
     else teacher_bwd_kernel<4><<<(unsigned)ctas(), kTh, bytes, st>>>(a);
     PCX_LAUNCH_CHECK();
