@@ -204,6 +204,22 @@ def call(name: str, *args) -> None:
     raise PcxError(f"{name} failed with status {rc}")
 
 
+def launch(name: str, device: torch.device, *args) -> None:
+    """`call` for arguments that are plain already (addresses of tensors known to be on ``device``): the host time of a call
+    is what small operators take."""
+    lib = _lib if _lib is not None else load()
+    global COUNT
+    COUNT += 1
+    index = device.index
+    if PROFILE is None and index == torch._C._cuda_getDevice():
+        rc = getattr(lib, name)(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = _invoke(lib, name, args, args, device)
+    if rc != 0:
+        raise PcxError(f"{name} failed with status {rc}")
+
+
 def _invoke(lib, name, conv, args, dev) -> int:
     stream = torch.cuda.current_stream(dev).cuda_stream
     if PROFILE is None:

@@ -287,22 +287,20 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_staged_kernel(FwdArgs a) {
         }
     };
     fetch(b_begin);
-    for (int c = lane; c < C; c += 64) {
-        constexpr int PER = MT / kW;                   // a warp's nodes, two categories a lane at a time
+    constexpr int PER = MT / kW, AT_ONCE = 32 / PER;   // a warp's nodes; categories a lane fetches at a time
+    for (int c = lane; c < C; c += 32 * AT_ONCE) {
         const float* row = a.table + seg.table + (int64_t)(m0 + warp * PER) * C + c;
-        float v[2][PER];
+        float v[AT_ONCE][PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const bool in = m0 + warp * PER + i < seg.M;
-            v[0][i] = in ? __ldg(row + (int64_t)i * C) : 1.0f;
-            v[1][i] = in && c + 32 < C ? __ldg(row + (int64_t)i * C + 32) : 1.0f;
-        }
+        for (int i = 0; i < PER; ++i)
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            float* to = part + c * (MT + 1) + warp * PER + i;
-            to[0] = LOG ? logf(v[0][i]) : v[0][i];
-            if (c + 32 < C) to[32 * (MT + 1)] = LOG ? logf(v[1][i]) : v[1][i];
-        }
+            for (int h = 0; h < AT_ONCE; ++h)
+                v[h][i] = m0 + warp * PER + i < seg.M && c + 32 * h < C ? __ldg(row + (int64_t)i * C + 32 * h) : 1.0f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int h = 0; h < AT_ONCE; ++h)
+                if (c + 32 * h < C) part[(c + 32 * h) * (MT + 1) + warp * PER + i] = LOG ? logf(v[h][i]) : v[h][i];
     }
     if (threadIdx.x < MT) part[C * (MT + 1) + threadIdx.x] = 0.0f;
     __syncthreads();
@@ -526,6 +524,34 @@ __global__ void __launch_bounds__(1024) teacher_sort_small_kernel(SortArgs a) {
         }
 }
 
+// A set of at most 256 slots, a thread each: a slot's place is the number of smaller ones.
+constexpr int kTinySort = 256;
+__global__ void __launch_bounds__(kTinySort) teacher_sort_tiny_kernel(SortArgs a) {
+    __shared__ alignas(16) uint32_t comp[kTinySort];
+    const int u = blockIdx.x, first = set_begin(a.g, u), N = set_size(a.g, u) * a.g.W * a.g.K, j = threadIdx.x;
+    const int2 e = j < N ? set_entry(a.g, a.ent, first, j) : make_int2(0, 0);
+    const uint32_t own = j < N ? ((uint32_t)key_of_entry(e, a.C) << 12) | (uint32_t)j : ~0u;
+    comp[j] = own;
+    __syncthreads();
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < (int)blockDim.x; i += 4) {
+        const uint4 o = *(const uint4*)(comp + i);
+        rank += (int)(o.x < own) + (int)(o.y < own) + (int)(o.z < own) + (int)(o.w < own);
+    }
+    const int64_t base = (int64_t)first * a.g.W * a.g.K;
+    if (j < N) {
+        a.keys[base + rank] = (int)(own >> 12);
+        a.slots[base + rank] = make_int2(j / a.g.K, e.y);
+    }
+    if (a.first != nullptr)
+        for (int c = j; c <= a.C; c += blockDim.x) {   // slots with a smaller key
+            int n = 0;
+            for (int i = 0; i < N; ++i) n += (int)((int)(comp[i] >> 12) < c);
+            a.first[(int64_t)u * (a.C + 1) + c] = n;
+        }
+}
+
 template <bool FIRST>
 __device__ __forceinline__ int sort_key(const SortArgs& a, int first, int64_t base, int j) {
     return FIRST ? key_of_entry(set_entry(a.g, a.ent, first, j), a.C) : a.key_in[base + j];
@@ -659,8 +685,8 @@ constexpr int kMaxTile = 64;       // categories of a tile
 // are dealt out to the warps in equal parts; a warp walks its part in order, lanes over the nodes, and closes a category's
 // sum where the next begins.  A category that an earlier warp began is added to that warp's sum afterwards, in order.
 template <int NV>
-__global__ void __launch_bounds__(kTh, 3) teacher_bwd_kernel(BwdArgs a) {
-    constexpr int MT = 32 * NV, AHEAD = 4;
+__global__ void __launch_bounds__(kTh, 2) teacher_bwd_kernel(BwdArgs a) {
+    constexpr int MT = 32 * NV, AHEAD = NV > 4 ? 4 : 8;
     extern __shared__ float acc[];                     // [c_tile][MT + 1], then [kW][MT]
     __shared__ int from[kMaxTile + 1], carry[kW];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -777,13 +803,14 @@ __global__ void __launch_bounds__(kTh, 3) teacher_bwd_kernel(BwdArgs a) {
     }
 }
 
-// Few slots in large tables: only the categories that occur are visited, one warp each (mode 0: the caller has cleared the
+// Few slots in large tables: only the categories that occur are visited, L lanes each (mode 0: the caller has cleared the
 // output).
+template <int L>
 __global__ void __launch_bounds__(kTh) teacher_bwd_runs_kernel(BwdArgs a, int blocks) {
     const Grp grp = grp_of(a.g, blockIdx.x / blocks);
-    const int N = set_size(a.g, grp.set) * a.g.W * a.g.K, lane = threadIdx.x & 31;
+    const int N = set_size(a.g, grp.set) * a.g.W * a.g.K, lane = threadIdx.x % L;
     const int64_t base = (int64_t)set_begin(a.g, grp.set) * a.g.W * a.g.K;
-    const int j = (blockIdx.x % blocks) * kW + (threadIdx.x >> 5);
+    const int j = (blockIdx.x % blocks) * (kTh / L) + threadIdx.x / L;
     if (j >= N) return;
     const int32_t* keys = a.keys + base;
     const int c = keys[j];
@@ -792,7 +819,7 @@ __global__ void __launch_bounds__(kTh) teacher_bwd_runs_kernel(BwdArgs a, int bl
     while (end < N && keys[end] == c) ++end;
     const int mp = pad4(grp.M);
     const float* flows = a.flows + grp.gbase * a.g.W;
-    for (int m = lane; m < grp.M; m += 32) {
+    for (int m = lane; m < grp.M; m += L) {
         float s = 0.0f;
 #pragma unroll 4
         for (int i = j; i < end; ++i) {
@@ -971,8 +998,11 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     SortArgs s{};
     s.g = g; s.ent = (const int2*)entries; s.C = geo->cats; s.bits = l.bits;
     s.keys = (int32_t*)(base + l.keys); s.slots = (int2*)(base + l.slots);
-    if (l.small) {
-        s.first = runs ? nullptr : (int32_t*)(base + l.first);
+    s.first = runs ? nullptr : (int32_t*)(base + l.first);
+    if (l.n_max <= kTinySort) {
+        teacher_sort_tiny_kernel<<<geo->n_sets, (unsigned)(pcx_cdiv(l.n_max, 32) * 32), 0, st>>>(s);
+        PCX_LAUNCH_CHECK();
+    } else if (l.small) {
         const int warps = (int)std::max<int64_t>(1, pcx_cdiv(l.n_max, 128));
         const int bytes = warps * (2 * 128 * 4 + (2 << l.bits));
         static PcxOnce done;
@@ -1010,9 +1040,13 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     a.g = g; a.out = out; a.touched = touched; a.flows = turned; a.keys = s.keys; a.slots = s.slots; a.R = turned_stride;
     a.C = geo->cats; a.mode = mode;
     if (runs) {
-        const int64_t blocks = pcx_cdiv(l.n_max, kW);
+        const int lanes = geo->nodes >= 32 ? 32 : geo->nodes >= 8 ? 8 : 1;
+        const int64_t blocks = pcx_cdiv(l.n_max, kTh / lanes);
         if (blocks * geo->n_groups > 0x7fffffff) return -1;
-        teacher_bwd_runs_kernel<<<(unsigned)(blocks * geo->n_groups), kTh, 0, st>>>(a, (int)blocks);
+        const unsigned grid = (unsigned)(blocks * geo->n_groups);
+        if (lanes == 32) teacher_bwd_runs_kernel<32><<<grid, kTh, 0, st>>>(a, (int)blocks);
+        else if (lanes == 8) teacher_bwd_runs_kernel<8><<<grid, kTh, 0, st>>>(a, (int)blocks);
+        else teacher_bwd_runs_kernel<1><<<grid, kTh, 0, st>>>(a, (int)blocks);
         PCX_LAUNCH_CHECK();
         return 0;
     }

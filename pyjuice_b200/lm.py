@@ -9,6 +9,7 @@ tensors' device; nothing synchronises, and every call can be captured into a CUD
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import List, NamedTuple, Optional, Tuple
 
 import numpy as np
@@ -70,8 +71,9 @@ def _prepare(teacher: TopLogits, width: int, out: Optional[torch.Tensor] = None)
         out = torch.empty(T, width, K, 2, dtype=torch.int32, device=ids.device)
     if out.numel() > 0:
         nb, nv = (0, 0) if norm is None else norm.stride()
-        _lib.call("pcx_teacher_prep", out, ids, int(ids.dtype == torch.int64), *ids.stride(), x, _TYPES[x.dtype], *x.stride(),
-                  None if norm is None else norm.detach(), nb, nv, B, T, K, width, float(teacher.temperature))
+        _lib.launch("pcx_teacher_prep", ids.device, out.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), *ids.stride(),
+                    x.data_ptr(), _TYPES[x.dtype], *x.stride(), None if norm is None else norm.data_ptr(), nb, nv, B, T, K, width,
+                    float(teacher.temperature))
     return out
 
 
@@ -147,48 +149,65 @@ class LeafTables:
                   2 if turned_stride else 1, runs, turned_stride, int(logspace))
 
 
+@functools.lru_cache(maxsize=256)
+def _sizes(T: int, M: int, C: int, W: int, K: int, tied: bool):
+    """(`_Geo` of T positions of M nodes, its address, form of the forward pass, row width of the turned table, whether the
+    backward pass visits only categories that occur, bytes of its workspace)."""
+    n, lib = (1 if tied else T), _lib.load()
+    geo = _Geo(flow_cols=T * -(-M // 4) * 4, positions=T, nodes=M, cats=C, tied=int(tied), n_segs=T, n_groups=n, n_sets=n,
+               max_vars=T if tied else 1, total_vars=T, width=W, slots=K)
+    named = geo.max_vars * W * K                        # slots that look a table up
+    form = stride = 0
+    if not tied and named * 8 >= C and M > 1 and lib.pcx_teacher_staged_nodes(C, M) > 0:
+        form = 2
+    elif M > 1 and named * 4 >= C:
+        form, stride = (3 if tied or M % 4 == 0 else 1), -(-(n * M) // 4) * 4
+    runs = int(named * 16 < C)
+    at = ctypes.addressof(geo)
+    return geo, at, form, stride, runs, lib.pcx_teacher_bwd_scratch_bytes(at, runs)
+
+
+def _expect(log_probs, entries):
+    T, W, K, _ = entries.shape
+    M, C = log_probs.shape[-2:]
+    device = log_probs.device
+    out = torch.empty(T, M, W, dtype=torch.float32, device=device)
+    if out.numel() == 0 or K == 0:
+        return out.zero_()
+    tied = log_probs.dim() == 2
+    _, geo, form, stride, _, _ = _sizes(T, M, C, W, K, tied)
+    table = log_probs.contiguous()
+    if stride:
+        turned = torch.empty(C, stride, dtype=torch.float32, device=device)
+        _lib.launch("pcx_teacher_turn", device, turned.data_ptr(), table.data_ptr(), M if tied else T * M, C, stride)
+        table = turned
+    _lib.launch("pcx_teacher_fwd", device, out.data_ptr(), table.data_ptr(), entries.data_ptr(), geo, form, stride, 0)
+    return out
+
+
 class _Expected(torch.autograd.Function):
     """Values of leaf tables under prepared entries; the gradient of the tables."""
 
     @staticmethod
     def forward(ctx, log_probs, entries):
-        T, W, K, _ = entries.shape
-        M, C = log_probs.shape[-2:]
-        tied = log_probs.dim() == 2
-        M4 = -(-M // 4) * 4
-        n = 1 if tied else T
-        geo = _Geo(flow_cols=T * M4, positions=T, nodes=M, cats=C, tied=int(tied), n_segs=T, n_groups=n, n_sets=n,
-                   max_vars=T if tied else 1, total_vars=T, width=W, slots=K)
-        ctx.geo, ctx.shape = geo, log_probs.shape
-        ctx.save_for_backward(entries)
-        out = torch.empty(T, M, W, dtype=torch.float32, device=log_probs.device)
-        if out.numel() == 0 or K == 0:
-            return out.zero_()
-        table, form, stride = log_probs.contiguous(), 0, 0
-        named = geo.max_vars * W * K                    # slots that look a table up
-        if not tied and named * 8 >= C and M > 1 and _lib.load().pcx_teacher_staged_nodes(C, M) > 0:
-            form = 2
-        elif M > 1 and named * 4 >= C:
-            rows = n * M
-            stride = -(-rows // 4) * 4
-            turned = torch.empty(C, stride, dtype=torch.float32, device=table.device)
-            _lib.call("pcx_teacher_turn", turned, table, rows, C, stride)
-            table, form = turned, 3 if tied or M % 4 == 0 else 1
-        _lib.call("pcx_teacher_fwd", out, table, entries, ctypes.addressof(geo), form, stride, 0)
-        return out
+        ctx.entries, ctx.shape = entries, log_probs.shape         # (neither an input's memory nor an output's)
+        return _expect(log_probs, entries)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        entries, = ctx.saved_tensors
-        geo = ctx.geo
-        runs = geo.max_vars * geo.width * geo.slots * 16 < geo.cats
-        out = (torch.zeros if runs else torch.empty)(ctx.shape, dtype=torch.float32, device=entries.device)
-        if grad.numel() == 0 or geo.slots == 0:
-            return out.zero_(), None
-        scratch = torch.empty(_lib.load().pcx_teacher_bwd_scratch_bytes(ctypes.addressof(geo), int(runs)), dtype=torch.uint8,
-                              device=entries.device)
-        _lib.call("pcx_teacher_bwd", out, None, scratch, grad.contiguous(), entries, ctypes.addressof(geo), 0, int(runs), 0, 0)
+        if torch.is_grad_enabled() and grad.requires_grad:
+            raise RuntimeError("`expected_log_probs` is differentiable once")
+        entries, shape = ctx.entries, ctx.shape
+        T, W, K, _ = entries.shape
+        device = entries.device
+        if grad.numel() == 0 or K == 0:
+            return torch.zeros(shape, dtype=torch.float32, device=device), None
+        _, geo, _, _, runs, nbytes = _sizes(T, *shape[-2:], W, K, len(shape) == 2)
+        out = (torch.zeros if runs else torch.empty)(shape, dtype=torch.float32, device=device)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        grad = grad.contiguous()
+        _lib.launch("pcx_teacher_bwd", device, out.data_ptr(), None, scratch.data_ptr(), grad.data_ptr(), entries.data_ptr(), geo, 0,
+                    runs, 0, 0)
         return out, None
 
 
@@ -214,14 +233,24 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
     if max(B * K, 1) * (T if log_probs.dim() == 2 else 1) >= 2 ** 30:
         raise ValueError("more than 2^30 slots share a table")
     _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
-    return _Expected.apply(log_probs, _prepare(teacher, B))
+    entries = _prepare(teacher, B)
+    if log_probs.requires_grad and torch.is_grad_enabled():
+        return _Expected.apply(log_probs, entries)
+    return _expect(log_probs.detach(), entries)
+
+
+@functools.lru_cache(maxsize=None)
+def _sm_count(index: int) -> int:
+    return torch.cuda.get_device_properties(index).multi_processor_count
+
+
+_PART = 16                     # bytes of a part's statistics
 
 
 def _scratch(rows: int, vocab: int, n: int, device) -> Tuple[torch.Tensor, int]:
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        splits = lib.pcx_vocab_splits(rows, vocab)
-    return torch.empty(lib.pcx_vocab_scratch_bytes(rows, splits, n), dtype=torch.uint8, device=device), splits
+    """Workspace of a selection, and into how many parts a row is cut (as `pcx_vocab_splits`)."""
+    splits = max(1, min(-(-_sm_count(device.index) * 4 // rows), -(-vocab // 4096), 32))
+    return torch.empty(rows * (splits + 1) * (8 * n + _PART), dtype=torch.uint8, device=device), splits
 
 
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
@@ -251,8 +280,8 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     norms = torch.empty(lead, dtype=torch.float32, device=device)
     if rows > 0:
         scratch, splits = _scratch(rows, V, k, device)
-        _lib.call("pcx_top_logits", ids, values, norms, scratch, x, _TYPES[x.dtype], rows, V, x.stride(0), k, splits,
-                  float(temperature))
+        _lib.launch("pcx_top_logits", device, ids.data_ptr(), values.data_ptr(), norms.data_ptr(), scratch.data_ptr(), x.data_ptr(),
+                    _TYPES[x.dtype], rows, V, x.stride(0), k, splits, float(temperature))
     return TopLogits(ids, values, temperature, norms)
 
 
@@ -293,11 +322,13 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[in
     finished = None if finished is None else finished.contiguous()
     device = x.device
     out = torch.empty(B, n, dtype=torch.float32, device=device)
-    parents, tokens = torch.empty(2, B, n, dtype=torch.int64, device=device)
+    parents = torch.empty(B, n, dtype=torch.int64, device=device)
+    tokens = torch.empty(B, n, dtype=torch.int64, device=device)
     if B > 0:
         scratch, splits = _scratch(B * K, V, n, device)
-        _lib.call("pcx_beam_select", out, parents, tokens, scratch, x, _TYPES[x.dtype], scores, finished, B, K, V,
-                  x.stride(0), x.stride(1), n, pad_id, int(bool(normalize)), splits)
+        _lib.launch("pcx_beam_select", device, out.data_ptr(), parents.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), x.data_ptr(),
+                    _TYPES[x.dtype], scores.data_ptr(), None if finished is None else finished.data_ptr(), B, K, V, x.stride(0),
+                    x.stride(1), n, pad_id, int(bool(normalize)), splits)
     return out, parents, tokens
 
 
@@ -358,6 +389,6 @@ def reorder(parents: torch.Tensor, *states: torch.Tensor, dim: int = 0) -> List[
     for unit, group in by_unit.items():
         for i in range(0, len(group), 8):
             part = [v for _, row in group[i:i + 8] for v in row]
-            _lib.call("pcx_reorder", (ctypes.c_int64 * len(part))(*part), len(part) // 6, parents,
-                      int(parents.dtype == torch.int64), B, beams, n, unit)
+            _lib.launch("pcx_reorder", parents.device, (ctypes.c_int64 * len(part))(*part), len(part) // 6, parents.data_ptr(),
+                        int(parents.dtype == torch.int64), B, beams, n, unit)
     return out

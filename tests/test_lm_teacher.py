@@ -100,7 +100,8 @@ def make(T, M, C, B, K, tied, seed=0, ids=torch.int64, dtype=torch.float32, temp
 # (forms of the forward pass: tables in place, in shared memory, turned; of the sort: one CTA a set, radix of 1 to 3 passes; of
 # the backward pass: by categories that occur, by tiles of categories)
 SIZES = [(1, 1, 1, 1, 1), (1, 1, 2, 1, 3), (3, 5, 7, 2, 4), (2, 128, 256, 33, 16), (5, 33, 100, 31, 9), (4, 130, 64, 40, 8), (7, 64, 31, 1, 1),
-         (2, 16, 1600, 70, 12), (3, 9, 20000, 5, 10), (40, 1, 500, 3, 12), (2, 257, 1000, 65, 40), (1, 3, 200000, 2, 7), (2, 6, 70001, 90, 33)]
+         (2, 16, 1600, 70, 12), (3, 9, 20000, 5, 10), (40, 1, 500, 3, 12), (2, 257, 1000, 65, 40), (1, 3, 200000, 2, 7), (2, 6, 70001, 90, 33),
+         (8, 40, 600, 200, 4), (9, 300, 601, 200, 4), (8, 5, 70, 300, 3), (3, 70, 40, 500, 5)]
 
 
 @pytest.mark.gpu
@@ -204,6 +205,15 @@ def test_gradient_against_differences(tied):
     # values of up to |lp| + |d| / 2, each with K + 12 + 2 * SPREAD roundings, summed over 4 * 17 * 6 outputs with weights below 1
     tol = 408 * 2 * (19 + 220) * 2 * STEP * float(lp.detach().abs().max() + d.abs().max())
     assert abs(difference - float((grad.double() * d.double()).sum())) < tol
+
+
+@pytest.mark.gpu
+def test_a_second_derivative_is_refused():
+    lp, teacher = make(2, 5, 9, 3, 4, True)
+    lp.requires_grad_()
+    g = torch.ones(2, 5, 3, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(lm.expected_log_probs(lp, teacher), lp, g, create_graph=True)
 
 
 @pytest.mark.gpu
