@@ -573,12 +573,9 @@ int pcx_colplan_blob(const void* blob, const int32_t** data, int64_t* n_data, co
 int pcx_colplan_blob_free(void* blob);
 
 /* ---- Language-model operators: selection over a vocabulary ----------------------------------------------------------
- * dtype: 0 fp32, 1 bf16, 2 fp16.  n (entries of an answer) is at most 128.  `scratch`: pcx_vocab_scratch_bytes(rows, splits,
- * n) bytes, 16-byte aligned, used by one call at a time; `splits`: CTAs per row (pcx_vocab_splits gives a good number).
- * Rows may start at any multiple of the element size; the elements of a row are adjacent.  [No counterpart in the
- * reference.] */
-int pcx_vocab_splits(int64_t rows, int64_t vocab);
-int64_t pcx_vocab_scratch_bytes(int64_t rows, int splits, int n);
+ * dtype: 0 fp32, 1 bf16, 2 fp16.  n (entries of an answer) is at most 128.  `splits`: the parts a row is cut into (1 to 32),
+ * one CTA each, or 0 for a warp a row.  `scratch`: rows * (max(splits, 1) + 1) * (8 * n + 16) bytes, 16-byte aligned, used by
+ * one call at a time.  Rows may start at any multiple of the element size; the elements of a row are adjacent.  [No counterpart in the reference.] */
 /* The n largest logits of every row (largest first, a lower id first among equals; -inf and NaN are none: id -1, value
  * -inf) and norms[r] = log sum_v exp(logits[r][v] / temperature). */
 int pcx_top_logits(int64_t* ids, void* values, float* norms, void* scratch, const void* logits, int dtype, int64_t rows,

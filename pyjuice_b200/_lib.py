@@ -91,7 +91,6 @@ SIGNATURES = {
 PLAIN = {"pcx_build_arch": [], "pcx_column_clusters": [I, I], "pcx_column_chain_clusters": [I], "pcx_column_chain_bytes": [I, I, I, I], "pcx_set_sum_mode": [I], "pcx_set_dependent_launch": [I], "pcx_set_stage_event": [P], "pcx_get_status": [], "pcx_clear_status": [],
          "pcx_packed_tile_count": [L, I, I, I, I], "pcx_dense_scratch_bytes": [I, I, I],
          "pcx_sm_packed_bytes": [L, I, I], "pcx_dense2_scratch_bytes": [I, I, I],
-         "pcx_vocab_splits": [L, L], "pcx_vocab_scratch_bytes": [L, I, I],
          "pcx_teacher_staged_nodes": [I, I], "pcx_teacher_bwd_scratch_bytes": [P, I]}
 # the planner of the column program (host only; the last two arguments of those that may refuse: a text buffer and its size)
 PLAIN.update({"pcx_colplan_new": [P, L, P, L, P, P, I], "pcx_colplan_free": [P], "pcx_colplan_info": [P, P, P, P],
@@ -158,7 +157,7 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.restype = c_int64 if name in ("pcx_packed_tile_count", "pcx_dense_scratch_bytes", "pcx_sm_packed_bytes",
                                         "pcx_dense2_scratch_bytes", "pcx_column_chain_bytes",
-                                        "pcx_vocab_scratch_bytes", "pcx_teacher_bwd_scratch_bytes") else c_int
+                                        "pcx_teacher_bwd_scratch_bytes") else c_int
         fn.argtypes = list(args)
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)

@@ -1,14 +1,16 @@
 // Selection over a vocabulary: the largest logits of every row with the row's log-normaliser, and the best continuations of
 // beams.  The language-model side of the circuits: a teacher's top logits to learn from, beam search to answer with.
 //
-// One pass over the logits.  A CTA walks a part of a row in tiles that stay in registers; its threads carry the running
-// maximum m and sum s = sum exp((x - m) / T) of a softmax, and the CTA keeps the n largest logits seen so far, sorted, in
-// shared memory.  Once that list is full its smallest entry is a threshold that few later logits pass, so that a tile
-// costs one comparison per thread and a barrier.  Places are part of the keys (a lower place first among equals): keys are
-// unique, and the answer does not depend on how rows are split over CTAs or in which order threads append.
-// A row takes as many CTAs as are needed to fill the device; the lists and the (m, s) of the parts are joined by a second
-// kernel, one CTA per answer, which for beams also adds the scores, in 64 bits: a sum of a score and a logit is rounded
-// only in the returned score, never before it is compared.
+// One pass over the logits, which carries the running maximum m and sum s = sum exp((x - m) / T) of a softmax and the n largest
+// logits.  Places are part of the keys (a lower place first among equals), keys are unique, and the answer does not depend on
+// how rows are cut or in which order logits come.  Two forms, by the number of rows (see `launch_rows`):
+//   a warp a row   Its lanes leave the maximum of every four loads of 16 bytes in shared memory.  After (at most) 16 tiles of 4
+//                  KB a threshold is bisected over these maxima that n, or a few more, of them reach: so do n logits, and the
+//                  n largest are among the logits of those maxima, which alone are read again.
+//   CTAs a row     The CTA keeps the n largest so far; rows are cut into parts until the device is full, and a second kernel
+//                  joins their lists, one CTA per row.
+// For beams another kernel joins the rows of a sequence and adds the scores, in 64 bits: a sum of a score and a logit is
+// rounded only in the returned score, never before it is compared.
 #include "pcx_common.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -55,14 +57,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 16 bytes of logits: their maximum (NaN skipped) and the logits one by one.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
-    static constexpr int N = 4;
+    static constexpr int N = 4, UNUSED = 0;                // UNUSED: low bits that all values have alike as 32-bit numbers
     static __device__ __forceinline__ float max(const uint4& v) {
         return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
     static __device__ __forceinline__ float at(const uint4& v, int i) { return __uint_as_float((&v.x)[i]); }
 };
 template <> struct Pack<__nv_bfloat16> {
-    static constexpr int N = 8;
+    static constexpr int N = 8, UNUSED = 16;
     static __device__ __forceinline__ float max(const uint4& v) {
         const __nv_bfloat162* h = (const __nv_bfloat162*)&v;
         const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -74,7 +76,7 @@ template <> struct Pack<__nv_bfloat16> {
     }
 };
 template <> struct Pack<__half> {
-    static constexpr int N = 8;
+    static constexpr int N = 8, UNUSED = 13;
     static __device__ __forceinline__ float max(const uint4& v) {
         const __half2* h = (const __half2*)&v;
         const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
@@ -86,15 +88,22 @@ template <> struct Pack<__half> {
     }
 };
 
-// The 16 bytes of elements e ... of a row; -inf beyond its ends.
+// The 16 bytes of elements e ... of a row, -inf beyond its ends.  (Out of line, as everything that few tiles need: the warps
+// of an SM are in different places of the code, and it has to fit the instruction cache.)
 template <typename T>
-__device__ __forceinline__ uint4 load_group(const T* x, int e, int vocab) {
+__device__ __noinline__ uint4 load_edge(const T* x, int e, int vocab) {
     constexpr int VE = Pack<T>::N;
-    if (e >= 0 && e + VE <= vocab) return __ldcs((const uint4*)(x + e));
     T edge[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) edge[i] = e + i >= 0 && e + i < vocab ? x[e + i] : (T)PCX_NEG_INF;
     return *(const uint4*)edge;
+}
+// Group `gi` of a row; whole groups are [whole0, whole1), there is none from g1 on.
+template <typename T>
+__device__ __forceinline__ uint4 load_group(const T* x, int gi, int off, int whole0, int whole1, int g1, int vocab) {
+    constexpr int VE = Pack<T>::N;
+    if (gi >= whole0 && gi < whole1) return __ldg((const uint4*)(x + (int64_t)gi * VE - off));
+    return load_edge<T>(x, gi < g1 ? gi * VE - off : -VE, vocab);
 }
 
 struct RowArgs {
@@ -225,10 +234,301 @@ __device__ __forceinline__ void leave(const RowArgs& a, const Shared& sh, int64_
     }
 }
 
-// G groups of 16 bytes a thread and tile.
+constexpr int kRowWarps = 4, kGroups = 8;           // warps of a CTA; groups of 16 bytes a lane and tile
+constexpr int kQuad = 4;                            // groups that share a maximum
+constexpr int kChunk = 16, kMaxima = kChunk * 32 * (kGroups / kQuad);       // tiles whose maxima a warp holds
+constexpr int kSet = 320;                           // keys a warp holds
+
+// Cuts a warp's set of `count` (at least n) unique keys back to n ... n + n / 8 of the largest.  Returns how many are left;
+// `bound`: a key that n of them reach.
+__device__ __noinline__ int cut(u64* keys, int count, int n, u64* bound) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    uint32_t least = ~0u, most = 0;
+    for (int i = lane; i < count; i += 32) {
+        const uint32_t v = (uint32_t)(keys[i] >> 32);
+        least = min(least, v);
+        most = max(most, v);
+    }
+    u64 lo = (u64)__reduce_min_sync(~0u, least) << 32;                        // #(keys >= lo) >= n
+    if (count > n + n / 8) {
+        u64 hi = ((u64)__reduce_max_sync(~0u, most) << 32) | 0xffffffffu;
+        while (lo < hi) {
+            const u64 mid = lo + ((hi - lo) >> 1) + ((hi - lo) & 1);
+            int c = 0;
+            for (int i = lane; i < count; i += 32) c += keys[i] >= mid;
+            c = __reduce_add_sync(~0u, c);
+            if (c >= n) {
+                lo = mid;
+                if (c <= n + n / 8) break;
+            } else {
+                hi = mid - 1;
+            }
+        }
+        int kept = 0;
+        for (int i0 = 0; i0 < count; i0 += 32) {
+            const u64 k = i0 + lane < count ? keys[i0 + lane] : 0;
+            __syncwarp();
+            const unsigned stays = __ballot_sync(~0u, i0 + lane < count && k >= lo);
+            if (stays >> lane & 1) keys[kept + __popc(stays & ((1u << lane) - 1))] = k;
+            kept += __popc(stays);
+        }
+        count = kept;
+        __syncwarp();
+    }
+    *bound = lo;
+    return count;
+}
+
+// The sum over the lanes before this one; `n` becomes the sum over all.
+__device__ __forceinline__ int warp_before(int& n) {
+    const int lane = threadIdx.x & 31;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int y = __shfl_up_sync(~0u, x, o); if (lane >= o) x += y; }
+    const int before = x - n;
+    n = __shfl_sync(~0u, x, 31);
+    return before;
+}
+
+// What a lane's part of a tile adds to its sum when the quick way gave no number: NaN, infinities, or a maximum near the
+// largest number.
+template <typename T>
+__device__ __noinline__ float careful_sum(const T* x, int first, int groups, int step, int end, float m, float r, float scale) {
+    constexpr int VE = Pack<T>::N;
+    float s = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < groups * VE; ++i) {
+        const int e = first + i / VE * step + i % VE;
+        if (e < 0 || e >= end) continue;
+        const float f = fmaxf((float)x[e], PCX_NEG_INF);
+        s += exp2_fast(f == m ? 0.0f : fabsf(r) < CUDART_INF_F ? fmaf(f, scale, -r) : (f - m) * scale);
+    }
+    return s;
+}
+
+// Many rows, or short ones: a warp a row.
+template <typename T>
+__global__ void __launch_bounds__(kRowWarps * 32, 4)
+top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
+    constexpr int VE = Pack<T>::N, G = kGroups, H = G / kQuad;
+    constexpr int SIDE = 32 / (kQuad * VE), AHEAD = 12;                   // maxima whose logits fit the lanes; such steps at once
+    __shared__ alignas(16) u64 all_keys[kRowWarps][kSet];
+    __shared__ float all_maxima[kRowWarps][kMaxima];
+    __shared__ uint16_t all_hot[kRowWarps][kMaxima];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t row = (int64_t)blockIdx.x * kRowWarps + warp;
+    if (row >= n_rows) return;                      // (no barrier of the CTA follows)
+    u64* keys = all_keys[warp];                     // the largest so far, keys[0, count), unsorted
+    float* maxima = all_maxima[warp];
+    uint16_t* hot = all_hot[warp];
+    int count = 0;
+    u64 bound = 0;                                  // n keys of the set are at least this large; 0 before there are n
+    // The terms of a sum are 2^(x * scale - r) with r = m * scale rounded once: one fused operation each, and all of them
+    // relative to the same r.  What r is off is put right when the sum is read.
+    float m = PCX_NEG_INF, r = PCX_NEG_INF, s = 0.0f;
+    bool skip = a.finished != nullptr && a.finished[row] != 0;
+    if (a.scores != nullptr) skip |= !(a.scores[row] > PCX_NEG_INF);
+    if (!skip) {
+        const T* x = (const T*)a.logits + (row / a.inner) * a.stride0 + (row % a.inner) * a.stride1;
+        // groups begin on 16-byte boundaries; the first and the last may reach over the row's ends
+        const int off = (int)(((uintptr_t)x & 15) / sizeof(T));
+        const int groups = (int)(((int64_t)off + a.vocab + VE - 1) / VE);
+        // whole groups: those of the row's ends are read element by element
+        const int whole0 = off != 0 ? 1 : 0, whole1 = (off + a.vocab) / VE;
+        for (int chunk = 0; chunk < groups; chunk += 32 * G * kChunk) {
+            const int tiles = min(kChunk, (groups - chunk + 32 * G - 1) / (32 * G));
+            auto load = [&](uint4 (&v)[G], int t) {
+                const int g = chunk + t * 32 * G;
+                const T* mine = x + (int64_t)(g + lane) * VE - off;
+                if (g >= whole0 && g + 32 * G <= whole1) {
+#pragma unroll
+                    for (int j = 0; j < G; ++j) v[j] = __ldg((const uint4*)(mine + j * 32 * VE));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < G; ++j) v[j] = load_group<T>(x, g + j * 32 + lane, off, whole0, whole1, groups, a.vocab);
+                }
+            };
+            auto take = [&](const uint4 (&v)[G], int t) {
+                float top = PCX_NEG_INF;
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    float f = Pack<T>::max(v[h * kQuad]);
+#pragma unroll
+                    for (int j = 1; j < kQuad; ++j) f = fmaxf(f, Pack<T>::max(v[h * kQuad + j]));
+                    f = fmaxf(f, PCX_NEG_INF);      // (not NaN)
+                    maxima[(t * H + h) * 32 + lane] = f;
+                    top = fmaxf(top, f);
+                }
+                if (top > m) {
+                    const float nr = top * a.scale;
+                    const bool plain = fabsf(r) < CUDART_INF_F && fabsf(nr) < CUDART_INF_F;
+                    s = m > PCX_NEG_INF ? s * exp2_fast(plain ? r - nr : (m - top) * a.scale) : 0.0f;
+                    m = top;
+                    r = nr;
+                }
+                if (m > PCX_NEG_INF) {
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < G; ++j)
+#pragma unroll
+                        for (int i = 0; i < VE; i += 2) {
+                            s0 += exp2_fast(fmaf(Pack<T>::at(v[j], i), a.scale, -r));
+                            s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
+                        }
+                    s0 += s1;
+                    if (!(s0 < CUDART_INF_F) || !(fabsf(r) < CUDART_INF_F))
+                        s0 = careful_sum<T>(x, (chunk + t * 32 * G + lane) * VE - off, G, 32 * VE, a.vocab, m, r, a.scale);
+                    s += s0;
+                }
+            };
+            uint4 even[G], odd[G];                  // a tile is on its way while the one before is taken
+            load(even, 0);
+#pragma unroll 1
+            for (int t = 0; t < tiles; t += 2) {
+                if (t + 1 < tiles) load(odd, t + 1);
+                take(even, t);
+                if (t + 1 >= tiles) break;
+                if (t + 2 < tiles) load(even, t + 2);
+                take(odd, t + 1);
+            }
+            __syncwarp();
+            // the threshold: n, or a few more, of the maxima (and of the keys so far) are that large
+            const int n_max = tiles * H;            // maxima a lane
+            float own[kChunk * H];
+            float least = bound != 0 ? value_of(bound) : -3.402823466e38f;
+            float most = PCX_NEG_INF;
+            int pass = 0;
+#pragma unroll
+            for (int q = 0; q < kChunk * H; ++q) {
+                own[q] = q < n_max ? maxima[q * 32 + lane] : PCX_NEG_INF;
+                most = fmaxf(most, own[q]);
+                pass += own[q] >= least;
+            }
+            pass = __reduce_add_sync(~0u, pass);
+            if (pass == 0) continue;
+            if (pass > 2 * a.n) {
+                // (every lane's largest reaches the smallest of them: a start for n up to 32)
+                constexpr int BITS = Pack<T>::UNUSED;
+                const uint32_t top = ordered(most), all = a.n <= 32 ? __reduce_min_sync(~0u, top) : 0;
+                uint32_t lo = max(ordered(least), all) >> BITS, hi = __reduce_max_sync(~0u, top) >> BITS;
+#pragma unroll 1
+                while (lo < hi) {
+                    const uint32_t mid = lo + ((hi - lo) >> 1) + ((hi - lo) & 1);
+                    const float f = unordered(mid << BITS);
+                    int c = 0;
+#pragma unroll
+                    for (int q = 0; q < kChunk * H; ++q) c += own[q] >= f;
+                    c = __reduce_add_sync(~0u, c);
+                    if (c >= a.n) {
+                        lo = mid;
+                        if (c <= a.n + a.n / 4 + 4) break;
+                    } else {
+                        hi = mid - 1;
+                    }
+                }
+                least = unordered(lo << BITS);
+            }
+            int n_hot = 0;
+#pragma unroll
+            for (int q = 0; q < kChunk * H; ++q) n_hot += own[q] >= least;
+            int to = warp_before(n_hot);
+#pragma unroll
+            for (int q = 0; q < kChunk * H; ++q)
+                if (own[q] >= least) hot[to++] = (uint16_t)(q * 32 + lane);
+            __syncwarp();
+            // their logits, a lane for each
+            const int h_own = lane / (kQuad * VE), e_own = chunk * VE - off + lane / VE % kQuad * 32 * VE + lane % VE;
+            auto place = [&](int h) { return e_own + (hot[h] / 32 * kQuad * 32 + hot[h] % 32) * VE; };     // (quads lie one after the other)
+#pragma unroll 1
+            for (int h0 = h_own; h0 - h_own < n_hot; h0 += SIDE * AHEAD) {
+                float f[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int h = h0 + i * SIDE;
+                    f[i] = PCX_NEG_INF;
+                    if (h < n_hot) {
+                        const int e = place(h);
+                        if (e >= 0 && e < a.vocab) f[i] = (float)x[e];
+                    }
+                }
+                unsigned wanted = 0;
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) wanted |= (unsigned)(f[i] >= least) << i;
+                int n_new = __popc(wanted);
+                int at_key = warp_before(n_new);
+                if (count + n_new <= kSet) {        // the usual case
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i)
+                        if (wanted >> i & 1) keys[count + at_key++] = key_of(f[i], (uint32_t)place(h0 + i * SIDE));
+                    count += n_new;
+                } else {                            // many equal or ordered logits: a few at a time, the set cut in between
+#pragma unroll
+                    for (int i = 0; i < AHEAD; ++i) {
+                        if (count > kSet - 32) count = cut(keys, count, a.n, &bound);
+                        const u64 key = wanted >> i & 1 ? key_of(f[i], (uint32_t)place(h0 + i * SIDE)) : 0;
+                        const bool fits = key != 0 && key >= bound;
+                        const unsigned lanes = __ballot_sync(~0u, fits);
+                        if (fits) keys[count + __popc(lanes & ((1u << lane) - 1))] = key;
+                        count += __popc(lanes);
+                    }
+                }
+                __syncwarp();
+            }
+            if (count >= a.n && chunk + 32 * G * kChunk < groups) count = cut(keys, count, a.n, &bound);
+            __syncwarp();
+        }
+    }
+    // statistics in fp32, then what the largest lane's r was off
+    float M = m;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
+    const float R = M * a.scale;
+    const bool plain = fabsf(R) < CUDART_INF_F;
+    s = m > PCX_NEG_INF ? s * exp2_fast(plain && fabsf(r) < CUDART_INF_F ? r - R : (m - M) * a.scale) : 0.0f;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    const double S = M > PCX_NEG_INF && M < CUDART_INF_F
+        ? plain ? (double)s * (1.0 + (double)fmaf(-M, a.scale, R) * 0.6931471805599453) : (double)s : 0.0;
+    // the set in order: a key's place is the number of larger ones
+    if (count > a.n + a.n / 2 + 16) count = cut(keys, count, a.n, &bound);
+    __syncwarp();
+    const int have = min(count, a.n);
+    if (lane == 0) {
+        if (a.ids == nullptr) a.parts[row] = Part{M, have, S};
+        else a.norms[row] = (float)log_norm(M, S, a.inv_t);
+    }
+#pragma unroll 1
+    for (int i = lane; i < count; i += 32) {
+        const u64 k = keys[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < (count & ~1); j += 2) {
+            const ulonglong2 o = *(const ulonglong2*)(keys + j);
+            rank += (int)(o.x > k) + (int)(o.y > k);
+        }
+        if (count & 1) rank += (int)(keys[count - 1] > k);
+        if (rank >= a.n) continue;
+        if (a.ids == nullptr) {
+            a.keys[row * a.n + rank] = k;
+        } else {
+            a.ids[row * a.n + rank] = (int64_t)place_of(k);
+            ((T*)a.values)[row * a.n + rank] = (T)value_of(k);
+        }
+    }
+    if (a.ids != nullptr)
+        for (int i = have + lane; i < a.n; i += 32) {
+            a.ids[row * a.n + i] = -1;
+            ((T*)a.values)[row * a.n + i] = (T)PCX_NEG_INF;
+        }
+}
+
+// Few rows: a CTA a row or part of one, tiles of G groups of 16 bytes a thread.  The CTA keeps the n largest logits so far,
+// sorted; the last of them is a bound that few later logits pass, so that a tile costs a comparison a thread and a barrier.
+// The first tile's bound comes from its threads' maxima.
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, G > 4 ? 3 : 4)
-top_rows_kernel(RowArgs a) {
+top_rows_block_kernel(RowArgs a) {
     constexpr int VE = Pack<T>::N;
     __shared__ Shared sh;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -247,14 +547,12 @@ top_rows_kernel(RowArgs a) {
         const int groups = (int)(((int64_t)off + a.vocab + VE - 1) / VE);
         const int per = (groups + a.splits - 1) / a.splits;
         const int g0 = part * per, g1 = min(groups, g0 + per);
+        const int whole0 = off != 0 ? 1 : 0, whole1 = (off + a.vocab) / VE;
         float bound = PCX_NEG_INF;             // value of the last entry of a full list
         for (int g = g0; g < g1; g += kThreads * G) {
             uint4 v[G];
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                const int gi = g + j * kThreads + tid;
-                v[j] = load_group<T>(x, gi < g1 ? gi * VE - off : -VE, a.vocab);
-            }
+            for (int j = 0; j < G; ++j) v[j] = load_group<T>(x, g + j * kThreads + tid, off, whole0, min(g1, whole1), g1, a.vocab);
             float top = PCX_NEG_INF, group_top[G];
 #pragma unroll
             for (int j = 0; j < G; ++j) {
@@ -278,16 +576,8 @@ top_rows_kernel(RowArgs a) {
                         s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
                     }
                 s0 += s1;
-                if (!(s0 < CUDART_INF_F) || !(fabsf(r) < CUDART_INF_F)) {        // NaN, infinities, or |m| near the largest number
-                    s0 = 0.0f;
-#pragma unroll 1
-                    for (int i = 0; i < G * VE; ++i) {
-                        const int gi = g + i / VE * kThreads + tid, e = gi * VE - off + i % VE;
-                        if (gi >= g1 || e < 0 || e >= a.vocab) continue;
-                        const float f = fmaxf((float)x[e], PCX_NEG_INF);
-                        s0 += exp2_fast(f == m ? 0.0f : fabsf(r) < CUDART_INF_F ? fmaf(f, a.scale, -r) : (f - m) * a.scale);
-                    }
-                }
+                if (!(s0 < CUDART_INF_F) || !(fabsf(r) < CUDART_INF_F))
+                    s0 = careful_sum<T>(x, (g + tid) * VE - off, G, kThreads * VE, min(a.vocab, g1 * VE - off), m, r, a.scale);
                 s += s0;
             }
             const int over = __syncthreads_count(top > bound);
@@ -322,7 +612,7 @@ top_rows_kernel(RowArgs a) {
             auto each = [&](u64 from, auto&& found) {
                 for (uint32_t left = hot; left != 0; left &= left - 1) {
                     const int e = (g + (__ffs(left) - 1) * kThreads + tid) * VE - off;
-                    const uint4 w = load_group<T>(x, e, a.vocab);
+                    const uint4 w = load_group<T>(x, g + (__ffs(left) - 1) * kThreads + tid, off, whole0, min(g1, whole1), g1, a.vocab);
 #pragma unroll
                     for (int i = 0; i < VE; ++i) {
                         const float f = Pack<T>::at(w, i);
@@ -546,25 +836,23 @@ __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
     ((U*)t.dst)[at] = u;
 }
 
-int sm_count() {
-    static int counts[64] = {};
-    int d = 0;
-    if (cudaGetDevice(&d) != cudaSuccess || d < 0 || d >= 64) return 148;
-    if (counts[d] == 0 && cudaDeviceGetAttribute(&counts[d], cudaDevAttrMultiProcessorCount, d) != cudaSuccess) counts[d] = 148;
-    return counts[d];
-}
-
 template <typename T>
-void launch_rows(const RowArgs& a, int64_t rows, cudaStream_t stream) {
+void launch_rows(const RowArgs& a, int64_t rows, bool warps, cudaStream_t stream) {
+    if (warps) {
+        top_rows_warp_kernel<T><<<(unsigned)pcx_cdiv(rows, kRowWarps), kRowWarps * 32, 0, stream>>>(a, rows);
+        return;
+    }
     const unsigned grid = (unsigned)(rows * a.splits);
     const int64_t groups = a.vocab / Pack<T>::N / a.splits;
-    if (groups > 3 * kThreads) top_rows_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
-    else top_rows_kernel<T, 2><<<grid, kThreads, 0, stream>>>(a);
+    if (groups > 3 * kThreads) top_rows_block_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
+    else top_rows_block_kernel<T, 2><<<grid, kThreads, 0, stream>>>(a);
 }
 
 // The lists of all rows, one part each when this returns: in the answer's place, or in `keys` and `parts`.
 template <typename T>
 int select_rows(RowArgs a, void* scratch, int64_t rows, cudaStream_t stream) {
+    const bool warps = a.splits == 0;
+    if (warps) a.splits = 1;
     const int64_t lists = rows * a.splits;
     u64* keys = (u64*)scratch;
     Part* parts = (Part*)(keys + lists * a.n);
@@ -575,12 +863,12 @@ int select_rows(RowArgs a, void* scratch, int64_t rows, cudaStream_t stream) {
     rows_args.parts = parts;
     if (a.splits == 1) {
         if (a.ids == nullptr) { rows_args.keys = joined_keys; rows_args.parts = joined_parts; }
-        launch_rows<T>(rows_args, rows, stream);
+        launch_rows<T>(rows_args, rows, warps, stream);
         PCX_LAUNCH_CHECK();
         return 0;
     }
     rows_args.ids = nullptr;
-    launch_rows<T>(rows_args, rows, stream);
+    launch_rows<T>(rows_args, rows, warps, stream);
     PCX_LAUNCH_CHECK();
     a.keys = joined_keys;
     a.parts = joined_parts;
@@ -601,21 +889,10 @@ int select_rows(const RowArgs& a, int dtype, void* scratch, int64_t rows, cudaSt
 
 extern "C" {
 
-// CTAs per row: enough to give every SM four, none of less than 4096 logits.
-int pcx_vocab_splits(int64_t rows, int64_t vocab) {
-    if (rows <= 0 || vocab <= 0) return 1;
-    const int64_t want = pcx_cdiv((int64_t)sm_count() * 4, rows);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, pcx_cdiv(vocab, 4096), kMaxSplits}));
-}
-
-int64_t pcx_vocab_scratch_bytes(int64_t rows, int splits, int n) {
-    return rows * (splits + 1) * ((int64_t)n * 8 + (int64_t)sizeof(Part));
-}
-
 int pcx_top_logits(int64_t* ids, void* values, float* norms, void* scratch, const void* logits, int dtype, int64_t rows,
                    int vocab, int64_t row_stride, int n, int splits, double temperature, void* stream) {
     if (rows <= 0 || n <= 0) return 0;
-    if (n > kMaxTop || vocab <= 0 || splits < 1 || splits > kMaxSplits || rows * splits > 0x7fffffff) return -1;
+    if (n > kMaxTop || vocab <= 0 || splits < 0 || splits > kMaxSplits || rows * std::max(splits, 1) > 0x7fffffff) return -1;
     RowArgs a{};
     a.logits = logits;
     a.stride1 = row_stride;
@@ -632,8 +909,8 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
                     int64_t stride_beam, int n, int pad_id, int normalize, int splits, void* stream) {
     if (batch <= 0 || n <= 0) return 0;
     const int64_t rows = batch * beams;
-    if (n > kMaxTop || vocab <= 0 || beams <= 0 || beams > kMaxTop || splits < 1 || splits > kMaxSplits ||
-        (int64_t)beams * vocab > 0x7fffffff || rows * splits > 0x7fffffff)
+    if (n > kMaxTop || vocab <= 0 || beams <= 0 || beams > kMaxTop || splits < 0 || splits > kMaxSplits ||
+        (int64_t)beams * vocab > 0x7fffffff || rows * std::max(splits, 1) > 0x7fffffff)
         return -1;
     RowArgs a{};
     a.logits = logits; a.scores = scores; a.finished = finished;
@@ -644,7 +921,7 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
     const int rc = select_rows(a, dtype, scratch, rows, (cudaStream_t)stream);
     if (rc != 0) return rc;
     BeamArgs j{};
-    j.keys = (const u64*)((const char*)scratch + rows * splits * ((int64_t)n * 8 + (int64_t)sizeof(Part)));
+    j.keys = (const u64*)((const char*)scratch + rows * std::max(splits, 1) * ((int64_t)n * 8 + (int64_t)sizeof(Part)));
     j.parts = (const Part*)(j.keys + rows * n);
     j.scores = scores; j.finished = finished;
     j.out_scores = out_scores; j.tokens = tokens; j.parents = parents;
