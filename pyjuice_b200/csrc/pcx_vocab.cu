@@ -805,11 +805,13 @@ join_beams_kernel(BeamArgs a) {
 
 // ---- reordering of states --------------------------------------------------------------------------------------------
 constexpr int kStates = 8;                          // tensors moved by one launch
+constexpr int kMoveRows = 8, kMoveUnits = 8;        // outer rows, and units of a row, that a thread moves
 struct Moved {
     const char* src;
     char* dst;
     int64_t outer, chunks, src_outer, src_beam;     // rows before the beams, units per beam, strides in bytes
-    int64_t first_block;
+    int64_t first_block, column_blocks, segments;   // blocks: columns, then segments of a beam's units, then outer rows
+    int lanes;                                      // threads side by side over a beam's units
 };
 struct MoveArgs {
     Moved t[kStates];
@@ -819,21 +821,44 @@ struct MoveArgs {
 };
 
 // dst[o, b * n + j, i] = src[o, b * beams + parents[b, j], i], in units of sizeof(U) bytes; zeros for a parent that is none
-// of the sequence's beams.  A thread moves one unit; neighbours write neighbouring units.
+// of the sequence's beams.  A thread looks its parent up once for up to 8 outer rows and 8 units of each, all of which it
+// has under way together; neighbours write neighbouring units.
 template <typename U>
 __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
     int w = 0;
     while (w + 1 < a.n_tensors && (int64_t)blockIdx.x >= a.t[w + 1].first_block) ++w;
     const Moved& t = a.t[w];
-    const int64_t at = ((int64_t)blockIdx.x - t.first_block) * 256 + threadIdx.x;
-    if (at >= t.outer * a.columns * t.chunks) return;
-    const int64_t i = at % t.chunks, r = at / t.chunks;
-    const int64_t c = r % a.columns, o = r / a.columns;
+    int64_t block = (int64_t)blockIdx.x - t.first_block;
+    const int64_t c = block % t.column_blocks * (256 / t.lanes) + threadIdx.x / t.lanes;
+    block /= t.column_blocks;
+    if (c >= a.columns) return;
+    const int64_t i0 = block % t.segments * (t.lanes * kMoveUnits) + threadIdx.x % t.lanes;
+    const int64_t o0 = block / t.segments * kMoveRows;
     const int64_t p = a.wide_ids ? ((const int64_t*)a.parents)[c] : (int64_t)((const int32_t*)a.parents)[c];
-    U u = {};
-    if (p >= 0 && p < a.beams)
-        u = *(const U*)(t.src + o * t.src_outer + (c / a.n * a.beams + p) * t.src_beam + i * (int64_t)sizeof(U));
-    ((U*)t.dst)[at] = u;
+    const bool is = p >= 0 && p < a.beams;
+    const char* src = t.src + o0 * t.src_outer + (c / a.n * a.beams + (is ? p : 0)) * t.src_beam;
+    U* dst = (U*)t.dst + (o0 * a.columns + c) * t.chunks;
+    const int rows = (int)min((int64_t)kMoveRows, t.outer - o0);
+    if (t.chunks <= t.lanes) {                      // a unit a row
+        if (i0 >= t.chunks) return;
+        U u[kMoveRows] = {};
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r)
+            if (r < rows && is) u[r] = ((const U*)(src + r * t.src_outer))[i0];
+#pragma unroll
+        for (int r = 0; r < kMoveRows; ++r)
+            if (r < rows) dst[r * a.columns * t.chunks + i0] = u[r];
+        return;
+    }
+    for (int r = 0; r < rows; ++r) {
+        U u[kMoveUnits] = {};
+#pragma unroll
+        for (int k = 0; k < kMoveUnits; ++k)
+            if (i0 + k * t.lanes < t.chunks && is) u[k] = ((const U*)(src + r * t.src_outer))[i0 + k * t.lanes];
+#pragma unroll
+        for (int k = 0; k < kMoveUnits; ++k)
+            if (i0 + k * t.lanes < t.chunks) dst[r * a.columns * t.chunks + i0 + k * t.lanes] = u[k];
+    }
 }
 
 template <typename T>
@@ -944,11 +969,13 @@ int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int w
     for (int i = 0; i < n_tensors; ++i) {
         const int64_t* s = states + 6 * i;
         if (s[3] % unit != 0) return -1;
-        a.t[a.n_tensors] = Moved{(const char*)s[0], (char*)s[1], s[2], s[3] / unit, s[4], s[5], blocks};
-        const int64_t units = s[2] * a.columns * (s[3] / unit);
-        if (units == 0) continue;
-        a.n_tensors += 1;
-        blocks += pcx_cdiv(units, 256);
+        const int64_t chunks = s[3] / unit;
+        if (s[2] == 0 || chunks == 0) continue;
+        int lanes = 1;
+        while (lanes < 256 && lanes < chunks) lanes *= 2;
+        const int64_t column_blocks = pcx_cdiv(a.columns, 256 / lanes), segments = pcx_cdiv(chunks, (int64_t)lanes * kMoveUnits);
+        a.t[a.n_tensors++] = Moved{(const char*)s[0], (char*)s[1], s[2], chunks, s[4], s[5], blocks, column_blocks, segments, lanes};
+        blocks += column_blocks * segments * pcx_cdiv(s[2], kMoveRows);
     }
     if (blocks == 0) return 0;
     if (blocks > 0x7fffffff) return -1;
