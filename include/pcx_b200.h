@@ -626,8 +626,8 @@ typedef struct PcxTeacherGeo {
 int pcx_teacher_prep(void* entries, const void* ids, int wide_ids, int64_t ids_b, int64_t ids_v, int64_t ids_k, const void* logits,
                      int dtype, int64_t logits_b, int64_t logits_v, int64_t logits_k, const float* norms, int64_t norms_b,
                      int64_t norms_v, int batch, int vars, int slots, int width, double temperature, void* stream);
-/* out[c * stride + r] = table[r * cats + c], 0 for r in [rows, stride). */
-int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int64_t stride, void* stream);
+/* out[c * stride + r] = table[r * cats + c] (its logarithm if take_log), 0 for r in [rows, stride). */
+int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int64_t stride, int take_log, void* stream);
 /* Nodes per CTA of form 2 of the forward pass; 0: tables of that many categories do not fit. */
 int pcx_teacher_staged_nodes(int cats, int nodes);
 /* form 0: the tables are read where they lie; 1: `table` is turned ([cats][turned_stride]); 2: the tables go through shared

@@ -392,15 +392,15 @@ __device__ __forceinline__ void turn_tile(float (*tile)[kTurn + 1], const float*
     }
 }
 
-// [R][C] -> [C][stride].
-template <bool VEC_IN, bool VEC_OUT>
+// [R][C] -> [C][stride], of logarithms if asked.
+template <bool VEC_IN, bool VEC_OUT, bool LOG>
 __global__ void __launch_bounds__(kTh) teacher_turn_kernel(float* __restrict__ out, const float* __restrict__ in, int64_t R, int C,
                                                           int64_t stride, int64_t r_tiles) {
     __shared__ float tile[kTurn][kTurn + 1];
     const int64_t r0 = (int64_t)(blockIdx.x % r_tiles) * kTurn;
     const int c0 = (int)(blockIdx.x / r_tiles) * kTurn;
     turn_tile<VEC_IN, VEC_OUT>(tile, in + r0 * C + c0, C, (int)max((int64_t)0, min((int64_t)kTurn, R - r0)), min(kTurn, C - c0),
-                               out + c0 * stride + r0, stride, (int)min((int64_t)kTurn, stride - r0), [](float v) { return v; });
+                               out + c0 * stride + r0, stride, (int)min((int64_t)kTurn, stride - r0), [](float v) { return LOG ? logf(v) : v; });
 }
 
 // Flows [node][sample] -> [sample][node] of every vector, exponentials if they are logarithms; padding nodes are 0.
@@ -898,17 +898,21 @@ int pcx_teacher_prep(void* entries, const void* ids, int wide_ids, int64_t ids_b
     return 0;
 }
 
-int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int64_t stride, void* stream) {
+int pcx_teacher_turn(float* out, const float* table, int64_t rows, int cats, int64_t stride, int take_log, void* stream) {
     if (rows <= 0 || cats <= 0) return 0;
     const int64_t r_tiles = pcx_cdiv(stride, kTurn), blocks = r_tiles * pcx_cdiv(cats, kTurn);
     if (blocks > 0x7fffffff) return -1;
     const bool in4 = cats % 4 == 0 && (uintptr_t)table % 16 == 0, out4 = stride % 4 == 0 && (uintptr_t)out % 16 == 0;
     const unsigned grid = (unsigned)blocks;
     cudaStream_t st = (cudaStream_t)stream;
-    if (in4 && out4) teacher_turn_kernel<true, true><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
-    else if (out4) teacher_turn_kernel<false, true><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
-    else if (in4) teacher_turn_kernel<true, false><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
-    else teacher_turn_kernel<false, false><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
+    auto launch = [&](auto vec_in, auto vec_out) {
+        if (take_log) teacher_turn_kernel<vec_in.value, vec_out.value, true><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
+        else teacher_turn_kernel<vec_in.value, vec_out.value, false><<<grid, kTh, 0, st>>>(out, table, rows, cats, stride, r_tiles);
+    };
+    if (in4 && out4) launch(std::true_type(), std::true_type());
+    else if (out4) launch(std::false_type(), std::true_type());
+    else if (in4) launch(std::true_type(), std::false_type());
+    else launch(std::false_type(), std::false_type());
     PCX_LAUNCH_CHECK();
     return 0;
 }

@@ -148,7 +148,7 @@ class HMMDecoder:
         rows = self._speak._values_of_inner([(self._heard_ns, state)], N)
         W = rows.size(1)
         out = torch.empty(W, self._v_pad, device=self.device)
-        _lib.call("pcx_teacher_turn", out, rows, self._v_pad, W, self._v_pad)
+        _lib.call("pcx_teacher_turn", out, rows, self._v_pad, W, self._v_pad, 0)
         return out[:N, :self.vocab]
 
     @torch.no_grad()

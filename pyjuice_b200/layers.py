@@ -375,7 +375,7 @@ class InputLayer(Layer, nn.Module):
 
     def _leaf_tables(self) -> LeafTables:
         if self._teacher_tables is None:
-            self._teacher_tables = LeafTables(self._vectors, self._shadow["C"] if self._shadow is not None else 0, self.device)
+            self._teacher_tables = LeafTables(self._vectors, self.num_parameters, self.device)
         return self._teacher_tables
 
     def _init_parameters(self, perturbation: float):

@@ -90,13 +90,28 @@ class Entries:
         return (self.tensor.data_ptr(), *self.tensor.shape)
 
 
+def _form(named: int, C: int, M: int, own: bool) -> int:
+    """How the forward pass reads tables of M nodes and C categories that ``named`` slots each look up (``own``: the table
+    belongs to one position).  2, through shared memory, takes the whole table once: tables of one position, at least an
+    eighth of whose categories are named, as long as 64 of their nodes fit (196 tables of 256 x 256, batch 100, 16 slots:
+    47 us, 62 turned, 387 in place; 64 of 512 x 1000, batch 77: 86, 68, 209).  3, turned, writes and reads the table once more
+    but then finds the nodes of a category side by side: from a quarter of the categories on.  0, in place, touches a sector
+    of 32 bytes per slot and node."""
+    if own and M > 1 and named * 8 >= C and _lib.load().pcx_teacher_staged_nodes(C, M) >= min(64, M):
+        return 2
+    return 3 if M > 1 and named * 4 >= C else 0
+
+
 class LeafTables:
     """The leaf vectors of an input layer as the teacher's kernels walk them: vectors, groups that share a table (in the
     order of their first vector), and the variables of each group."""
 
-    def __init__(self, vectors, cats_per_row: int, device):
+    def __init__(self, vectors, num_params: int, device):
         """``vectors``: (variable, nodes, categories, first row of the value buffers, first parameter, first flow or None for a
-        tied vector) of every leaf vector."""
+        tied vector) of every leaf vector; ``num_params``: parameters of all of them."""
+        cats = {v[2] for v in vectors}
+        cats_per_row = min(cats) if len(cats) == 1 else 0           # (tables can be turned as one)
+        self.rows = num_params // cats_per_row if cats_per_row else 0
         segs, groups, sets, by_table = [], [], {}, {}
         for v in vectors:
             by_table.setdefault(v[4], []).append(v)
@@ -129,14 +144,20 @@ class LeafTables:
 
     def forward(self, node_mars: torch.Tensor, params: torch.Tensor, entries: Entries, turned_stride: int = 0):
         """``params``: probabilities of the tables, or (``turned_stride``) their transposed logarithms."""
-        geo = self.geo(entries)
-        if turned_stride:
+        geo, take_log = self.geo(entries), 1
+        form = 3 if turned_stride else _form(self._named(entries), geo.cats, geo.nodes, geo.max_vars == 1)
+        if form == 3 and not turned_stride:
+            if 0 < self.rows < 2 ** 29:
+                turned_stride = -(-self.rows // 4) * 4
+                turned = torch.empty(geo.cats, turned_stride, dtype=torch.float32, device=params.device)
+                _lib.call("pcx_teacher_turn", turned, params, self.rows, geo.cats, turned_stride, 1)
+                params = turned
+            else:
+                form = 0
+        if form == 3:
+            take_log = 0
             form = 3 if self.cols_by_four and turned_stride % 4 == 0 else 1
-        else:
-            form = 2 if (self._named(entries) * 8 >= geo.cats and
-                         _lib.load().pcx_teacher_staged_nodes(geo.cats, geo.nodes) > 0) else 0
-        _lib.call("pcx_teacher_fwd", node_mars, params, entries.tensor, ctypes.addressof(geo), form, turned_stride,
-                  int(turned_stride == 0))
+        _lib.call("pcx_teacher_fwd", node_mars, params, entries.tensor, ctypes.addressof(geo), form, turned_stride, take_log)
 
     def backward(self, flows: torch.Tensor, node_flows: torch.Tensor, entries: Entries, logspace: bool, turned_stride: int = 0,
                  touched: Optional[torch.Tensor] = None):
@@ -157,11 +178,10 @@ def _sizes(T: int, M: int, C: int, W: int, K: int, tied: bool):
     geo = _Geo(flow_cols=T * -(-M // 4) * 4, positions=T, nodes=M, cats=C, tied=int(tied), n_segs=T, n_groups=n, n_sets=n,
                max_vars=T if tied else 1, total_vars=T, width=W, slots=K)
     named = geo.max_vars * W * K                        # slots that look a table up
-    form = stride = 0
-    if not tied and named * 8 >= C and M > 1 and lib.pcx_teacher_staged_nodes(C, M) > 0:
-        form = 2
-    elif M > 1 and named * 4 >= C:
-        form, stride = (3 if tied or M % 4 == 0 else 1), -(-(n * M) // 4) * 4
+    form, stride = _form(named, C, M, not tied), 0
+    if form == 3:                                       # (rows of a turned table are addressed with 32 bits)
+        stride = -(-(n * M) // 4) * 4 if n * M < 2 ** 29 else 0
+        form = 0 if stride == 0 else 3 if tied or M % 4 == 0 else 1
     runs = int(named * 16 < C)
     at = ctypes.addressof(geo)
     return geo, at, form, stride, runs, lib.pcx_teacher_bwd_scratch_bytes(at, runs)
@@ -179,7 +199,7 @@ def _expect(log_probs, entries):
     table = log_probs.contiguous()
     if stride:
         turned = torch.empty(C, stride, dtype=torch.float32, device=device)
-        _lib.launch("pcx_teacher_turn", device, turned.data_ptr(), table.data_ptr(), M if tied else T * M, C, stride)
+        _lib.launch("pcx_teacher_turn", device, turned.data_ptr(), table.data_ptr(), M if tied else T * M, C, stride, 0)
         table = turned
     _lib.launch("pcx_teacher_fwd", device, out.data_ptr(), table.data_ptr(), entries.data_ptr(), geo, form, stride, 0)
     return out
@@ -232,6 +252,8 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
         raise ValueError("tables of 1 to 1000000 categories are supported")
     if max(B * K, 1) * (T if log_probs.dim() == 2 else 1) >= 2 ** 30:
         raise ValueError("more than 2^30 slots share a table")
+    if T * log_probs.size(-2) >= 2 ** 31:
+        raise ValueError("more than 2^31 nodes over all positions")
     _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
     entries = _prepare(teacher, B)
     if log_probs.requires_grad and torch.is_grad_enabled():

@@ -27,6 +27,7 @@ STRUCTURES = {
     "hmm-shadow": lambda: pj.structures.HMM(seq_length=7, num_latents=32, num_emits=600),
     "hmm-vocabulary": lambda: pj.structures.HMM(seq_length=5, num_latents=32, num_emits=9001),
     "hmm-untied": lambda: pj.structures.HMM(seq_length=5, num_latents=20, num_emits=33, homogeneous=False),
+    "hclt-many-cats": lambda: hclt(16, 700, 5),
     "pd": lambda: pj.structures.PD((4, 4), num_latents=8, split_points=[[2], [2]], num_cats=7),
     "rat": lambda: pj.structures.RAT_SPN(num_vars=16, num_latents=8, depth=2, num_repetitions=3, num_cats=6),
 }
@@ -222,7 +223,7 @@ def test_tables_of_the_leaf_vectors():
         random.seed(4)
         pc = pj.compile(STRUCTURES[name](), verbose=False)
         for layer in pc.input_layer_group:
-            t = lm.LeafTables(layer._vectors, 0, "cpu")
+            t = lm.LeafTables(layer._vectors, layer.num_parameters, "cpu")
             seg = t._held[0].numpy().view(np.dtype([("var", "i4"), ("M", "i4"), ("C", "i4"), ("col", "i4"), ("row0", "i8"), ("table", "i8"), ("flow_col", "i8")]))
             grp = t._held[1].numpy().view(np.dtype([("set", "i4"), ("M", "i4"), ("C", "i4"), ("col", "i4"), ("out", "i8"), ("flow_col", "i8")]))
             first, vars_ = t._held[2].numpy().view(np.int32), t._held[3].numpy().view(np.int32)

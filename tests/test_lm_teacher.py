@@ -101,7 +101,7 @@ def make(T, M, C, B, K, tied, seed=0, ids=torch.int64, dtype=torch.float32, temp
 # the backward pass: by categories that occur, by tiles of categories)
 SIZES = [(1, 1, 1, 1, 1), (1, 1, 2, 1, 3), (3, 5, 7, 2, 4), (2, 128, 256, 33, 16), (5, 33, 100, 31, 9), (4, 130, 64, 40, 8), (7, 64, 31, 1, 1),
          (2, 16, 1600, 70, 12), (3, 9, 20000, 5, 10), (40, 1, 500, 3, 12), (2, 257, 1000, 65, 40), (1, 3, 200000, 2, 7), (2, 6, 70001, 90, 33),
-         (8, 40, 600, 200, 4), (9, 300, 601, 200, 4), (8, 5, 70, 300, 3), (3, 70, 40, 500, 5)]
+         (2, 3, 400, 3, 300), (3, 2, 50, 2, 60), (8, 40, 600, 200, 4), (9, 300, 601, 200, 4), (8, 5, 70, 300, 3), (3, 70, 40, 500, 5)]
 
 
 @pytest.mark.gpu
@@ -261,8 +261,11 @@ def test_forms_of_the_forward_pass_agree(form, tied):
                   n_sets=1 if tied else T, max_vars=T if tied else 1, total_vars=T, width=B, slots=K)
     table, stride = lp, 0
     if form in (1, 3):
-        table = lp.reshape(-1, C).t().contiguous()
-        stride = table.size(1)
+        rows, stride = lp.numel() // C, lp.numel() // C
+        for take_log, source in ((0, lp), (1, lp.exp())):
+            table = torch.full((C, stride), NAN, device="cuda")
+            _lib.call("pcx_teacher_turn", table, source, rows, C, stride, take_log)
+            assert float((table - lp.reshape(-1, C).t()).abs().max()) <= take_log * 4 * STEP * float(lp.abs().max()) * 8
     out = torch.full((T, M, B), NAN, device="cuda")
     _lib.call("pcx_teacher_fwd", out, table, entries, ctypes.addressof(geo), form, stride, 0)
     want, size = expected(lp, teacher)
