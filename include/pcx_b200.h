@@ -634,7 +634,13 @@ int pcx_teacher_staged_nodes(int cats, int nodes);
  * memory; 3: as 1, with turned_stride and all `col` multiples of 4.  take_log (forms 0, 2): the tables hold probabilities. */
 int pcx_teacher_fwd(float* out, const float* table, const void* entries, const PcxTeacherGeo* geo, int form, int64_t turned_stride,
                     int take_log, void* stream);
-/* mode 0: all of `out` is written (runs: only categories that occur, the caller has cleared it); 1: added; 2: added to a turned
+/* Preparation, turning (form 1 or 3: `turned` has room for cats rows of turned_stride) and forward pass of tables of logarithms
+ * in one call, for a geometry without tables of its own. */
+int pcx_teacher_expect(float* out, void* entries, float* turned, const float* table, const void* ids, int wide_ids, int64_t ids_b,
+                       int64_t ids_v, int64_t ids_k, const void* logits, int dtype, int64_t logits_b, int64_t logits_v, int64_t logits_k,
+                       const float* norms, int64_t norms_b, int64_t norms_v, int batch, double temperature, const PcxTeacherGeo* geo,
+                       int form, int64_t turned_stride, void* stream);
+/* mode 0: all of `out` is written; 1: added; 2: added to a turned
  * table, touched[c] = 1 for the categories that occur.  runs: visit only categories that occur.  logspace: flows are
  * logarithms.  `scratch`: pcx_teacher_bwd_scratch_bytes, 256-byte aligned. */
 int64_t pcx_teacher_bwd_scratch_bytes(const PcxTeacherGeo* geo, int runs);

@@ -84,6 +84,7 @@ SIGNATURES = {
     "pcx_teacher_prep": [P, P, I, L, L, L, P, I, L, L, L, P, L, L, I, I, I, I, D],
     "pcx_teacher_turn": [P, P, L, I, L, I],
     "pcx_teacher_fwd": [P, P, P, P, I, L, I],
+    "pcx_teacher_expect": [P, P, P, P, P, I, L, L, L, P, I, L, L, L, P, L, L, I, D, P, I, L],
     "pcx_teacher_bwd": [P, P, P, P, P, P, I, I, L, I],
 }
 

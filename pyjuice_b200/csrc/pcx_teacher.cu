@@ -803,8 +803,8 @@ __global__ void __launch_bounds__(kTh, 2) teacher_bwd_kernel(BwdArgs a) {
     }
 }
 
-// Few slots in large tables: only the categories that occur are visited, L lanes each (mode 0: the caller has cleared the
-// output).
+// Few slots in large tables: only the categories that occur are visited, L lanes each, in an output that has been cleared
+// (mode 0).
 template <int L>
 __global__ void __launch_bounds__(kTh) teacher_bwd_runs_kernel(BwdArgs a, int blocks) {
     const Grp grp = grp_of(a.g, blockIdx.x / blocks);
@@ -981,6 +981,22 @@ int pcx_teacher_fwd(float* out, const float* table, const void* entries, const P
     return 0;
 }
 
+// Preparation, turning (form 1 or 3: `turned` has room for cats rows of turned_stride) and forward pass in one call.
+int pcx_teacher_expect(float* out, void* entries, float* turned, const float* table, const void* ids, int wide_ids, int64_t ids_b,
+                       int64_t ids_v, int64_t ids_k, const void* logits, int dtype, int64_t logits_b, int64_t logits_v, int64_t logits_k,
+                       const float* norms, int64_t norms_b, int64_t norms_v, int batch, double temperature, const PcxTeacherGeo* geo,
+                       int form, int64_t turned_stride, void* stream) {
+    int rc = pcx_teacher_prep(entries, ids, wide_ids, ids_b, ids_v, ids_k, logits, dtype, logits_b, logits_v, logits_k, norms, norms_b,
+                              norms_v, batch, geo->positions, geo->slots, geo->width, temperature, stream);
+    if (rc != 0) return rc;
+    if (form == 1 || form == 3) {
+        rc = pcx_teacher_turn(turned, table, (int64_t)geo->n_groups * geo->nodes, geo->cats, turned_stride, 0, stream);
+        if (rc != 0) return rc;
+        table = turned;
+    }
+    return pcx_teacher_fwd(out, table, entries, geo, form, turned_stride, 0, stream);
+}
+
 int64_t pcx_teacher_bwd_scratch_bytes(const PcxTeacherGeo* geo, int runs) { return layout(geo, runs != 0).total; }
 
 int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* flows, const void* entries, const PcxTeacherGeo* geo,
@@ -1044,6 +1060,10 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     a.g = g; a.out = out; a.touched = touched; a.flows = turned; a.keys = s.keys; a.slots = s.slots; a.R = turned_stride;
     a.C = geo->cats; a.mode = mode;
     if (runs) {
+        if (mode == 0) {
+            const cudaError_t e = cudaMemsetAsync(out, 0, (size_t)geo->n_groups * geo->nodes * geo->cats * 4, st);
+            if (e != cudaSuccess) return (int)e;
+        }
         const int lanes = geo->nodes >= 32 ? 32 : geo->nodes >= 8 ? 8 : 1;
         const int64_t blocks = pcx_cdiv(l.n_max, kTh / lanes);
         if (blocks * geo->n_groups > 0x7fffffff) return -1;

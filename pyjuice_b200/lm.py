@@ -65,7 +65,7 @@ class _Geo(ctypes.Structure):
 
 def _prepare(teacher: TopLogits, width: int, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Categories and weights of a teacher's slots, ``[T, width, K]`` pairs of 32 bits, from ids ``[B, T, K]``."""
-    ids, x, norm = teacher.ids, teacher.logits.detach(), teacher.log_norm
+    ids, x, norm = teacher.ids, teacher.logits, teacher.log_norm
     B, T, K = ids.shape
     if out is None:
         out = torch.empty(T, width, K, 2, dtype=torch.int32, device=ids.device)
@@ -187,31 +187,33 @@ def _sizes(T: int, M: int, C: int, W: int, K: int, tied: bool):
     return geo, at, form, stride, runs, lib.pcx_teacher_bwd_scratch_bytes(at, runs)
 
 
-def _expect(log_probs, entries):
-    T, W, K, _ = entries.shape
+def _expect(log_probs, teacher):
+    """Values and the prepared slots of the teacher."""
+    ids, x, norm, device = teacher.ids, teacher.logits, teacher.log_norm, log_probs.device
+    B, T, K = ids.shape
     M, C = log_probs.shape[-2:]
-    device = log_probs.device
-    out = torch.empty(T, M, W, dtype=torch.float32, device=device)
-    if out.numel() == 0 or K == 0:
-        return out.zero_()
-    tied = log_probs.dim() == 2
-    _, geo, form, stride, _, _ = _sizes(T, M, C, W, K, tied)
+    entries = torch.empty(T, B, K, 2, dtype=torch.int32, device=device)
+    out = torch.empty(T, M, B, dtype=torch.float32, device=device)
+    if T * M * B * K == 0:
+        return out.zero_(), entries
+    _, geo, form, stride, _, _ = _sizes(T, M, C, B, K, log_probs.dim() == 2)
     table = log_probs.contiguous()
-    if stride:
-        turned = torch.empty(C, stride, dtype=torch.float32, device=device)
-        _lib.launch("pcx_teacher_turn", device, turned.data_ptr(), table.data_ptr(), M if tied else T * M, C, stride, 0)
-        table = turned
-    _lib.launch("pcx_teacher_fwd", device, out.data_ptr(), table.data_ptr(), entries.data_ptr(), geo, form, stride, 0)
-    return out
+    turned = torch.empty(C, stride, dtype=torch.float32, device=device) if stride else None
+    nb, nv = (0, 0) if norm is None else norm.stride()
+    _lib.launch("pcx_teacher_expect", device, out.data_ptr(), entries.data_ptr(), None if turned is None else turned.data_ptr(),
+                table.data_ptr(), ids.data_ptr(), int(ids.dtype == torch.int64), *ids.stride(), x.data_ptr(), _TYPES[x.dtype],
+                *x.stride(), None if norm is None else norm.data_ptr(), nb, nv, B, float(teacher.temperature), geo, form, stride)
+    return out, entries
 
 
 class _Expected(torch.autograd.Function):
-    """Values of leaf tables under prepared entries; the gradient of the tables."""
+    """Values of leaf tables under a teacher; the gradient of the tables."""
 
     @staticmethod
-    def forward(ctx, log_probs, entries):
-        ctx.entries, ctx.shape = entries, log_probs.shape         # (neither an input's memory nor an output's)
-        return _expect(log_probs, entries)
+    def forward(ctx, log_probs, teacher):
+        out, ctx.entries = _expect(log_probs, teacher)  # (neither an input's memory nor an output's)
+        ctx.shape = log_probs.shape
+        return out
 
     @staticmethod
     def backward(ctx, grad):
@@ -222,8 +224,8 @@ class _Expected(torch.autograd.Function):
         device = entries.device
         if grad.numel() == 0 or K == 0:
             return torch.zeros(shape, dtype=torch.float32, device=device), None
-        _, geo, _, _, runs, nbytes = _sizes(T, *shape[-2:], W, K, len(shape) == 2)
-        out = (torch.zeros if runs else torch.empty)(shape, dtype=torch.float32, device=device)
+        _, geo, _, _, runs, nbytes = _sizes(T, shape[-2], shape[-1], W, K, len(shape) == 2)
+        out = torch.empty(shape, dtype=torch.float32, device=device)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
         grad = grad.contiguous()
         _lib.launch("pcx_teacher_bwd", device, out.data_ptr(), None, scratch.data_ptr(), grad.data_ptr(), entries.data_ptr(), geo, 0,
@@ -255,10 +257,9 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
     if T * log_probs.size(-2) >= 2 ** 31:
         raise ValueError("more than 2^31 nodes over all positions")
     _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
-    entries = _prepare(teacher, B)
     if log_probs.requires_grad and torch.is_grad_enabled():
-        return _Expected.apply(log_probs, entries)
-    return _expect(log_probs.detach(), entries)
+        return _Expected.apply(log_probs, teacher)
+    return _expect(log_probs.detach(), teacher)[0]
 
 
 @functools.lru_cache(maxsize=None)
