@@ -129,11 +129,11 @@ __device__ __forceinline__ double log_norm(float m, double s, double inv_t) {
 }
 
 struct Shared {
-    alignas(16) u64 keys[kRoom + kMaxTop];     // the list (sorted, first), behind it the candidates of a tile
+    alignas(16) u64 keys[kRoom + kMaxTop]; // the list (sorted, first), behind it the candidates of a tile
     u64 list[kMaxTop];
     float red_m[kWarps];
     double red_s[kWarps];
-    uint32_t warp_t[kWarps];
+    uint32_t warp_t[kWarps], warp_u[kWarps];
     int count;
 };
 
@@ -147,14 +147,15 @@ __device__ __forceinline__ int block_sum(int mine, int* total) {       // every 
     return *total;
 }
 
-// The largest threshold t, by bisection, with least <= #(keys >= t) <= most, or (keys are unique, so only when `most` <
-// `least`) the smallest count above; `count(t)` gives a thread's share.
+// A threshold t with least <= #(keys >= t) <= most, by bisection between the smallest and the largest key; where equal keys
+// allow none, the largest t with at least `least`.  `at_least(i, t)`: whether key i < total is t or more.
 template <typename F>
-__device__ __forceinline__ u64 bisect(int least, int most, int* total, F count) {
-    u64 lo = 0, hi = ~0ull;
+__device__ __forceinline__ u64 bisect(int total, int least, int most, u64 lo, u64 hi, F at_least) {
+    const int tid = threadIdx.x;
     while (lo < hi) {
         const u64 mid = lo + ((hi - lo) >> 1) + ((hi - lo) & 1);
-        const int c = block_sum(count(mid), total);
+        int c = 0;
+        for (int i0 = 0; i0 < total; i0 += kThreads) c += __syncthreads_count(i0 + tid < total && at_least(i0 + tid, mid));
         if (c >= least) {
             lo = mid;
             if (c <= most) break;
@@ -162,29 +163,52 @@ __device__ __forceinline__ u64 bisect(int least, int most, int* total, F count) 
             hi = mid - 1;
         }
     }
-    __syncthreads();
     return lo;
+}
+
+// Smallest and largest of the high halves of keys[0, total), as bounds of all keys.
+__device__ __forceinline__ void key_range(const u64* keys, int total, uint32_t* low, uint32_t* high, u64& lo, u64& hi) {
+    uint32_t least = ~0u, most = 0;
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        const uint32_t v = (uint32_t)(keys[i] >> 32);
+        least = min(least, v);
+        most = max(most, v);
+    }
+    least = __reduce_min_sync(~0u, least);
+    most = __reduce_max_sync(~0u, most);
+    if ((threadIdx.x & 31) == 0) { low[threadIdx.x >> 5] = least; high[threadIdx.x >> 5] = most; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) { least = min(least, low[w]); most = max(most, high[w]); }
+    lo = (u64)least << 32;
+    hi = ((u64)most << 32) | 0xffffffffu;
+}
+
+// Cuts the `total` (more than kFew) unique keys in sh.keys back to n ... kFew / 2 of the largest, at its front.  Returns how
+// many are left.
+__device__ __noinline__ int trim(Shared& sh, int total, int n) {
+    const int tid = threadIdx.x;
+    u64 lo, hi;
+    key_range(sh.keys, total, sh.warp_t, sh.warp_u, lo, hi);
+    lo = bisect(total, n, kFew / 2, lo, hi, [&](int i, u64 mid) { return sh.keys[i] >= mid; });
+    // compaction, a block of keys after the other: those of a block are read before any is overwritten
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    for (int i0 = 0; i0 < total; i0 += kThreads) {
+        const u64 own = i0 + tid < total ? sh.keys[i0 + tid] : 0;
+        __syncthreads();
+        if (own >= lo && own != 0) sh.keys[atomicAdd(&sh.count, 1)] = own;
+    }
+    __syncthreads();
+    total = sh.count;
+    __syncthreads();
+    return total;
 }
 
 // Keeps the n largest of the `total` unique keys in sh.keys, sorted, at its front.  Returns how many there are.
 __device__ int prune(Shared& sh, int total, int n) {
     const int tid = threadIdx.x;
-    if (total > kFew) {
-        const u64 t = bisect(n, kFew, &sh.count, [&](u64 mid) {
-            int c = 0;
-            for (int i = tid; i < total; i += kThreads) c += sh.keys[i] >= mid;
-            return c;
-        });
-        // compaction, a block of keys after the other: those of a block are read before any is overwritten
-        if (tid == 0) sh.count = 0;
-        for (int i0 = 0; i0 < total; i0 += kThreads) {
-            const u64 own = i0 + tid < total ? sh.keys[i0 + tid] : 0;
-            __syncthreads();
-            if (own >= t && own != 0) sh.keys[atomicAdd(&sh.count, 1)] = own;
-        }
-        __syncthreads();
-        total = sh.count;
-    }
+    if (total > kFew) total = trim(sh, total, n);
     const int kept = min(total, n);
     for (int i = tid; i < total; i += kThreads) {
         const u64 k = sh.keys[i];
@@ -637,13 +661,22 @@ top_rows_block_kernel(RowArgs a) {
             };
             int total = collect(0);
             if (total > kRoom + kMaxTop) {
-                // too many (ordered or equal logits): the exact n-th largest, whatever it takes
-                const u64 from = bisect(a.n, kRoom, &sh.count, [&](u64 mid) {
+                // too many (ordered or equal logits): a key that n to kRoom of them reach
+                u64 lo = 0, hi = ~0ull;
+                while (lo < hi) {
+                    const u64 mid = lo + ((hi - lo) >> 1) + ((hi - lo) & 1);
                     int c = 0;
                     each(mid, [&](u64) { ++c; });
-                    return c;
-                });
-                total = collect(from);
+                    c = block_sum(c, &sh.count);
+                    if (c >= a.n) {
+                        lo = mid;
+                        if (c <= kRoom) break;
+                    } else {
+                        hi = mid - 1;
+                    }
+                }
+                __syncthreads();
+                total = collect(lo);
             }
             have = prune(sh, total, a.n);
             if (have == a.n) bound = value_of(sh.keys[a.n - 1]);
@@ -718,6 +751,7 @@ struct BeamShared {
     u64 list_s[kMaxTop];
     uint32_t list_p[kMaxTop];
     double base[kMaxTop];                           // what a beam's logits are raised by
+    uint32_t low[kWarps], high[kWarps];
     int count;
 };
 
@@ -758,11 +792,10 @@ join_beams_kernel(BeamArgs a) {
         __syncthreads();
         const int few = max(64, 2 * a.n);
         if (total > few) {
-            const u64 t = bisect(a.n, few, &sh.count, [&](u64 mid) {
-                int c = 0;
-                for (int i = tid; i < total; i += kThreads) c += sh.score[i] >= mid;
-                return c;
-            });
+            u64 t, most;
+            key_range(sh.score, total, sh.low, sh.high, t, most);
+            t = bisect(total, a.n, few, t, most, [&](int i, u64 mid) { return sh.score[i] >= mid; });
+            __syncthreads();
             if (tid == 0) sh.count = 0;
             for (int i0 = 0; i0 < total; i0 += kThreads) {
                 const u64 own = i0 + tid < total ? sh.score[i0 + tid] : 0;
@@ -781,6 +814,7 @@ join_beams_kernel(BeamArgs a) {
             const u64 s = sh.score[i];
             const uint32_t p = sh.place[i];
             int rank = 0;
+#pragma unroll 4
             for (int j = 0; j < total; ++j) {
                 const u64 o = sh.score[j];
                 rank += (int)(o > s) | ((int)(o == s) & (int)(sh.place[j] < p));
