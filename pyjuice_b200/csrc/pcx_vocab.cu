@@ -844,14 +844,14 @@ struct Moved {
     const char* src;
     char* dst;
     int64_t outer, chunks, src_outer, src_beam;     // rows before the beams, units per beam, strides in bytes
-    int64_t first_block, column_blocks, segments;   // blocks: columns, then segments of a beam's units, then outer rows
-    int lanes;                                      // threads side by side over a beam's units
+    uint32_t first_block, column_blocks, segments;  // blocks: columns, then segments of a beam's units, then outer rows
+    uint32_t lanes;                                 // threads side by side over a beam's units
 };
 struct MoveArgs {
     Moved t[kStates];
     const void* parents;
-    int n_tensors, wide_ids, beams, n;
-    int64_t columns;                                // batch * n
+    int n_tensors, wide_ids;
+    uint32_t beams, n, columns;                     // columns: batch * n
 };
 
 // dst[o, b * n + j, i] = src[o, b * beams + parents[b, j], i], in units of sizeof(U) bytes; zeros for a parent that is none
@@ -860,18 +860,19 @@ struct MoveArgs {
 template <typename U>
 __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
     int w = 0;
-    while (w + 1 < a.n_tensors && (int64_t)blockIdx.x >= a.t[w + 1].first_block) ++w;
+    while (w + 1 < a.n_tensors && blockIdx.x >= a.t[w + 1].first_block) ++w;
     const Moved& t = a.t[w];
-    int64_t block = (int64_t)blockIdx.x - t.first_block;
-    const int64_t c = block % t.column_blocks * (256 / t.lanes) + threadIdx.x / t.lanes;
+    uint32_t block = blockIdx.x - t.first_block;
+    const uint32_t c = block % t.column_blocks * (256 / t.lanes) + threadIdx.x / t.lanes;
     block /= t.column_blocks;
     if (c >= a.columns) return;
-    const int64_t i0 = block % t.segments * (t.lanes * kMoveUnits) + threadIdx.x % t.lanes;
-    const int64_t o0 = block / t.segments * kMoveRows;
+    const int64_t i0 = (int64_t)(block % t.segments) * (t.lanes * kMoveUnits) + threadIdx.x % t.lanes;
+    const int64_t o0 = (int64_t)(block / t.segments) * kMoveRows;
     const int64_t p = a.wide_ids ? ((const int64_t*)a.parents)[c] : (int64_t)((const int32_t*)a.parents)[c];
     const bool is = p >= 0 && p < a.beams;
-    const char* src = t.src + o0 * t.src_outer + (c / a.n * a.beams + (is ? p : 0)) * t.src_beam;
-    U* dst = (U*)t.dst + (o0 * a.columns + c) * t.chunks;
+    const char* src = t.src + o0 * t.src_outer + ((int64_t)(c / a.n) * a.beams + (is ? p : 0)) * t.src_beam;
+    const int64_t row = a.columns * t.chunks;
+    U* dst = (U*)t.dst + o0 * row + c * t.chunks;
     const int rows = (int)min((int64_t)kMoveRows, t.outer - o0);
     if (t.chunks <= t.lanes) {                      // a unit a row
         if (i0 >= t.chunks) return;
@@ -881,7 +882,7 @@ __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
             if (r < rows && is) u[r] = ((const U*)(src + r * t.src_outer))[i0];
 #pragma unroll
         for (int r = 0; r < kMoveRows; ++r)
-            if (r < rows) dst[r * a.columns * t.chunks + i0] = u[r];
+            if (r < rows) dst[r * row + i0] = u[r];
         return;
     }
     for (int r = 0; r < rows; ++r) {
@@ -891,7 +892,7 @@ __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
             if (i0 + k * t.lanes < t.chunks && is) u[k] = ((const U*)(src + r * t.src_outer))[i0 + k * t.lanes];
 #pragma unroll
         for (int k = 0; k < kMoveUnits; ++k)
-            if (i0 + k * t.lanes < t.chunks) dst[r * a.columns * t.chunks + i0 + k * t.lanes] = u[k];
+            if (i0 + k * t.lanes < t.chunks) dst[r * row + i0 + k * t.lanes] = u[k];
     }
 }
 
@@ -995,10 +996,10 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
 int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int wide_ids, int64_t batch, int beams, int n,
                 int unit, void* stream) {
     if (n_tensors <= 0 || batch <= 0 || n <= 0) return 0;
-    if (n_tensors > kStates || beams <= 0) return -1;
+    if (n_tensors > kStates || beams <= 0 || batch * n > 0x7fffffff) return -1;
     MoveArgs a{};
     a.parents = parents;
-    a.wide_ids = wide_ids; a.beams = beams; a.n = n; a.columns = batch * n;
+    a.wide_ids = wide_ids; a.beams = (uint32_t)beams; a.n = (uint32_t)n; a.columns = (uint32_t)(batch * n);
     int64_t blocks = 0;
     for (int i = 0; i < n_tensors; ++i) {
         const int64_t* s = states + 6 * i;
@@ -1007,9 +1008,12 @@ int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int w
         if (s[2] == 0 || chunks == 0) continue;
         int lanes = 1;
         while (lanes < 256 && lanes < chunks) lanes *= 2;
-        const int64_t column_blocks = pcx_cdiv(a.columns, 256 / lanes), segments = pcx_cdiv(chunks, (int64_t)lanes * kMoveUnits);
-        a.t[a.n_tensors++] = Moved{(const char*)s[0], (char*)s[1], s[2], chunks, s[4], s[5], blocks, column_blocks, segments, lanes};
-        blocks += column_blocks * segments * pcx_cdiv(s[2], kMoveRows);
+        const int64_t column_blocks = pcx_cdiv((int64_t)a.columns, 256 / lanes), segments = pcx_cdiv(chunks, (int64_t)lanes * kMoveUnits);
+        const int64_t more = column_blocks * segments * pcx_cdiv(s[2], kMoveRows);
+        if (segments > 0x7fffffff || more > 0x7fffffff - blocks) return -1;
+        a.t[a.n_tensors++] = Moved{(const char*)s[0], (char*)s[1], s[2], chunks, s[4], s[5], (uint32_t)blocks, (uint32_t)column_blocks,
+                                   (uint32_t)segments, (uint32_t)lanes};
+        blocks += more;
     }
     if (blocks == 0) return 0;
     if (blocks > 0x7fffffff) return -1;
