@@ -8,6 +8,9 @@
 // SM, so that the nodes of one category lie side by side wherever a table is read often (in shared memory for a table of
 // one position, in a transposed copy for a table that many positions share).  The backward pass sorts the slots by category
 // first; a category's sum then has one owner and one order, whatever the schedule, and every flow is written once.
+//
+// Times below: "large" is a table of 4096 nodes x 32768 categories that 128 positions x 64 samples of 32 slots share (250 K
+// slots with weight, 4.1 GB looked up in each direction); "small" is 196 tables of 256 x 256, 100 samples of 16 slots.
 #include "pcx_common.cuh"
 #include "../../include/pcx_b200.h"
 #include <cuda_bf16.h>
@@ -74,7 +77,7 @@ struct PrepArgs {
 };
 
 // L lanes per position, four slots a lane in registers (more are read again).  Slots that say something come first, in their
-// order: what reads them stops at the first empty one.
+// order: what reads them stops at the first empty one.  7 us large and small: latency (one warp a position took 13 small).
 template <int L>
 __global__ void __launch_bounds__(kTh) teacher_prep_kernel(PrepArgs a) {
     constexpr int HELD = 4;
@@ -143,7 +146,8 @@ struct FwdArgs {
 };
 
 // Few slots, or tables of a single node: the table is read where it lies.  Eight lanes share an output; the outputs of the
-// same nodes at all positions run side by side, since their reads meet in the same parts of the table.
+// same nodes at all positions run side by side, since their reads meet in the same parts of the table.  1024 nodes x 50257
+// categories, 128 positions of 50 slots: 28 us, 148 MB read at 5 TB/s: HBM, whose sectors of 32 bytes bring 4 wanted ones.
 __global__ void __launch_bounds__(kTh) teacher_fwd_direct_kernel(FwdArgs a) {
     const int64_t task = (int64_t)blockIdx.x * (kTh / 8) + (threadIdx.x >> 3);
     const int W = a.g.W, s = (int)(task / W % a.g.n_segs), b = (int)(task % W);
@@ -193,7 +197,9 @@ __device__ __forceinline__ void store_rows(const float* tile, float* out, int m_
 }
 
 // Turned table: a warp takes one position at a time, its lanes NV nodes each.  The same nodes of all positions run side by
-// side, so that their part of the table stays in L2.
+// side, so that their part of the table stays in L2 (all nodes of a position in a row: 379 us large).  Large: 226 us, at which
+// L2 delivers 15.6 TB/s to the SMs, which is what bounds it: 64 registers and 4 CTAs per SM beat more loads in flight (80
+// registers: 291 us).
 template <bool VEC, int NV>
 __global__ void __launch_bounds__(kTh, 4) teacher_fwd_turned_kernel(FwdArgs a) {
     constexpr int MT = 32 * NV;
@@ -266,7 +272,8 @@ __global__ void __launch_bounds__(kTh, 4) teacher_fwd_turned_kernel(FwdArgs a) {
     }
 }
 
-// A table of its own: NV * 32 nodes of it go through shared memory, the nodes of a category side by side.
+// A table of its own: NV * 32 nodes of it go through shared memory, the nodes of a category side by side.  Small: 45 us for 54
+// MB; 25 M instructions at 57% of the issue slots, seven for each slot and 64 nodes.  32 or 128 nodes a CTA: 60, 64 us.
 template <int NV, bool LOG>
 __global__ void __launch_bounds__(kTh) teacher_fwd_staged_kernel(FwdArgs a) {
     constexpr int MT = 32 * NV;
@@ -345,7 +352,8 @@ __global__ void __launch_bounds__(kTh) teacher_fwd_staged_kernel(FwdArgs a) {
 }
 
 // ---- turning -----------------------------------------------------------------------------------------------------------
-// 64 x 64 tiles; a thread reads and writes four neighbours at a time where rows allow it (VEC).
+// 64 x 64 tiles; a thread reads and writes four neighbours at a time where rows allow it (VEC).  Large: 167 us for the table (1.07
+// GB, 6.4 TB/s, as a copy; 32 x 32 tiles of single words: 370), 38 us for the flows.
 constexpr int kTurn = 64;
 
 // out[c][r] = value(r, c) for r < n_r, c < n_c of a tile, 0 for n_r <= r < pad_r.  `in` and `out` point at the tile.
@@ -420,7 +428,8 @@ __global__ void __launch_bounds__(kTh) teacher_turn_flows_kernel(float* __restri
 // Per set of variables: keys (category; C for empty slots) with the slot's place (position in the set * W + sample) and
 // weight, in the order of categories, the slots of a category in their own order.
 // Radix passes of at most 10 bits: the digit counts of the warps (and tiles), their running sums in the order of digits,
-// then every slot moves to its place; slots of one digit keep their order.
+// then every slot moves to its place; slots of one digit keep their order.  Large: 262 K slots in two passes, 38 us; small: 15 us
+// for 1600 slots a CTA (a bitonic network: 26).
 constexpr int kSmallSort = 4096, kSortRounds = 8, kSortTile = kTh * kSortRounds, kMaxCats = 1000000;
 
 struct SortArgs {
@@ -684,6 +693,9 @@ constexpr int kMaxTile = 64;       // categories of a tile
 // c_tile categories x NV * 32 nodes of one group.  The slots of the tile's categories, side by side after the sort,
 // are dealt out to the warps in equal parts; a warp walks its part in order, lanes over the nodes, and closes a category's
 // sum where the next begins.  A category that an earlier warp began is added to that warp's sum afterwards, in order.
+// Large: 410 us, of which writing the 537 MB alone takes 147; L2 delivers 10 TB/s.  What bounds it is latency: the sixteen
+// warps that 110 registers and 74 KB leave an SM wait for their four looked-up rows.  Tiles of 32 categories: 461 us; three
+// CTAs an SM: 450; a warp a category, long ones shared: 534.  Small: 40 us.
 template <int NV>
 __global__ void __launch_bounds__(kTh, 2) teacher_bwd_kernel(BwdArgs a) {
     constexpr int MT = 32 * NV, AHEAD = NV > 4 ? 4 : 8;
@@ -803,6 +815,7 @@ __global__ void __launch_bounds__(kTh, 2) teacher_bwd_kernel(BwdArgs a) {
     }
 }
 
+// (2048 rows of 64 slots: 8 us beside the 42 that clearing 268 MB takes.)
 // Few slots in large tables: only the categories that occur are visited, L lanes each, in an output that has been cleared
 // (mode 0).
 template <int L>

@@ -196,7 +196,8 @@ def _expect(log_probs, teacher):
     out = torch.empty(T, M, B, dtype=torch.float32, device=device)
     if T * M * B * K == 0:
         return out.zero_(), entries
-    _, geo, form, stride, _, _ = _sizes(T, M, C, B, K, log_probs.dim() == 2)
+    plan = _sizes(T, M, C, B, K, log_probs.dim() == 2)  # (holds what `geo` is the address of)
+    geo, form, stride = plan[1:4]
     table = log_probs.contiguous()
     turned = torch.empty(C, stride, dtype=torch.float32, device=device) if stride else None
     nb, nv = (0, 0) if norm is None else norm.stride()
@@ -224,12 +225,12 @@ class _Expected(torch.autograd.Function):
         device = entries.device
         if grad.numel() == 0 or K == 0:
             return torch.zeros(shape, dtype=torch.float32, device=device), None
-        _, geo, _, _, runs, nbytes = _sizes(T, shape[-2], shape[-1], W, K, len(shape) == 2)
+        plan = _sizes(T, shape[-2], shape[-1], W, K, len(shape) == 2)
         out = torch.empty(shape, dtype=torch.float32, device=device)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        scratch = torch.empty(plan[5], dtype=torch.uint8, device=device)
         grad = grad.contiguous()
-        _lib.launch("pcx_teacher_bwd", device, out.data_ptr(), None, scratch.data_ptr(), grad.data_ptr(), entries.data_ptr(), geo, 0,
-                    runs, 0, 0)
+        _lib.launch("pcx_teacher_bwd", device, out.data_ptr(), None, scratch.data_ptr(), grad.data_ptr(), entries.data_ptr(),
+                    plan[1], 0, plan[4], 0, 0)
         return out, None
 
 
