@@ -589,10 +589,10 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
                     int64_t stride_beam, int n, int pad_id, int normalize, int splits, void* stream);
 /* dst[o, b * n + j, :] = src[o, b * beams + parents[b][j], :] for up to 8 tensors at once; zeros for a parent outside
  * [0, beams).  `states` (HOST memory): per tensor source, destination, outer rows, bytes per beam, strides in bytes of outer
- * rows and of beams in the source; all of them multiples of `unit` (1, 2, 4, 8 or 16).  parents: int32, or int64 if
+ * rows and of beams in the source, and a unit (1, 2, 4, 8 or 16 bytes) that divides all of them.  parents: int32, or int64 if
  * wide_ids. */
 int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int wide_ids, int64_t batch, int beams, int n,
-                int unit, void* stream);
+                void* stream);
 
 /* ---- Language-model operators: leaf tables under a teacher's top logits ---------------------------------------------
  * entries[v][b][k] = (category or -1, weight) (8 bytes each; v < vars, b < width, k < slots), made by pcx_teacher_prep from ids

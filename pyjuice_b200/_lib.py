@@ -80,7 +80,7 @@ SIGNATURES = {
     "pcx_sum_par_dense2_gemm": [P, P, P, P, P, P, P, L, I, I, I],
     "pcx_top_logits": [P, P, P, P, P, I, L, I, L, I, I, D],
     "pcx_beam_select": [P, P, P, P, P, I, P, P, L, I, I, L, L, I, I, I, I],
-    "pcx_reorder": [P, I, P, I, L, I, I, I],
+    "pcx_reorder": [P, I, P, I, L, I, I],
     "pcx_teacher_prep": [P, P, I, L, L, L, P, I, L, L, L, P, L, L, I, I, I, I, D],
     "pcx_teacher_turn": [P, P, L, I, L, I],
     "pcx_teacher_fwd": [P, P, P, P, I, L, I],

@@ -851,7 +851,7 @@ struct Moved {
     char* dst;
     int64_t outer, chunks, src_outer, src_beam;     // rows before the beams, units per beam, strides in bytes
     uint32_t first_block, column_blocks, segments;  // blocks: columns, then segments of a beam's units, then outer rows
-    uint32_t lanes;                                 // threads side by side over a beam's units
+    uint32_t lanes, unit;                           // threads side by side over a beam's units; bytes of a unit
 };
 struct MoveArgs {
     Moved t[kStates];
@@ -865,11 +865,7 @@ struct MoveArgs {
 // has under way together; neighbours write neighbouring units.  4096 rows of 1024 beams, 4 bytes each: 12 us (2.8 TB/s read and
 // written; 25 us with a parent looked up per unit).
 template <typename U>
-__global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
-    int w = 0;
-    while (w + 1 < a.n_tensors && blockIdx.x >= a.t[w + 1].first_block) ++w;
-    const Moved& t = a.t[w];
-    uint32_t block = blockIdx.x - t.first_block;
+__device__ __forceinline__ void move(const MoveArgs& a, const Moved& t, uint32_t block) {
     const uint32_t c = block % t.column_blocks * (256 / t.lanes) + threadIdx.x / t.lanes;
     block /= t.column_blocks;
     if (c >= a.columns) return;
@@ -900,6 +896,20 @@ __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
 #pragma unroll
         for (int k = 0; k < kMoveUnits; ++k)
             if (i0 + k * t.lanes < t.chunks) dst[r * row + i0 + k * t.lanes] = u[k];
+    }
+}
+
+__global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
+    int w = 0;
+    while (w + 1 < a.n_tensors && blockIdx.x >= a.t[w + 1].first_block) ++w;
+    const Moved& t = a.t[w];
+    const uint32_t block = blockIdx.x - t.first_block;
+    switch (t.unit) {
+        case 16: move<uint4>(a, t, block); break;
+        case 8: move<uint2>(a, t, block); break;
+        case 4: move<uint32_t>(a, t, block); break;
+        case 2: move<uint16_t>(a, t, block); break;
+        default: move<uint8_t>(a, t, block);
     }
 }
 
@@ -999,9 +1009,9 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
 }
 
 // `states`: n_tensors times (source, destination, outer rows, bytes per beam, source strides in bytes of outer rows and
-// beams), host memory.
+// beams, unit), host memory.
 int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int wide_ids, int64_t batch, int beams, int n,
-                int unit, void* stream) {
+                void* stream) {
     if (n_tensors <= 0 || batch <= 0 || n <= 0) return 0;
     if (n_tensors > kStates || beams <= 0 || batch * n > 0x7fffffff) return -1;
     MoveArgs a{};
@@ -1009,8 +1019,9 @@ int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int w
     a.wide_ids = wide_ids; a.beams = (uint32_t)beams; a.n = (uint32_t)n; a.columns = (uint32_t)(batch * n);
     int64_t blocks = 0;
     for (int i = 0; i < n_tensors; ++i) {
-        const int64_t* s = states + 6 * i;
-        if (s[3] % unit != 0) return -1;
+        const int64_t* s = states + 7 * i;
+        const int64_t unit = s[6];
+        if ((unit != 1 && unit != 2 && unit != 4 && unit != 8 && unit != 16) || s[3] % unit != 0) return -1;
         const int64_t chunks = s[3] / unit;
         if (s[2] == 0 || chunks == 0) continue;
         int lanes = 1;
@@ -1019,20 +1030,12 @@ int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int w
         const int64_t more = column_blocks * segments * pcx_cdiv(s[2], kMoveRows);
         if (segments > 0x7fffffff || more > 0x7fffffff - blocks) return -1;
         a.t[a.n_tensors++] = Moved{(const char*)s[0], (char*)s[1], s[2], chunks, s[4], s[5], (uint32_t)blocks, (uint32_t)column_blocks,
-                                   (uint32_t)segments, (uint32_t)lanes};
+                                   (uint32_t)segments, (uint32_t)lanes, (uint32_t)unit};
         blocks += more;
     }
     if (blocks == 0) return 0;
     if (blocks > 0x7fffffff) return -1;
-    cudaStream_t st = (cudaStream_t)stream;
-    switch (unit) {
-        case 16: reorder_kernel<uint4><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-        case 8: reorder_kernel<uint2><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-        case 4: reorder_kernel<uint32_t><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-        case 2: reorder_kernel<uint16_t><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-        case 1: reorder_kernel<uint8_t><<<(unsigned)blocks, 256, 0, st>>>(a); break;
-        default: return -1;
-    }
+    reorder_kernel<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(a);
     PCX_LAUNCH_CHECK();
     return 0;
 }

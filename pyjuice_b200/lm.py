@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import List, NamedTuple, Optional, Tuple
 
 import numpy as np
@@ -361,8 +362,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[in
 def _beam_rows(x: torch.Tensor, dim: int):
     """(tensor, outer rows, bytes per beam, strides in bytes of outer rows and beams) of a state as the kernel walks it: a
     copy where the dimensions before or after the beams are not laid out as one."""
-    size, stride, es = x.shape, x.stride(), x.element_size()
-    inner = 1
+    size, es = x.shape, x.element_size()
+    if x.is_contiguous():
+        inner = math.prod(size[dim + 1:]) * es
+        return x, math.prod(size[:dim]), inner, inner * size[dim], inner
+    stride, inner = x.stride(), 1
     for d in range(x.dim() - 1, dim, -1):
         if size[d] != 1 and stride[d] != inner:
             return _beam_rows(x.contiguous(), dim)
@@ -403,18 +407,16 @@ def reorder(parents: torch.Tensor, *states: torch.Tensor, dim: int = 0) -> List[
         moved.append((x, at))
     _require_cuda(parents, *states)
     parents = parents.contiguous()
-    out, by_unit = [], {}
+    out, rows = [], []
     for x, at in moved:
         x, outer, nbytes, outer_step, beam_step = _beam_rows(x, at)
         y = torch.empty((*x.shape[:at], B * n, *x.shape[at + 1:]), dtype=x.dtype, device=x.device)
         out.append(y)
-        if y.numel() == 0:
-            continue
-        bits = x.data_ptr() | nbytes | outer_step | beam_step | 16
-        by_unit.setdefault(bits & -bits, []).append((x, (x.data_ptr(), y.data_ptr(), outer, nbytes, outer_step, beam_step)))
-    for unit, group in by_unit.items():
-        for i in range(0, len(group), 8):
-            part = [v for _, row in group[i:i + 8] for v in row]
-            _lib.launch("pcx_reorder", parents.device, (ctypes.c_int64 * len(part))(*part), len(part) // 6, parents.data_ptr(),
-                        int(parents.dtype == torch.int64), B, beams, n, unit)
+        if y.numel() > 0:
+            bits = x.data_ptr() | nbytes | outer_step | beam_step | 16
+            rows.append((x, (x.data_ptr(), y.data_ptr(), outer, nbytes, outer_step, beam_step, bits & -bits)))
+    for i in range(0, len(rows), 8):
+        part = [v for _, row in rows[i:i + 8] for v in row]
+        _lib.launch("pcx_reorder", parents.device, (ctypes.c_int64 * len(part))(*part), len(part) // 7, parents.data_ptr(),
+                    int(parents.dtype == torch.int64), B, beams, n)
     return out
