@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from typing import List, NamedTuple, Optional, Tuple
 
 import numpy as np
@@ -227,7 +228,7 @@ class _Expected(torch.autograd.Function):
         if grad.numel() == 0 or K == 0:
             return torch.zeros(shape, dtype=torch.float32, device=device), None
         plan = _sizes(T, shape[-2], shape[-1], W, K, len(shape) == 2)
-        out = torch.empty(shape, dtype=torch.float32, device=device)
+        out = torch.empty(*shape, dtype=torch.float32, device=device)
         scratch = torch.empty(plan[5], dtype=torch.uint8, device=device)
         grad = grad.contiguous()
         _lib.launch("pcx_teacher_bwd", device, out.data_ptr(), None, scratch.data_ptr(), grad.data_ptr(), entries.data_ptr(),
@@ -261,7 +262,7 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
     _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
     if log_probs.requires_grad and torch.is_grad_enabled():
         return _Expected.apply(log_probs, teacher)
-    return _expect(log_probs.detach(), teacher)[0]
+    return _expect(log_probs.detach() if log_probs.requires_grad else log_probs, teacher)[0]
 
 
 @functools.lru_cache(maxsize=None)
@@ -297,14 +298,14 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLog
     if not 0.0 < temperature < float("inf"):
         raise ValueError("`temperature` should be positive")
     _require_cuda(logits)
-    x = logits.detach()
+    x = logits
     if x.dim() != 2 or x.stride(1) != 1:
-        x = x.reshape(-1, V)
+        x = x.detach().reshape(-1, V)
         x = x if x.stride(1) == 1 or V == 1 else x.contiguous()
     rows, device = x.size(0), x.device
-    ids = torch.empty((*lead, k), dtype=torch.int64, device=device)
-    values = torch.empty((*lead, k), dtype=x.dtype, device=device)
-    norms = torch.empty(lead, dtype=torch.float32, device=device)
+    ids = torch.empty(*lead, k, dtype=torch.int64, device=device)       # (sizes one by one: a tuple of them costs a microsecond)
+    values = torch.empty(*lead, k, dtype=x.dtype, device=device)
+    norms = torch.empty(*(lead or ((),)), dtype=torch.float32, device=device)
     if rows > 0:
         scratch, splits = _scratch(rows, V * x.element_size(), k, device)
         _lib.launch("pcx_top_logits", device, ids.data_ptr(), values.data_ptr(), norms.data_ptr(), scratch.data_ptr(), x.data_ptr(),
@@ -343,9 +344,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_out: Optional[in
     if not 0 <= pad_id < V:
         raise ValueError("`pad_id` is not in the vocabulary")
     _require_cuda(logits, scores, finished)
-    x = logits.detach()
-    x = x if x.stride(2) == 1 or V == 1 else x.contiguous()
-    scores = scores.detach().contiguous()
+    x = logits if logits.stride(2) == 1 or V == 1 else logits.detach().contiguous()
+    scores = scores if scores.is_contiguous() else scores.detach().contiguous()
     finished = None if finished is None else finished.contiguous()
     device = x.device
     out = torch.empty(B, n, dtype=torch.float32, device=device)
@@ -388,35 +388,40 @@ def reorder(parents: torch.Tensor, *states: torch.Tensor, dim: int = 0) -> List[
 
     Returns the new states, contiguous, with B * n beams in that dimension.  A parent outside [0, K) gives zeros.  States
     may have any real type, other shapes than each other, and any strides; they are not differentiable."""
-    if parents.dim() != 2 or parents.dtype not in (torch.int32, torch.int64):
+    wide = parents.dtype == torch.int64
+    if parents.dim() != 2 or not (wide or parents.dtype == torch.int32):
         raise ValueError("`parents` must be int32 or int64 [B, n]")
     B, n = parents.shape
     moved, beams = [], None
     for x in states:
-        if x.dim() < 1 or not -x.dim() <= dim < x.dim():
-            raise ValueError(f"a state of shape {tuple(x.shape)} has no dimension {dim}")
-        at = dim % x.dim()
+        size = x.shape
+        if not -len(size) <= dim < len(size):
+            raise ValueError(f"a state of shape {tuple(size)} has no dimension {dim}")
+        at = dim % len(size)
         if x.is_complex():
             raise TypeError("states must be real")
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError("`reorder` is not differentiable: call it under torch.no_grad()")
-        if B > 0 and (x.size(at) % B != 0 or x.size(at) == 0 or (beams is not None and x.size(at) != B * beams)):
-            raise ValueError(f"a state with {x.size(at)} beams does not fit {B} sequences" +
+        width = size[at]
+        if B > 0 and (width == 0 or width % B != 0 or (beams is not None and width != B * beams)):
+            raise ValueError(f"a state with {width} beams does not fit {B} sequences" +
                              (f" of {beams}" if beams is not None else ""))
-        beams = x.size(at) // B if B > 0 else 1
-        moved.append((x, at))
+        beams = width // B if B > 0 else 1
+        moved.append((x, at, size))
     _require_cuda(parents, *states)
-    parents = parents.contiguous()
-    out, rows = [], []
-    for x, at in moved:
+    parents, device = parents.contiguous(), parents.device
+    out, held, rows = [], [], []
+    for x, at, size in moved:
         x, outer, nbytes, outer_step, beam_step = _beam_rows(x, at)
-        y = torch.empty((*x.shape[:at], B * n, *x.shape[at + 1:]), dtype=x.dtype, device=x.device)
+        y = torch.empty(*size[:at], B * n, *size[at + 1:], dtype=x.dtype, device=device)
         out.append(y)
-        if y.numel() > 0:
-            bits = x.data_ptr() | nbytes | outer_step | beam_step | 16
-            rows.append((x, (x.data_ptr(), y.data_ptr(), outer, nbytes, outer_step, beam_step, bits & -bits)))
-    for i in range(0, len(rows), 8):
-        part = [v for _, row in rows[i:i + 8] for v in row]
-        _lib.launch("pcx_reorder", parents.device, (ctypes.c_int64 * len(part))(*part), len(part) // 7, parents.data_ptr(),
-                    int(parents.dtype == torch.int64), B, beams, n)
+        if outer * nbytes * B * n > 0:
+            source = x.data_ptr()
+            bits = source | nbytes | outer_step | beam_step | 16
+            held.append(x)                              # (a copy has to live until the launch)
+            rows += (source, y.data_ptr(), outer, nbytes, outer_step, beam_step, bits & -bits)
+    for i in range(0, len(rows), 56):
+        part = rows[i:i + 56]
+        _lib.launch("pcx_reorder", device, struct.pack(f"{len(part)}q", *part), len(part) // 7, parents.data_ptr(), int(wide), B,
+                    beams, n)
     return out
