@@ -428,9 +428,9 @@ __global__ void __launch_bounds__(kTh) teacher_turn_flows_kernel(float* __restri
 // Per set of variables: keys (category; C for empty slots) with the slot's place (position in the set * W + sample) and
 // weight, in the order of categories, the slots of a category in their own order.
 // Radix passes of at most 10 bits: the digit counts of the warps (and tiles), their running sums in the order of digits,
-// then every slot moves to its place; slots of one digit keep their order.  Large: 262 K slots in two passes, 38 us; small: 15 us
+// then every slot moves to its place; slots of one digit keep their order.  Large: 262 K slots in two passes, 37 us (eight rounds a tile: 42); small: 15 us
 // for 1600 slots a CTA (a bitonic network: 26).
-constexpr int kSmallSort = 4096, kSortRounds = 8, kSortTile = kTh * kSortRounds, kMaxCats = 1000000;
+constexpr int kSmallSort = 4096, kSortRounds = 4, kSortTile = kTh * kSortRounds, kMaxCats = 1000000;
 
 struct SortArgs {
     Geo g;
@@ -647,6 +647,7 @@ __global__ void __launch_bounds__(kTh) teacher_move_kernel(SortArgs a) {
         const int total = d < D ? a.totals[(int64_t)u * D + d] : 0;
         const int before = run + scan_before(total, warp_sum);
         if (d < D) {
+            if (tile == 0 && a.first != nullptr && d <= a.C) a.first[(int64_t)u * (a.C + 1) + d] = before;
             int at = before + a.hist[((int64_t)u * D + d) * a.tiles + tile];
             for (int w = 0; w < kW; ++w) { const int c = sm_move[w * D + d]; sm_move[w * D + d] = at; at += c; }
         }
@@ -693,9 +694,11 @@ constexpr int kMaxTile = 64;       // categories of a tile
 // c_tile categories x NV * 32 nodes of one group.  The slots of the tile's categories, side by side after the sort,
 // are dealt out to the warps in equal parts; a warp walks its part in order, lanes over the nodes, and closes a category's
 // sum where the next begins.  A category that an earlier warp began is added to that warp's sum afterwards, in order.
-// Large: 410 us, of which writing the 537 MB alone takes 147; L2 delivers 10 TB/s.  What bounds it is latency: the sixteen
-// warps that 110 registers and 74 KB leave an SM wait for their four looked-up rows.  Tiles of 32 categories: 461 us; three
-// CTAs an SM: 450; a warp a category, long ones shared: 534.  Small: 40 us.
+// Large: 405 us, of which writing the 537 MB alone takes 147; L2 delivers 10 TB/s, and its 4.1 GB would take 277 at the 15.5 that
+// the forward pass reaches.  Neither more rows under way nor balance is what it lacks: rows kept under way without a pause, in
+// registers 419, through a ring in shared memory (cp.async) 640; full tiles first 408; flows laid out tile by tile 410.  Tiles
+// of 32 categories: 461; three CTAs an SM: 450; a warp a category, long ones shared: 534.  Small: 39 us.  512 nodes, 1000 categories: 35
+// us (512 threads a CTA 31, more launched forms for 3% of a call; tiles of 64 or 32 nodes 42, 63).
 template <int NV>
 __global__ void __launch_bounds__(kTh, 2) teacher_bwd_kernel(BwdArgs a) {
     constexpr int MT = 32 * NV, AHEAD = NV > 4 ? 4 : 8;
@@ -1049,6 +1052,7 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     } else {
         s.hist = (int32_t*)(base + l.hist); s.totals = (int32_t*)(base + l.totals);
         s.tiles = l.tiles;
+        if (l.passes > 1) s.first = nullptr;            // (one pass: the categories are the digits)
         const int64_t digits = (int64_t)geo->n_sets << l.bits;
         if ((int64_t)l.tiles * geo->n_sets > 0x7fffffff || pcx_cdiv(digits, kW) > 0x7fffffff) return -1;
         const unsigned grid = (unsigned)(l.tiles * geo->n_sets);
@@ -1087,7 +1091,7 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
         PCX_LAUNCH_CHECK();
         return 0;
     }
-    if (!l.small) {
+    if (!l.small && l.passes > 1) {
         const int64_t blocks = pcx_cdiv(l.n_max + 1, kTh);
         if (blocks * geo->n_sets > 0x7fffffff) return -1;
         teacher_first_kernel<<<(unsigned)(blocks * geo->n_sets), kTh, 0, st>>>((int32_t*)(base + l.first), s.keys, g, geo->cats, (int)blocks);

@@ -101,7 +101,8 @@ def make(T, M, C, B, K, tied, seed=0, ids=torch.int64, dtype=torch.float32, temp
 # the backward pass: by categories that occur, by tiles of categories)
 SIZES = [(1, 1, 1, 1, 1), (1, 1, 2, 1, 3), (3, 5, 7, 2, 4), (2, 128, 256, 33, 16), (5, 33, 100, 31, 9), (4, 130, 64, 40, 8), (7, 64, 31, 1, 1),
          (2, 16, 1600, 70, 12), (3, 9, 20000, 5, 10), (40, 1, 500, 3, 12), (2, 257, 1000, 65, 40), (1, 3, 200000, 2, 7), (2, 6, 70001, 90, 33),
-         (2, 3, 400, 3, 300), (3, 2, 50, 2, 60), (8, 40, 600, 200, 4), (9, 300, 601, 200, 4), (8, 5, 70, 300, 3), (3, 70, 40, 500, 5)]
+         (2, 3, 400, 3, 300), (3, 2, 50, 2, 60), (8, 40, 600, 200, 4), (9, 300, 601, 200, 4), (8, 5, 70, 300, 3), (3, 70, 40, 500, 5),
+         (3, 8, 1023, 160, 10), (3, 8, 1024, 160, 10)]      # the most categories of a sort in one pass, the fewest in two
 
 
 @pytest.mark.gpu
