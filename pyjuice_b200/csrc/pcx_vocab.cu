@@ -54,6 +54,23 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+// The terms of a sum are 2^(x * scale - r) with r = m * scale rounded once: one fused operation each, and all of them relative to
+// the same r.  That is off by up to half a step of r, at most 64 below kNear: far from the range's ends, and put right when the
+// sum is read.  Larger r (logits of -1e30, the lowest number of a type) leave nothing of a difference: their terms are 2^((x - m) *
+// scale), more slowly.
+constexpr float kNear = 2147483648.0f;
+__device__ __forceinline__ bool near(float r) { return fabsf(r) < kNear; }
+// What the sum relative to (m, r) is multiplied by to be relative to (top, nr).
+__device__ __forceinline__ float to_other(float m, float r, float top, float nr, float scale) {
+    if (m == top) return 1.0f;
+    if (near(r) && near(nr)) return exp2_fast(r - nr);
+    return exp2_fast((m - top) * scale + (near(r) ? fmaf(-m, scale, r) : 0.0f) - (near(nr) ? fmaf(-top, scale, nr) : 0.0f));
+}
+// The sum relative to m itself.
+__device__ __forceinline__ double to_own(float s, float m, float r, float scale) {
+    return near(r) ? (double)s * exp2((double)fmaf(-m, scale, r)) : (double)s;
+}
+
 // 16 bytes of logits: their maximum (NaN skipped) and the logits one by one.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
@@ -315,20 +332,21 @@ __device__ __forceinline__ int warp_before(int& n) {
     return before;
 }
 
-// What a lane's part of a tile adds to its sum when the quick way gave no number: NaN, infinities, or a maximum near the
-// largest number.
+// What a lane's part of a tile adds to its sum when the quick way gave no number: NaN, infinities, or a maximum that is not `near`.
 template <typename T>
 __device__ __noinline__ float careful_sum(const T* x, int first, int groups, int step, int end, float m, float r, float scale) {
     constexpr int VE = Pack<T>::N;
-    float s = 0.0f;
+    float s[2] = {};
 #pragma unroll 1
-    for (int i = 0; i < groups * VE; ++i) {
-        const int e = first + i / VE * step + i % VE;
-        if (e < 0 || e >= end) continue;
-        const float f = fmaxf((float)x[e], PCX_NEG_INF);
-        s += exp2_fast(f == m ? 0.0f : fabsf(r) < CUDART_INF_F ? fmaf(f, scale, -r) : (f - m) * scale);
-    }
-    return s;
+    for (int i = 0; i < groups * VE; i += 2)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = first + i / VE * step + i % VE + h;
+            if (e < 0 || e >= end) continue;
+            const float f = fmaxf((float)x[e], PCX_NEG_INF);
+            s[h] += exp2_fast(near(r) ? fmaf(f, scale, -r) : f == m ? 0.0f : (f - m) * scale);
+        }
+    return s[0] + s[1];
 }
 
 // Many rows, or short ones: a warp a row, sixteen rows under way per SM (128 registers: a tile is on its way while the one
@@ -351,8 +369,6 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
     uint16_t* hot = all_hot[warp];
     int count = 0;
     u64 bound = 0;                                  // n keys of the set are at least this large; 0 before there are n
-    // The terms of a sum are 2^(x * scale - r) with r = m * scale rounded once: one fused operation each, and all of them
-    // relative to the same r.  What r is off is put right when the sum is read.
     float m = PCX_NEG_INF, r = PCX_NEG_INF, s = 0.0f;
     bool skip = a.finished != nullptr && a.finished[row] != 0;
     if (a.scores != nullptr) skip |= !(a.scores[row] > PCX_NEG_INF);
@@ -389,8 +405,7 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
                 }
                 if (top > m) {
                     const float nr = top * a.scale;
-                    const bool plain = fabsf(r) < CUDART_INF_F && fabsf(nr) < CUDART_INF_F;
-                    s = m > PCX_NEG_INF ? s * exp2_fast(plain ? r - nr : (m - top) * a.scale) : 0.0f;
+                    s = m > PCX_NEG_INF ? s * to_other(m, r, top, nr, a.scale) : 0.0f;
                     m = top;
                     r = nr;
                 }
@@ -404,7 +419,7 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
                             s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
                         }
                     s0 += s1;
-                    if (!(s0 < CUDART_INF_F) || !(fabsf(r) < CUDART_INF_F))
+                    if (!(s0 < CUDART_INF_F) || !near(r))
                         s0 = careful_sum<T>(x, (chunk + t * 32 * G + lane) * VE - off, G, 32 * VE, a.vocab, m, r, a.scale);
                     s += s0;
                 }
@@ -506,17 +521,15 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
             __syncwarp();
         }
     }
-    // statistics in fp32, then what the largest lane's r was off
+    // statistics in fp32
     float M = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
     const float R = M * a.scale;
-    const bool plain = fabsf(R) < CUDART_INF_F;
-    s = m > PCX_NEG_INF ? s * exp2_fast(plain && fabsf(r) < CUDART_INF_F ? r - R : (m - M) * a.scale) : 0.0f;
+    s = m > PCX_NEG_INF ? s * to_other(m, r, M, R, a.scale) : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    const double S = M > PCX_NEG_INF && M < CUDART_INF_F
-        ? plain ? (double)s * (1.0 + (double)fmaf(-M, a.scale, R) * 0.6931471805599453) : (double)s : 0.0;
+    const double S = M > PCX_NEG_INF && M < CUDART_INF_F ? to_own(s, M, R, a.scale) : 0.0;
     // the set in order: a key's place is the number of larger ones
     if (count > a.n + a.n / 2 + 16) count = cut(keys, count, a.n, &bound);
     __syncwarp();
@@ -563,8 +576,6 @@ top_rows_block_kernel(RowArgs a) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x / a.splits;
     const int part = blockIdx.x % a.splits;
-    // The terms of a sum are 2^(x * scale - r) with r = m * scale rounded once: one fused operation each, and all of them
-    // relative to the same r.  What r is off is put right when the sum is read.
     float m = PCX_NEG_INF, r = PCX_NEG_INF, s = 0.0f;
     int have = 0;
     bool skip = a.finished != nullptr && a.finished[row] != 0;
@@ -590,8 +601,7 @@ top_rows_block_kernel(RowArgs a) {
             }
             if (top > m) {
                 const float nr = top * a.scale;
-                const bool plain = fabsf(r) < CUDART_INF_F && fabsf(nr) < CUDART_INF_F;
-                s = m > PCX_NEG_INF ? s * exp2_fast(plain ? r - nr : (m - top) * a.scale) : 0.0f;
+                s = m > PCX_NEG_INF ? s * to_other(m, r, top, nr, a.scale) : 0.0f;
                 m = top;
                 r = nr;
             }
@@ -605,7 +615,7 @@ top_rows_block_kernel(RowArgs a) {
                         s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
                     }
                 s0 += s1;
-                if (!(s0 < CUDART_INF_F) || !(fabsf(r) < CUDART_INF_F))
+                if (!(s0 < CUDART_INF_F) || !near(r))
                     s0 = careful_sum<T>(x, (g + tid) * VE - off, G, kThreads * VE, min(a.vocab, g1 * VE - off), m, r, a.scale);
                 s += s0;
             }
@@ -692,14 +702,13 @@ top_rows_block_kernel(RowArgs a) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(~0u, wm, o));
     const float wr = wm * a.scale;
-    const bool plain = fabsf(wr) < CUDART_INF_F;
-    s = m > PCX_NEG_INF ? s * exp2_fast(plain && fabsf(r) < CUDART_INF_F ? r - wr : (m - wm) * a.scale) : 0.0f;
+    s = m > PCX_NEG_INF ? s * to_other(m, r, wm, wr, a.scale) : 0.0f;
 #pragma unroll
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     // ... and those of the warps in 64 bits
     float M;
     double S;
-    block_stats(sh, wm, plain ? (double)s * (1.0 + (double)fmaf(-wm, a.scale, wr) * 0.6931471805599453) : (double)s, a.inv_t, M, S);
+    block_stats(sh, wm, to_own(s, wm, wr, a.scale), a.inv_t, M, S);
     leave<T>(a, sh, row, have, M, S);
 }
 

@@ -1,0 +1,85 @@
+"""Operators of language-model circuits at the edges: rows of large logits, continuations whose scores are equal or nearly so, tokens
+and slots that say something unusual, every form of the selection at every cut of a row."""
+import math
+
+import pytest
+import torch
+
+from pyjuice_b200 import lm
+
+NEG_INF, NAN, INF = float("-inf"), float("nan"), float("inf")
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+STEP = 2.0 ** -24                    # half a step of fp32, relative
+
+
+def norm_tol(vocab):
+    """How far a log-normaliser may be off before it is rounded to fp32, in steps of 2^-24 of the sum: an exponential of 2^-22 (4); its
+    argument, rounded twice, whose distance from the maximum is at most log2(vocab) + 2 bits on average under the weights (2 ln 2
+    each); up to 34 sums in a tile; per tile of a lane (128 logits of a part or more) a sum, and a product with an
+    exponential where the maximum rises (6); and as many joins of lanes (5 + 5, arguments of 2 log2(vocab) bits)."""
+    bits = math.log2(vocab) + 2
+    return (4 + 2 * 0.7 * bits + 34 + 6 * (vocab // 1024 + 1) + 10 + 2 * 0.7 * bits) * STEP
+
+
+def exact_norm(row):
+    """log sum exp of a list, the sum rounded once (NaN counts nothing)."""
+    row = [v for v in row if v > NEG_INF]
+    if not row:
+        return NEG_INF
+    m = max(row)
+    return INF if m == INF else m + math.log(math.fsum(math.exp(v - m) for v in row))
+
+
+def best(x, scores, n, finished=None, pad=0):
+    """The n best continuations of one sequence, ``x`` [K, V], by the definition in 64 bits: [(score, parent, token)]."""
+    found = []
+    for k, (row, s) in enumerate(zip(x.double().tolist(), scores.double().tolist())):
+        if not s > NEG_INF:
+            continue
+        if finished is not None and bool(finished[k]):
+            found.append((-s, k, pad))
+            continue
+        norm = exact_norm(row)
+        found += sorted((-((s + v) - norm), k, t) for t, v in enumerate(row) if v > NEG_INF and norm < INF)[:n]
+    found = sorted(found)[:n]
+    return [(-s, k, t) for s, k, t in found] + [(NEG_INF, 0, -1)] * (n - len(found))
+
+
+def check_best(x, scores, n, finished=None, pad=0):
+    got = [t.cpu() for t in lm.beam_select(x, scores, n, finished, pad)]
+    for b in range(x.size(0)):
+        want = best(x[b], scores[b], n, None if finished is None else finished[b], pad)
+        assert got[1][b].tolist() == [w[1] for w in want] and got[2][b].tolist() == [w[2] for w in want]
+        for s, w in zip(got[0][b].tolist(), want):
+            assert s == w[0] or abs(s - w[0]) <= norm_tol(x.size(2)) + abs(w[0]) * STEP
+
+
+LARGE = [-1e9, 1e9, 1e5, -1e6, 3e7, -1e12, -1e30, 2e38, torch.finfo(torch.float32).min]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("value", LARGE)
+def test_rows_of_large_logits_have_their_normaliser(value, dtype):
+    """A row that a mask's number fills altogether, or in part, scores as any other row: what counts is how far logits are apart."""
+    value = max(min(value, torch.finfo(dtype).max), torch.finfo(dtype).min)
+    for B, K, V in ((1, 4, 5003), (700, 4, 257), (2, 4, 60)):
+        x = torch.randn(1, K, V, generator=torch.Generator().manual_seed(V))
+        x[:, 0] = value
+        x[:, 1] += value
+        x[:, 2, ::7] = value
+        x = x.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype)
+        scores = torch.tensor([[-3.0, -5.0, -4.0, -6.0]])
+        got = [t.cpu() for t in lm.beam_select(x.expand(B, K, V).contiguous().cuda(), scores.expand(B, K).cuda(), 9)]
+        want = best(x[0], scores[0], 9)
+        for b in (0, B - 1):
+            assert got[1][b].tolist() == [w[1] for w in want] and got[2][b].tolist() == [w[2] for w in want]
+            for s, w in zip(got[0][b].tolist(), want):
+                assert abs(s - w[0]) <= norm_tol(V) + abs(w[0]) * STEP
+        for temperature in (0.5, 1.0, 2.0, 30.0):
+            norm = lm.top_logits(x[0].cuda(), 1, temperature).log_norm.double().cpu().tolist()
+            for row, n in zip(x[0].double().tolist(), norm):
+                want = exact_norm([v / temperature for v in row])
+                # (a normaliser beyond the range of fp32 is infinite)
+                if abs(want) < torch.finfo(torch.float32).max:
+                    assert abs(n - want) <= norm_tol(V) + abs(want) * STEP, (temperature, n, want)
