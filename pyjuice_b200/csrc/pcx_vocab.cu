@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <cmath>
 
 namespace {
 
@@ -758,94 +759,177 @@ struct BeamArgs {
     const Part* parts;             // [batch * beams]
     const float* scores;
     const uint8_t* finished;
+    const void* logits;
+    int64_t stride_batch, stride_beam;
     float* out_scores;
     int64_t *tokens, *parents;
-    int beams, n, vocab, pad_id, normalize;
+    int beams, n, vocab, pad_id, normalize, dtype;
+    double slack;                  // scores of different beams that are no further apart than this may be in the wrong order
 };
 
 constexpr int kBeamTile = 2048;                     // candidates looked at together
 struct BeamShared {
     u64 score[kBeamTile + kMaxTop];
     uint32_t place[kBeamTile + kMaxTop];            // beam * vocab + token: a lower one first among equal scores
-    u64 list_s[kMaxTop];
-    uint32_t list_p[kMaxTop];
-    double base[kMaxTop];                           // what a beam's logits are raised by
+    u64 list_s[kMaxTop + 1];
+    uint32_t list_p[kMaxTop + 1];
+    double norm[kMaxTop], red[kWarps];              // what a beam's logits are lowered by
+    float own[kMaxTop];                             // its score
+    uint8_t exact[kMaxTop], doubt[kMaxTop];
     uint32_t low[kWarps], high[kWarps];
     int count;
 };
 
+// log sum exp of a row in 64 bits, from its maximum.  The order of the sum goes by the places alone: equal rows, wherever they
+// lie, have equal bits.
+template <typename T>
+__device__ __noinline__ double exact_norm(const T* x, int vocab, float m, double* red) {
+    constexpr int AHEAD = 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    double s = 0.0;
+    for (int64_t e0 = threadIdx.x; e0 < vocab; e0 += kThreads * AHEAD) {
+        float f[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) f[i] = e0 + i * kThreads < vocab ? (float)x[e0 + i * kThreads] : PCX_NEG_INF;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+            if (f[i] > PCX_NEG_INF) s += exp((double)f[i] - (double)m);      // (not NaN)
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    __syncthreads();
+    if (lane == 0) red[warp] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) s += red[w];
+    return log_norm(m, s, 1.0);
+}
+
 // One CTA per sequence; 64 sequences of 16 lists of 32: 8 us, in which 512 candidates are bisected down to at most 64 before
 // they are ranked (ranking them all: 65 us).
+// The normalisers of the rows carry the error of their fp32 terms.  Where that leaves two continuations of different beams in
+// doubt, among the n best or at their end, those beams' normalisers are taken again in 64 bits and the choice is made again.  Once is
+// enough: a score moves by half the slack at most, so that only pairs within the slack can change places.
 __global__ void __launch_bounds__(kThreads)
 join_beams_kernel(BeamArgs a) {
     __shared__ BeamShared sh;
     const int tid = threadIdx.x;
     const int64_t first = (int64_t)blockIdx.x * a.beams;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
     after_previous();
     for (int b = tid; b < a.beams; b += kThreads) {
         const Part p = a.parts[first + b];
-        const float sc = a.scores[first + b];
-        sh.base[b] = (double)sc - (a.normalize ? log_norm(p.m, p.s, 1.0) : 0.0);
-        if (a.finished != nullptr && a.finished[first + b] != 0 && sc > PCX_NEG_INF) {
-            const int at = atomicAdd(&sh.count, 1); // a finished beam has one continuation, at its own score
-            sh.score[at] = ordered((double)sc);
-            sh.place[at] = (uint32_t)b * a.vocab + a.pad_id;
-        }
+        const bool done = a.finished != nullptr && a.finished[first + b] != 0;
+        sh.own[b] = a.scores[first + b];
+        sh.norm[b] = a.normalize && !done ? log_norm(p.m, p.s, 1.0) : 0.0;
+        sh.exact[b] = done || !a.normalize;
+        sh.doubt[b] = 0;
     }
     __syncthreads();
     const int slots = a.beams * a.n;
-    int have = 0;
-    for (int at = 0; at < slots; at += kBeamTile - kMaxTop) {
-        for (int i = tid; i < kBeamTile - kMaxTop && at + i < slots; i += kThreads) {
-            const int b = (at + i) / a.n, entry = (at + i) % a.n;
-            if (entry >= a.parts[first + b].count) continue;
-            const u64 k = a.keys[first * a.n + at + i];
-            const double score = sh.base[b] + (double)value_of(k);
-            if (!(score > -CUDART_INF)) continue;   // NaN: a row without a normaliser
-            const int to = atomicAdd(&sh.count, 1);
-            sh.score[to] = ordered(score);
-            sh.place[to] = (uint32_t)b * a.vocab + place_of(k);
-        }
+    // The score of an entry of the lists, its place; not above -inf if there is none (NaN: a row without a normaliser)
+    auto candidate = [&](int i, uint32_t& place) {
+        const int b = i / a.n;
+        if (i % a.n >= a.parts[first + b].count) return -CUDART_INF;
+        const u64 k = a.keys[first * a.n + i];
+        place = (uint32_t)b * a.vocab + place_of(k);
+        return ((double)sh.own[b] + (double)value_of(k)) - sh.norm[b];
+    };
+    auto is_finished = [&](int b) { return a.finished != nullptr && a.finished[first + b] != 0 && sh.own[b] > PCX_NEG_INF; };
+    int have = 0;                                   // (one entry more than asked for: the best that is left out)
+    for (bool again = false;; again = true) {
+        if (tid == 0) sh.count = 0;
         __syncthreads();
-        int total = sh.count;
+        for (int b = tid; b < a.beams; b += kThreads)
+            if (is_finished(b)) {                   // a finished beam has one continuation, at its own score
+                const int at = atomicAdd(&sh.count, 1);
+                sh.score[at] = ordered((double)sh.own[b]);
+                sh.place[at] = (uint32_t)b * a.vocab + a.pad_id;
+            }
         __syncthreads();
-        const int few = max(64, 2 * a.n);
-        if (total > few) {
-            u64 t, most;
-            key_range(sh.score, total, sh.low, sh.high, t, most);
-            t = bisect(total, a.n, few, t, most, [&](int i, u64 mid) { return sh.score[i] >= mid; });
+        for (int at = 0; at < slots; at += kBeamTile - kMaxTop) {
+            for (int i = tid; i < kBeamTile - kMaxTop && at + i < slots; i += kThreads) {
+                uint32_t place;
+                const double score = candidate(at + i, place);
+                if (!(score > -CUDART_INF)) continue;
+                const int to = atomicAdd(&sh.count, 1);
+                sh.score[to] = ordered(score);
+                sh.place[to] = place;
+            }
             __syncthreads();
-            if (tid == 0) sh.count = 0;
-            for (int i0 = 0; i0 < total; i0 += kThreads) {
-                const u64 own = i0 + tid < total ? sh.score[i0 + tid] : 0;
-                const uint32_t place = i0 + tid < total ? sh.place[i0 + tid] : 0;
+            int total = sh.count;
+            __syncthreads();
+            const int few = max(64, 2 * a.n);
+            if (total > few) {
+                u64 t, most;
+                key_range(sh.score, total, sh.low, sh.high, t, most);
+                t = bisect(total, a.n + 1, few, t, most, [&](int i, u64 mid) { return sh.score[i] >= mid; });
                 __syncthreads();
-                if (own >= t && own != 0) {
-                    const int to = atomicAdd(&sh.count, 1);
-                    sh.score[to] = own;
-                    sh.place[to] = place;
+                if (tid == 0) sh.count = 0;
+                for (int i0 = 0; i0 < total; i0 += kThreads) {
+                    const u64 own = i0 + tid < total ? sh.score[i0 + tid] : 0;
+                    const uint32_t place = i0 + tid < total ? sh.place[i0 + tid] : 0;
+                    __syncthreads();
+                    if (own >= t && own != 0) {
+                        const int to = atomicAdd(&sh.count, 1);
+                        sh.score[to] = own;
+                        sh.place[to] = place;
+                    }
                 }
+                __syncthreads();
+                total = sh.count;
+            }
+            for (int i = tid; i < total; i += kThreads) {
+                const u64 s = sh.score[i];
+                const uint32_t p = sh.place[i];
+                int rank = 0;
+#pragma unroll 4
+                for (int j = 0; j < total; ++j) {
+                    const u64 o = sh.score[j];
+                    rank += (int)(o > s) | ((int)(o == s) & (int)(sh.place[j] < p));
+                }
+                if (rank <= a.n) { sh.list_s[rank] = s; sh.list_p[rank] = p; }
             }
             __syncthreads();
-            total = sh.count;
+            have = min(total, a.n + 1);
+            for (int i = tid; i < have; i += kThreads) { sh.score[i] = sh.list_s[i]; sh.place[i] = sh.list_p[i]; }
+            if (tid == 0) sh.count = have;
+            __syncthreads();
         }
-        for (int i = tid; i < total; i += kThreads) {
-            const u64 s = sh.score[i];
-            const uint32_t p = sh.place[i];
-            int rank = 0;
-#pragma unroll 4
-            for (int j = 0; j < total; ++j) {
-                const u64 o = sh.score[j];
-                rank += (int)(o > s) | ((int)(o == s) & (int)(sh.place[j] < p));
+        if (again || a.beams == 1 || !a.normalize) break;
+        // neighbours of different beams, or at the end of the n best, within the slack
+        bool close = false;
+        for (int i = tid; i + 1 < have; i += kThreads) {
+            const int b = sh.place[i] / (uint32_t)a.vocab, c = sh.place[i + 1] / (uint32_t)a.vocab;
+            close |= unordered(sh.score[i]) - unordered(sh.score[i + 1]) <= a.slack &&
+                     (i + 1 == a.n || (b != c && !(sh.exact[b] && sh.exact[c])));
+        }
+        if (!__syncthreads_or(close)) break;
+        // every pair of one of the n best and any continuation within the slack
+        const int chosen = min(have, a.n);
+        const double least = have > a.n ? unordered(sh.score[a.n - 1]) - a.slack : -CUDART_INF;
+        auto against = [&](double score, int b) {
+            for (int i = 0; i < chosen; ++i) {
+                const int c = sh.place[i] / (uint32_t)a.vocab;
+                if (c != b && fabs(score - unordered(sh.score[i])) <= a.slack) sh.doubt[b] = sh.doubt[c] = 1;
             }
-            if (rank < a.n) { sh.list_s[rank] = s; sh.list_p[rank] = p; }
+        };
+        for (int b = tid; b < a.beams; b += kThreads)
+            if (is_finished(b)) against((double)sh.own[b], b);
+        for (int i = tid; i < slots; i += kThreads) {
+            uint32_t place;
+            const double score = candidate(i, place);
+            if (score > -CUDART_INF && score >= least) against(score, i / a.n);
         }
         __syncthreads();
-        have = min(total, a.n);
-        for (int i = tid; i < have; i += kThreads) { sh.score[i] = sh.list_s[i]; sh.place[i] = sh.list_p[i]; }
-        if (tid == 0) sh.count = have;
+        for (int b = 0; b < a.beams; ++b) {
+            if (!sh.doubt[b] || sh.exact[b]) continue;
+            const char* row = (const char*)a.logits + (blockIdx.x * a.stride_batch + b * a.stride_beam) * (a.dtype == 0 ? 4 : 2);
+            const float m = a.parts[first + b].m;
+            const double norm = a.dtype == 0 ? exact_norm((const float*)row, a.vocab, m, sh.red)
+                : a.dtype == 1 ? exact_norm((const __nv_bfloat16*)row, a.vocab, m, sh.red) : exact_norm((const __half*)row, a.vocab, m, sh.red);
+            if (tid == 0) sh.norm[b] = norm;
+        }
         __syncthreads();
     }
     for (int i = tid; i < a.n; i += kThreads) {
@@ -856,6 +940,15 @@ join_beams_kernel(BeamArgs a) {
         a.parents[to] = is ? (int64_t)(p / (uint32_t)a.vocab) : 0;
         a.out_scores[to] = is ? (float)unordered(sh.score[i]) : PCX_NEG_INF;
     }
+}
+
+// How far log_norm may be off, in steps of 2^-24 of the sum: an exponential of 2^-22 (4); its argument, rounded twice, whose distance
+// from the maximum is at most log2(vocab) + 2 bits on average under the weights (2 ln 2 each); the sums of a tile (34); for every
+// tile of a lane a sum, and a product with an exponential where the maximum rises (6), whose arguments add up to log2(vocab) bits
+// while anything is left of the sum; and as much where the lanes are joined.
+double norm_error(int vocab, int tiles) {
+    const double bits = std::log2((double)vocab) + 2.0;
+    return (4.0 + 34.0 + 6.0 * tiles + 12.0 + 4.0 * 0.7 * bits) * 5.9604644775390625e-8;
 }
 
 // ---- reordering of states --------------------------------------------------------------------------------------------
@@ -940,6 +1033,9 @@ cudaError_t launch_next(void (*kernel)(P...), unsigned grid, cudaStream_t stream
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
+// Groups a thread of a CTA that takes a part of a row, per tile
+int block_groups(int vocab, int ve, int splits) { return vocab / ve / splits > 3 * kThreads ? 8 : 2; }
+
 template <typename T>
 void launch_rows(const RowArgs& a, int64_t rows, bool warps, cudaStream_t stream) {
     if (warps) {
@@ -947,8 +1043,7 @@ void launch_rows(const RowArgs& a, int64_t rows, bool warps, cudaStream_t stream
         return;
     }
     const unsigned grid = (unsigned)(rows * a.splits);
-    const int64_t groups = a.vocab / Pack<T>::N / a.splits;
-    if (groups > 3 * kThreads) top_rows_block_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
+    if (block_groups(a.vocab, Pack<T>::N, a.splits) == 8) top_rows_block_kernel<T, 8><<<grid, kThreads, 0, stream>>>(a);
     else top_rows_block_kernel<T, 2><<<grid, kThreads, 0, stream>>>(a);
 }
 
@@ -1022,12 +1117,16 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
     a.scale = 1.4426950408889634f;
     const int rc = select_rows(a, dtype, scratch, rows, (cudaStream_t)stream);
     if (rc != 0) return rc;
+    const int ve = dtype == 0 ? 4 : 8, part = vocab / std::max(splits, 1);
+    const int in_tile = ve * (splits == 0 ? 32 * kGroups : kThreads * block_groups(vocab, ve, splits));
     BeamArgs j{};
     j.keys = (const u64*)((const char*)scratch + rows * std::max(splits, 1) * ((int64_t)n * 8 + (int64_t)sizeof(Part)));
     j.parts = (const Part*)(j.keys + rows * n);
     j.scores = scores; j.finished = finished;
     j.out_scores = out_scores; j.tokens = tokens; j.parents = parents;
+    j.logits = logits; j.stride_batch = stride_batch; j.stride_beam = stride_beam; j.dtype = dtype;
     j.beams = beams; j.n = n; j.vocab = vocab; j.pad_id = pad_id; j.normalize = normalize;
+    j.slack = 2.0 * norm_error(vocab, part / in_tile + 1);
     return (int)launch_next(join_beams_kernel, (unsigned)batch, (cudaStream_t)stream, j);
 }
 

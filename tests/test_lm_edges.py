@@ -83,3 +83,51 @@ def test_rows_of_large_logits_have_their_normaliser(value, dtype):
                 # (a normaliser beyond the range of fp32 is infinite)
                 if abs(want) < torch.finfo(torch.float32).max:
                     assert abs(n - want) <= norm_tol(V) + abs(want) * STEP, (temperature, n, want)
+
+
+def check_all_alike(x, scores, n, B, finished=None):
+    """One sequence, B times."""
+    rows = lambda t: t.expand(B, *t.shape[1:]).contiguous().cuda()
+    got = [t.cpu() for t in lm.beam_select(rows(x), rows(scores), n, None if finished is None else rows(finished), 3)]
+    want = best(x[0], scores[0], n, None if finished is None else finished[0], 3)
+    assert bool((got[1] == torch.tensor([w[1] for w in want])).all()) and bool((got[2] == torch.tensor([w[2] for w in want])).all())
+    for s, w in zip(got[0][0].tolist(), want):
+        assert s == w[0] or abs(s - w[0]) <= norm_tol(x.size(2)) + abs(w[0]) * STEP
+
+
+# (a warp a row, a CTA a row, parts of a row; a beam's rows begin at other places of 16 bytes than its neighbours')
+CUTS = [(2, 6, 257), (1, 6, 4501), (3, 5, 50257), (320, 6, 5001), (1, 128, 41)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,V", CUTS)
+def test_equal_beams_go_by_their_place(B, K, V, dtype):
+    x = (torch.randn(1, 1, V, generator=torch.Generator().manual_seed(V)) * 3).to(dtype).expand(1, K, V)
+    scores = torch.full((1, K), -3.0)
+    for n in (1, K - 1, K, min(2 * K + 1, 128)):
+        check_all_alike(x, scores, n, B)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,K,V", CUTS)
+def test_beams_whose_normalisers_differ_by_little(B, K, V, dtype):
+    """Rows that differ in a logit of next to no weight: the order of their continuations is that of their normalisers in 64 bits,
+    which are 1e-10 to 1e-6 apart."""
+    g = torch.Generator().manual_seed(K + V)
+    x = (torch.randn(1, 1, V, generator=g) * 3).to(dtype).expand(1, K, V).clone()
+    low = x[0, 0].float().argmin()
+    x[0, :, low] += (torch.randperm(K, generator=g).float() * (8.0 / K)).to(dtype)
+    scores = torch.full((1, K), -3.0)
+    norms = [exact_norm(row) for row in x[0].double().tolist()]
+    assert K < 10 and 1e-11 < max(norms) - min(norms) < 1e-4 or K == 128
+    for n in (2, K - 1, min(3 * K, 128)):
+        check_all_alike(x, scores, n, B)
+    # finished beams in between, at scores within a rounding of a continuation's
+    finished = torch.zeros(1, K, dtype=torch.bool)
+    finished[0, 1::3] = True
+    top = x[0, 0].double().max() - 3.0
+    for k in range(1, K, 3):
+        scores[0, k] = float(top) - norms[0]
+    check_all_alike(x, scores, K, B, finished)
