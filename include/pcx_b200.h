@@ -597,8 +597,8 @@ int pcx_reorder(const int64_t* states, int n_tensors, const void* parents, int w
 /* ---- Language-model operators: leaf tables under a teacher's top logits ---------------------------------------------
  * entries[v][b][k] = (category or -1, weight) (8 bytes each; v < vars, b < width, k < slots), made by pcx_teacher_prep from ids
  * and logits of any strides (in elements): a weight is exp(logit / temperature - norm), norm = norms[b, v], or (norms null, or
- * not finite) the logsumexp over the position's slots.  Negative ids, logits of -inf and NaN and columns from `batch` on are
- * empty.
+ * not finite, or a logit of +inf, which share the weight) the logsumexp over the position's slots.  Negative ids, logits of -inf and
+ * NaN and columns from `batch` on are empty.
  *   fwd   out[row0 + m, b] = sum_k weight[var][b][k] * log p_m(category)            (a category >= cats: -inf)
  *   bwd   table flow of (m, c) = sum over the group's vectors, b and k with category c of weight * flow[row0 + m, b]
  * A PcxTeacherGeo lists the leaf vectors (PcxTeacherSeg), the groups of vectors that share a table (PcxTeacherGroup) and the

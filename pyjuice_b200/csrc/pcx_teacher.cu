@@ -110,11 +110,11 @@ __global__ void __launch_bounds__(kTh) teacher_prep_kernel(PrepArgs a) {
         }
     };
     const float norm = a.norms != nullptr && b < a.B ? a.norms[b * a.nb + v * a.nv] : CUDART_INF_F;
-    const bool given = fabsf(norm) < CUDART_INF_F;
     float m = PCX_NEG_INF, sum = 0.0f;
     each([&](int, float x) { m = fmaxf(m, x); });
 #pragma unroll
     for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    const bool given = fabsf(norm) < CUDART_INF_F && m < CUDART_INF_F;       // (logits of +inf leave no other normaliser than theirs)
     auto raw = [&](float x) {
         if (x == PCX_NEG_INF) return 0.0f;
         if (given) return expf((float)((double)x * a.inv_t64 - (double)norm));

@@ -30,7 +30,7 @@ class TopLogits(NamedTuple):
     logits float32, bfloat16 or float16.  A slot is empty when its id is negative or its logit is -inf or NaN.  The weight
     of a slot is ``exp(logits / temperature - log_norm)``; without ``log_norm`` (the shape of ``ids`` less its last
     dimension), or where it is not finite, the weights of a position's slots sum to one.  A position whose slots are all
-    empty says nothing: it is marginalised.  Logits of +inf share the whole weight of their position."""
+    empty says nothing: it is marginalised.  Logits of +inf share the whole weight of their position, with or without ``log_norm``."""
     ids: torch.Tensor
     logits: torch.Tensor
     temperature: float = 1.0

@@ -131,3 +131,25 @@ def test_beams_whose_normalisers_differ_by_little(B, K, V, dtype):
     for k in range(1, K, 3):
         scores[0, k] = float(top) - norms[0]
     check_all_alike(x, scores, K, B, finished)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [3, 40, 300])
+def test_logits_of_plus_infinity_share_the_weight_under_a_given_normaliser(K):
+    ids = torch.arange(K).expand(1, 3, K)
+    x = torch.randn(1, 3, K, generator=torch.Generator().manual_seed(1))
+    x[0, 0, 1], x[0, 0, K - 1], x[0, 1, 0] = INF, INF, INF
+    log_probs = -torch.arange(1.0, K + 1).expand(2, K).contiguous()
+    log_probs[0, 0] = 0.0                              # (nothing of an infinite weight times zero)
+    norm = torch.tensor([[2.0, 0.0, 7.0]])
+    lp = log_probs.cuda().requires_grad_()
+    got = lm.expected_log_probs(lp, lm.TopLogits(ids.cuda(), x.cuda(), 1.0, norm.cuda()))
+    assert got[0, :, 0].tolist() == [-(2.0 + K) / 2] * 2                     # two of them, a half each
+    assert got[1, :, 0].tolist() == [0.0, -1.0]
+    q = (x[0, 2].double() - 7.0).exp()                 # the position without any keeps its normaliser
+    want = (q * log_probs.double()).sum(-1)
+    assert float((got[2, :, 0].detach().double().cpu() - want).abs().max()) <= (K + 12) * 2 * STEP * float(want.abs().max())
+    grad, = torch.autograd.grad(got[:2].sum(), lp)
+    want = torch.zeros(K)
+    want[1], want[K - 1], want[0] = 0.5, 0.5, 1.0
+    assert torch.equal(grad.cpu(), want.expand(2, K))
