@@ -43,7 +43,7 @@ class HMMDecoder:
 
     The parameters are taken over when the decoder is made and on ``reload()``; training the circuit later does not change
     it.  A state is a ``[num_latents, N]`` tensor: column n holds the logarithm of the distribution of beam n's next hidden
-    state given its tokens (up to rounding; ``log_probs`` does not rely on its sum)."""
+    state given its tokens, up to a constant, which ``log_probs`` takes out."""
 
     def __init__(self, pc: TensorCircuit):
         pc._require_cuda()
@@ -140,8 +140,13 @@ class HMMDecoder:
 
     @torch.no_grad()
     def log_probs(self, state: torch.Tensor) -> torch.Tensor:
-        """Log-probabilities of every beam's next token, ``[N, vocab]``."""
+        """Log-probabilities of every beam's next token, ``[N, vocab]``, whatever the columns' sums; -inf for a column of -inf."""
         self._check(state)
+        mass = state.logsumexp(0)
+        return self._next(state - mass.masked_fill_(mass == float("-inf"), 0.0))
+
+    def _next(self, state: torch.Tensor) -> torch.Tensor:
+        """As `log_probs`, joint with what a column's sum holds."""
         N = state.size(1)
         if N == 0:
             return torch.empty(0, self.vocab, device=self.device)
@@ -189,7 +194,7 @@ def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1,
     state = decoder.start(B)
     for t in range(prompts.size(1)):
         said = prompts[:, t].long()
-        state = decoder.advance(state, said, decoder.log_probs(state).gather(1, said.clamp(0, V - 1)[:, None])[:, 0])
+        state = decoder.advance(state, said, decoder._next(state).gather(1, said.clamp(0, V - 1)[:, None])[:, 0])
     scores = torch.zeros(B, 1, device=device)
     finished = torch.zeros(B, 1, dtype=torch.bool, device=device)
     tokens = torch.empty(B, 0, dtype=torch.int64, device=device)
@@ -197,7 +202,7 @@ def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1,
     for t in range(num_tokens):
         k = scores.size(1)
         n = min(K, k * V)
-        logits = decoder.log_probs(state).unflatten(0, (B, k))
+        logits = decoder._next(state).unflatten(0, (B, k))         # (the selection normalises)
         scores, parents, said = lm.beam_select(logits, scores, n, finished if eos_id is not None else None, pad)
         finished, tokens = lm.reorder(parents, finished.reshape(B * k), tokens.reshape(B * k, t))
         state, = lm.reorder(parents, state, dim=1)

@@ -153,3 +153,42 @@ def test_logits_of_plus_infinity_share_the_weight_under_a_given_normaliser(K):
     want = torch.zeros(K)
     want[1], want[K - 1], want[0] = 0.5, 0.5, 1.0
     assert torch.equal(grad.cpu(), want.expand(2, K))
+
+
+# ---- decoding: three products of 8-bit-mantissa halves per factor (2^-16 each way) and fp32 sums over the states, per token
+DECODE_TOL = 2.0 ** -13
+
+
+def hmm(latents, vocab, length=4, seed=0):
+    """A circuit and its (alpha, beta, gamma) in 64 bits."""
+    import pyjuice_b200 as pj
+    g = torch.Generator().manual_seed(seed)
+    p = lambda *s: torch.rand(*s, generator=g).pow(3).add_(1e-4)
+    alpha, beta, gamma = p(latents, latents), p(latents, vocab), p(latents)
+    alpha, beta, gamma = alpha / alpha.sum(1, keepdim=True), beta / beta.sum(1, keepdim=True), gamma / gamma.sum()
+    torch.manual_seed(seed)
+    ns = pj.structures.HMM(seq_length=length, num_latents=latents, num_emits=vocab, alpha=alpha, beta=beta, gamma=gamma)
+    return pj.compile(ns, verbose=False).to("cuda:0"), (alpha.double(), beta.double(), gamma.double())
+
+
+@pytest.mark.gpu
+def test_next_tokens_of_a_joint_state():
+    """Without the tokens' log-probabilities a state goes on as a joint distribution; the next token's probabilities are the same."""
+    from pyjuice_b200.decoding import HMMDecoder
+    pc, (alpha, beta, z) = hmm(20, 33)
+    decoder = HMMDecoder(pc)
+    state = decoder.start(2)
+    said = torch.tensor([[3, 7, 0, 32], [1, 1, 1, 1]])
+    rows = [z, z]
+    for t in range(4):
+        state = decoder.advance(state, said[:, t].cuda())
+        rows = [(r * beta[:, v]) @ alpha for r, v in zip(rows, said[:, t].tolist())]
+        got = decoder.log_probs(state)
+        want = torch.stack([((r / r.sum()) @ beta).log() for r in rows])
+        assert float((got.double().cpu() - want).abs().max()) < (t + 2) * DECODE_TOL
+        mass = torch.stack([r.sum().log() for r in rows])
+        assert float((state.logsumexp(0).double().cpu() - mass).abs().max()) < (t + 2) * DECODE_TOL
+    assert float((decoder.log_probs(state + 40) - got).abs().max()) < 40 * 8 * STEP + DECODE_TOL
+    state[:, 1] = NEG_INF                              # nothing is possible
+    got = decoder.log_probs(state)
+    assert bool((got[1] == NEG_INF).all()) and bool(got[0].isfinite().all())
