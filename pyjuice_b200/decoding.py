@@ -43,7 +43,8 @@ class HMMDecoder:
 
     The parameters are taken over when the decoder is made and on ``reload()``; training the circuit later does not change
     it.  A state is a ``[num_latents, N]`` tensor: column n holds the logarithm of the distribution of beam n's next hidden
-    state given its tokens, up to a constant, which ``log_probs`` takes out."""
+    state given its tokens, up to a constant, which ``log_probs`` takes out.  As in every circuit, a sum is at least 1e-24 of its
+    largest term: what has a probability of zero beside others that have not has that one."""
 
     def __init__(self, pc: TensorCircuit):
         pc._require_cuda()
@@ -65,8 +66,9 @@ class HMMDecoder:
         self._speak_ns = summate(state, num_node_blocks=self._v_pad // vbs, block_size=vbs)
         # transitions: the state of the previous position times the emission of its token
         state = inputs(0, num_node_blocks=L // bs, block_size=bs, dist=Categorical(1))
-        self._said_ns = inputs(1, num_node_blocks=L // bs, block_size=bs, dist=Categorical(V))
-        self._said_ns.set_params(torch.full((L, V), 1.0 / V), normalize=False)
+        # (two categories more: a token that the vocabulary does not have, one that is not known)
+        self._said_ns = inputs(1, num_node_blocks=L // bs, block_size=bs, dist=Categorical(V + 2))
+        self._said_ns.set_params(torch.full((L, V + 2), 1.0 / (V + 2)), normalize=False)
         self._step_ns = summate(multiply(state, self._said_ns), num_node_blocks=L // bs, block_size=bs)
         self._state_ns = state
         self._speak = compile(self._speak_ns, verbose=False).to(self.device)
@@ -128,7 +130,8 @@ class HMMDecoder:
         _set_dense(self._speak, self._speak_ns, spoken)
         leaf = self._step.input_layer_group[0]
         s, e = self._said_ns._param_range
-        leaf.params[s:e].copy_(emission.reshape(-1))
+        said = leaf.params[s:e].view(L, V + 2)
+        said[:, :V], said[:, V], said[:, V + 1] = emission, 0.0, 1.0
 
     def start(self, n: int) -> torch.Tensor:
         """States of ``n`` beams without tokens."""
@@ -159,7 +162,9 @@ class HMMDecoder:
     @torch.no_grad()
     def advance(self, state: torch.Tensor, tokens: torch.Tensor, log_probs: Optional[torch.Tensor] = None) -> torch.Tensor:
         """States after one more token each: ``tokens`` ``[N]``; ``log_probs`` ``[N]``: what the tokens had, which keeps the
-        probabilities of a column at a sum of one (without it they go on as joint probabilities with the tokens)."""
+        probabilities of a column at a sum of one (without it they go on as joint probabilities with the tokens).  A negative
+        token is one that is not known: the state goes on by the transition alone.  A token that is impossible, or that the
+        vocabulary does not have, leaves a column of -inf."""
         self._check(state)
         N = state.size(1)
         if tokens.shape != (N,) or tokens.is_floating_point():
@@ -167,8 +172,9 @@ class HMMDecoder:
         if N == 0:
             return state.clone()
         if log_probs is not None:
-            state = state - log_probs
-        x = torch.stack([torch.zeros_like(tokens), tokens.clamp(0, self.vocab - 1)], 1)
+            state = state - log_probs.nan_to_num(0.0, neginf=0.0)
+        tokens = tokens.long()
+        x = torch.stack([torch.zeros_like(tokens), tokens.clamp(-1, self.vocab).remainder_(self.vocab + 2)], 1)
         return self._step._values_of_inner([(self._state_ns, state)], N, x)[:, :N].clone()
 
 
@@ -178,7 +184,10 @@ def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1,
     """The likeliest continuations of ``prompts`` ``[B, P]`` (integer; None: ``batch`` empty ones) under an HMM circuit or an
     :class:`HMMDecoder`: tokens ``[B, num_beams, num_tokens]`` (int64) and their log-probabilities ``[B, num_beams]``, best
     first.  A beam that says ``eos_id`` is finished and goes on with ``eos_id`` at no cost.  Where there are fewer
-    continuations than beams the rest has the score -inf and tokens -1."""
+    continuations than beams the rest has the score -inf and tokens -1.
+
+    A negative token of a prompt is one that is not known (its position is marginalised, as a circuit's variable without slots);
+    after one that is impossible, or that the vocabulary does not have, there are no continuations."""
     decoder = pc if isinstance(pc, HMMDecoder) else HMMDecoder(pc)
     V, device = decoder.vocab, decoder.device
     if num_tokens < 1 or not 1 <= num_beams <= lm.MAX_TOP:
@@ -194,7 +203,8 @@ def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1,
     state = decoder.start(B)
     for t in range(prompts.size(1)):
         said = prompts[:, t].long()
-        state = decoder.advance(state, said, decoder._next(state).gather(1, said.clamp(0, V - 1)[:, None])[:, 0])
+        heard = decoder._next(state).gather(1, said.clamp(0, V - 1)[:, None])[:, 0]
+        state = decoder.advance(state, said, heard.masked_fill_(said < 0, 0.0))
     scores = torch.zeros(B, 1, device=device)
     finished = torch.zeros(B, 1, dtype=torch.bool, device=device)
     tokens = torch.empty(B, 0, dtype=torch.int64, device=device)

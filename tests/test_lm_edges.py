@@ -192,3 +192,69 @@ def test_next_tokens_of_a_joint_state():
     state[:, 1] = NEG_INF                              # nothing is possible
     got = decoder.log_probs(state)
     assert bool((got[1] == NEG_INF).all()) and bool(got[0].isfinite().all())
+
+
+def after(model, tokens):
+    """(log p(tokens), next-token log-probabilities) in 64 bits; None: a token that is not known."""
+    alpha, beta, z = model
+    total = 0.0
+    for t in tokens:
+        z = z if t is None else z * beta[:, t]
+        total += math.log(float(z.sum())) if t is not None else 0.0
+        z = (z / z.sum()) @ alpha
+    return total, (z @ beta).log()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("latents,vocab", [(20, 33), (16, 9), (64, 700)])
+def test_tokens_that_are_unknown_or_not_in_the_vocabulary(latents, vocab):
+    from pyjuice_b200.decoding import HMMDecoder, beam_search
+    pc, model = hmm(latents, vocab)
+    decoder = HMMDecoder(pc)
+    prompts = torch.tensor([[3, -1, 2], [-1, -7, -2 ** 40], [5, 1, -1], [5, vocab, 1], [2 ** 40, 1, 1], [4, 3, 2]])
+    names = lambda row: [None if t < 0 else t for t in row]
+    for ids in (torch.int64, torch.int32):
+        rows = prompts.clamp(-2 ** 31, 2 ** 31 - 1).to(ids)
+        tokens, scores = beam_search(decoder, rows, 1, 4)
+        for b, row in enumerate(prompts.tolist()):
+            if max(row) >= vocab:
+                assert bool((scores[b] == NEG_INF).all()) and bool((tokens[b] == -1).all())
+                continue
+            want, at = after(model, names(row))[1].sort(descending=True)
+            assert float((scores[b].double().cpu() - want[:4]).abs().max()) < 5 * DECODE_TOL
+            if float((want[:4] - want[1:5]).min()) > 10 * DECODE_TOL:
+                assert tokens[b, :, 0].tolist() == at[:4].tolist()
+    # the same through `advance`, with and without the tokens' log-probabilities; unsigned tokens
+    joint = own = decoder.start(6)
+    for t in range(3):
+        said = prompts[:, t].cuda()
+        heard = decoder.log_probs(own).gather(1, said.clamp(0, vocab - 1)[:, None])[:, 0]
+        own = decoder.advance(own, said, torch.where(said < 0, 0.0, heard))
+        joint = decoder.advance(joint, said)
+    a, b = decoder.log_probs(own).double().cpu(), decoder.log_probs(joint).double().cpu()
+    for n, row in enumerate(prompts.tolist()):
+        if max(row) >= vocab:
+            assert bool((own[:, n] == NEG_INF).all()) and bool((joint[:, n] == NEG_INF).all()) and bool((a[n] == NEG_INF).all())
+        else:
+            total, want = after(model, names(row))
+            assert float((a[n] - want).abs().max()) < 5 * DECODE_TOL and float((b[n] - want).abs().max()) < 5 * DECODE_TOL
+            assert abs(float(joint[:, n].logsumexp(0)) - total) < 5 * DECODE_TOL
+    assert torch.equal(decoder.advance(decoder.start(1), torch.tensor([7], dtype=torch.uint8).cuda()), decoder.advance(decoder.start(1), torch.tensor([7]).cuda()))
+
+
+@pytest.mark.gpu
+def test_an_impossible_token_ends_its_own_beam_alone():
+    import pyjuice_b200 as pj
+    from pyjuice_b200.decoding import HMMDecoder, beam_search
+    eye = torch.eye(4)
+    beta = torch.cat([eye, torch.zeros(4, 2)], 1)              # state z says token z; tokens 4 and 5 are never said
+    alpha = torch.roll(eye, 1, 1)                              # and is followed by the next state
+    ns = pj.structures.HMM(seq_length=3, num_latents=4, num_emits=6, alpha=alpha, beta=beta, gamma=torch.full((4,), 0.25))
+    decoder = HMMDecoder(pj.compile(ns, verbose=False).to("cuda:0"))
+    tokens, scores = beam_search(decoder, torch.tensor([[4], [1], [5], [-1]]), 3, 2)
+    assert bool((scores[[0, 2]] == NEG_INF).all()) and bool((tokens[[0, 2]] == -1).all())
+    assert tokens[1, 0].tolist() == [2, 3, 0] and abs(float(scores[1, 0])) < 3 * DECODE_TOL
+    # a sum of the circuit's kernels is 1e-24 of its largest term at least, so that a sentence of probability zero has log(1e-24) (and
+    # the selection's normaliser is off by 5 tokens of it: nothing)
+    assert abs(float(scores[1, 1]) - math.log(1e-24)) < 3 * DECODE_TOL + 55.3 * STEP
+    assert bool((scores[3] + math.log(4)).abs().max() < 3 * DECODE_TOL)
