@@ -16,6 +16,7 @@ from typing import List, NamedTuple, Optional, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -56,6 +57,12 @@ def _require_cuda(*tensors):
             raise NotImplementedError("language-model operators run on CUDA only (no CPU path)")
         if t is not None and t.device != device:
             raise ValueError(f"tensors on {device} and {t.device}")
+
+
+def _refuse_tangents(name: str, *tensors):
+    if getattr(forward_ad, "_current_level", 0) >= 0:            # (only within a level of forward-mode differentiation)
+        if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise RuntimeError(f"`{name}` has no forward-mode derivative")
 
 
 class _Geo(ctypes.Structure):
@@ -243,8 +250,9 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
     ``log_probs`` (float32) is ``[M, C]``, one table of M nodes for all T positions, or ``[T, M, C]``, a table for each.
     Empty slots add nothing, whatever they hold; a weight of zero takes nothing of a log-probability of -inf; an id of C
     or more has the log-probability -inf.  Returns float32 ``[T, M, B]``.  The gradient goes to ``log_probs`` (sums in a
-    fixed order: the same bits on every call), none to the teacher.  Up to a million categories.  A backward pass captured
-    into a CUDA graph needs, as torch's own do, that no eager graph of the same leaf is alive while it is captured."""
+    fixed order: the same bits on every call), none to the teacher; second and forward-mode derivatives are refused.  Up
+    to a million categories.  A backward pass captured into a CUDA graph needs, as torch's own do, that no eager graph of the
+    same leaf is alive while it is captured."""
     teacher._check()
     if log_probs.dtype != torch.float32 or log_probs.dim() not in (2, 3):
         raise TypeError("log_probs must be float32 [M, C] or [T, M, C]")
@@ -259,6 +267,7 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
         raise ValueError("more than 2^30 slots share a table")
     if T * log_probs.size(-2) >= 2 ** 31:
         raise ValueError("more than 2^31 nodes over all positions")
+    _refuse_tangents("expected_log_probs", log_probs)
     _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
     if log_probs.requires_grad and torch.is_grad_enabled():
         return _Expected.apply(log_probs, teacher)
@@ -408,6 +417,7 @@ def reorder(parents: torch.Tensor, *states: torch.Tensor, dim: int = 0) -> List[
                              (f" of {beams}" if beams is not None else ""))
         beams = width // B if B > 0 else 1
         moved.append((x, at, size))
+    _refuse_tangents("reorder", *states)
     _require_cuda(parents, *states)
     parents, device = parents.contiguous(), parents.device
     out, held, rows = [], [], []

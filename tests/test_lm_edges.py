@@ -258,3 +258,22 @@ def test_an_impossible_token_ends_its_own_beam_alone():
     # the selection's normaliser is off by 5 tokens of it: nothing)
     assert abs(float(scores[1, 1]) - math.log(1e-24)) < 3 * DECODE_TOL + 55.3 * STEP
     assert bool((scores[3] + math.log(4)).abs().max() < 3 * DECODE_TOL)
+
+
+def test_forward_mode_derivatives_are_refused():
+    from torch.autograd import forward_ad
+    lp, parents = torch.zeros(4, 9), torch.zeros(2, 3, dtype=torch.int64)
+    teacher = lm.TopLogits(torch.zeros(2, 3, 5, dtype=torch.int64), torch.zeros(2, 3, 5))
+    calls = (lambda x: lm.expected_log_probs(x, teacher), lambda x: lm.reorder(parents, x)[0])
+    for f in calls:
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                f(forward_ad.make_dual(lp, torch.ones_like(lp)))
+            with pytest.raises(NotImplementedError):               # (a tensor without a tangent: no CPU path, as ever)
+                f(lp)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            torch.func.jvp(f, (lp,), (torch.ones_like(lp),))
+        with pytest.raises(NotImplementedError):
+            f(lp)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+        calls[0](forward_ad.make_dual(lp.clone().requires_grad_(), torch.ones_like(lp)))
