@@ -416,8 +416,9 @@ template <bool VEC_IN>
 __global__ void __launch_bounds__(kTh) teacher_turn_flows_kernel(float* __restrict__ out, const float* __restrict__ flows, Geo g,
                                                                 int m_tiles, int logspace) {
     __shared__ float tile[kTurn][kTurn + 1];
-    const Seg seg = seg_of(g, blockIdx.x / m_tiles);
-    const int m0 = (blockIdx.x % m_tiles) * kTurn, b0 = blockIdx.y * kTurn, mp = pad4(seg.M);
+    const unsigned tiles = (unsigned)g.n_segs * m_tiles, at = blockIdx.x % tiles;
+    const Seg seg = seg_of(g, at / m_tiles);
+    const int m0 = at % m_tiles * kTurn, b0 = blockIdx.x / tiles * kTurn, mp = pad4(seg.M);
     if (m0 >= seg.M) return;
     turn_tile<VEC_IN, true>(tile, flows + (seg.row0 + m0) * g.W + b0, g.W, min(kTurn, seg.M - m0), min(kTurn, g.W - b0),
                             out + seg.gcol * g.W + (int64_t)b0 * mp + m0, mp, min(kTurn, mp - m0),
@@ -1025,8 +1026,9 @@ int pcx_teacher_bwd(float* out, int32_t* touched, void* scratch, const float* fl
     float* turned = (float*)(base + l.flows);
     {
         const int m_tiles = (int)pcx_cdiv(geo->nodes, kTurn);
-        if ((int64_t)m_tiles * geo->n_segs > 0x7fffffff || pcx_cdiv(geo->width, kTurn) > 65535) return -1;
-        const dim3 grid((unsigned)(m_tiles * geo->n_segs), (unsigned)pcx_cdiv(geo->width, kTurn));
+        const int64_t blocks = (int64_t)m_tiles * geo->n_segs * pcx_cdiv(geo->width, kTurn);
+        if (blocks > 0x7fffffff) return -1;
+        const unsigned grid = (unsigned)blocks;
         if (geo->width % 4 == 0 && (uintptr_t)flows % 16 == 0) teacher_turn_flows_kernel<true><<<grid, kTh, 0, st>>>(turned, flows, g, m_tiles, logspace);
         else teacher_turn_flows_kernel<false><<<grid, kTh, 0, st>>>(turned, flows, g, m_tiles, logspace);
         PCX_LAUNCH_CHECK();

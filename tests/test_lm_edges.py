@@ -277,3 +277,21 @@ def test_forward_mode_derivatives_are_refused():
             f(lp)
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
         calls[0](forward_ad.make_dual(lp.clone().requires_grad_(), torch.ones_like(lp)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [True, False])
+def test_more_samples_than_a_grid_has_rows(tied):
+    """4.2 million samples, both directions: 65536 tiles of 64 samples and a few."""
+    B, M, C = 65536 * 64 + 37, 2, 3
+    g = torch.Generator().manual_seed(0)
+    ids = torch.randint(-1, C, (B, 1, 1), generator=g).cuda()
+    lp = torch.randn(M, C, generator=g).cuda() if tied else torch.randn(1, M, C, generator=g).cuda()
+    lp.requires_grad_()
+    out = lm.expected_log_probs(lp, lm.TopLogits(ids, torch.zeros(B, 1, 1, device="cuda")))
+    table, at = lp.detach().view(M, C), ids.flatten()
+    assert torch.equal(out.detach()[0], torch.where(at >= 0, table[:, at.clamp_min(0)], 0.0))
+    flow = torch.randint(0, 3, (1, M, B), generator=g).float().cuda()            # (sums of whole numbers below 2^24 are exact)
+    grad, = torch.autograd.grad(out, lp, flow)
+    want = torch.stack([flow[0][:, at == c].double().sum(1) for c in range(C)], 1)
+    assert float(want.max()) < 2 ** 24 and torch.equal(grad.view(M, C).double(), want)
