@@ -372,7 +372,8 @@ class TensorCircuit(nn.Module):
         self._fusing_dev = [(start, n, torch.tensor(accs, dtype=torch.int64, device=device))
                             for start, n, accs in self._tied_sum_groups]
         self._nm = self._em = self._nf = self._ef = self.param_flows = None
-        self._data_buf = self._token_buf = self._teacher_buf = self._root_view = self._root_w = self._cum_buf = None
+        self._data_buf = self._token_buf = self._root_view = self._root_w = self._cum_buf = None
+        self._teacher_bufs = []
         if device.type == "cuda":
             self._mask_parentless_in_device_tables()
         self._setup_fusion()
@@ -573,7 +574,7 @@ class TensorCircuit(nn.Module):
         """The batch as ``[V, W]`` int32 (variables outermost, batch padded with category 0), the layout every leaf
         kernel reads.  ``out`` is written when it fits."""
         if isinstance(inputs, TopLogits):
-            return self._prepare_teacher(inputs, out)
+            return self._prepare_teacher(inputs)
         assert inputs.dim() == 2 and inputs.size(1) >= self.num_vars
         if inputs.is_floating_point():
             raise TypeError("categorical inputs must be an integer tensor")
@@ -587,8 +588,9 @@ class TensorCircuit(nn.Module):
         _lib.call("pcx_load_inputs", out, x, x.element_size(), B, V, x.stride(0), x.stride(1), W)
         return out
 
-    def _prepare_teacher(self, teacher: TopLogits, out: Optional[Entries] = None) -> Entries:
-        """The slots of a teacher, variables outermost, batch padded with empty slots."""
+    def _prepare_teacher(self, teacher: TopLogits, keep: bool = False) -> Entries:
+        """The slots of a teacher, variables outermost, batch padded with empty slots.  ``keep``: in a buffer that captured
+        passes go by."""
         teacher._check()
         if teacher.ids.dim() != 3 or teacher.ids.size(1) < self.num_vars or teacher.ids.size(2) < 1:
             raise ValueError(f"the teacher's ids must be [B, {self.num_vars}, K] with at least one slot")
@@ -598,9 +600,22 @@ class TensorCircuit(nn.Module):
             raise ValueError("more than 2^30 slots in a batch")
         move = lambda t: t if t is None else t[:, :self.num_vars].to(self.device, non_blocking=True)
         shape = (self.num_vars, W, K, 2)
-        if out is None or tuple(out.tensor.shape) != shape:
-            out = Entries(torch.empty(shape, dtype=torch.int32, device=self.device))
+        out = self._teacher_buffer(shape) if keep else Entries(torch.empty(shape, dtype=torch.int32, device=self.device))
         _prepare(teacher._replace(ids=move(teacher.ids), logits=move(teacher.logits), log_norm=move(teacher.log_norm)), W, out.tensor)
+        return out
+
+    def _teacher_buffer(self, shape) -> Entries:
+        """The buffer for slots of one shape.  The last two shapes keep theirs; the captured passes on any other go with it
+        (they hold the workspaces of a backward pass: for 128 positions of 4096 states and 64 samples 134 MB of flows each)."""
+        out = next((e for e in self._teacher_bufs if tuple(e.tensor.shape) == shape), None)
+        others = [e for e in self._teacher_bufs if e is not out]
+        if out is None:
+            out = Entries(torch.empty(shape, dtype=torch.int32, device=self.device))
+        self._teacher_bufs = [out] + others[:1]
+        for gone in others[1:]:
+            at = gone.data_ptr()
+            self._graphs = {k: g for k, g in self._graphs.items() if k[0] not in ("fw", "bk") or at not in k}
+            self._bk_par_pending = {k: v for k, v in self._bk_par_pending.items() if at not in k}
         return out
 
     def _run_inner(self, key, fn):
@@ -856,7 +871,7 @@ class TensorCircuit(nn.Module):
         origin_inputs = inputs
         with torch.no_grad():
             if isinstance(inputs, TopLogits):
-                data = self._teacher_buf = self._prepare_teacher(inputs, self._teacher_buf)
+                data = self._prepare_teacher(inputs, keep=True)
                 B = inputs.ids.size(0)
             else:
                 data, B = None, inputs.size(0)

@@ -295,3 +295,30 @@ def test_more_samples_than_a_grid_has_rows(tied):
     grad, = torch.autograd.grad(out, lp, flow)
     want = torch.stack([flow[0][:, at == c].double().sum(1) for c in range(C)], 1)
     assert float(want.max()) < 2 ** 24 and torch.equal(grad.view(M, C).double(), want)
+
+
+@pytest.mark.gpu
+def test_batches_of_many_slot_counts_leave_no_passes_behind():
+    """Captured passes of two slot counts at most, whatever comes; each replays on the buffer it was captured with."""
+    pc, _ = hmm(128, 700, length=16)
+    g = torch.Generator().manual_seed(0)
+    top = lambda K: lm.TopLogits(torch.randint(700, (32, 16, K), generator=g).cuda(), torch.randn(32, 16, K, generator=g).cuda())
+
+    def step(teacher):
+        pc.init_param_flows(flows_memory=0.0)
+        lls = pc(teacher).detach().clone()
+        pc.backward(teacher)
+        return lls, pc.input_layer_group[0].param_flows.clone()
+
+    held, counts = [], []
+    for K in (3, 3, 3, 8, 8, 3, 8, 3, 5, 5, 5, 3, 3, 3, 1, 1, 1, 9, 9, 9, 12, 12, 12, 20, 20, 20, 3, 3, 3):
+        teacher = top(K)
+        held.append((teacher, step(teacher)))
+        counts.append((len(pc._graphs), len(pc._bk_par_pending)))
+    # a first pass and those after it (with and without new tables), twice, forward and backward
+    assert max(c for c, _ in counts[8:]) <= max(c for c, _ in counts[:8]) and max(c for _, c in counts) <= 4
+    assert len(pc._teacher_bufs) == 2
+    pc.use_cuda_graphs = False
+    for teacher, (lls, flows) in held:
+        eager = step(teacher)
+        assert torch.equal(eager[0], lls) and torch.equal(eager[1], flows)
