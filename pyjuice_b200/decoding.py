@@ -20,6 +20,12 @@ def _power_of_two(n: int, most: int) -> int:
     return min(n & -n, most)
 
 
+def _padded(n: int) -> int:
+    """States as the decoder holds them: in blocks of 64 nodes at least, so that the tiles of parameters are few and large (1000 states
+    and 8000 tokens in blocks of 8: more than a second of host time for every layout)."""
+    return -(-n // 64) * 64
+
+
 def _dense(pc: TensorCircuit, ns) -> torch.Tensor:
     """Parameters of a fully connected sum vector, ``[nodes, children]``."""
     p = pc.get_node_params(ns)
@@ -29,13 +35,19 @@ def _dense(pc: TensorCircuit, ns) -> torch.Tensor:
 
 
 def _set_dense(pc: TensorCircuit, ns, weights: torch.Tensor):
-    """Writes ``weights`` ``[nodes, children]`` into the parameters of a fully connected sum vector, as they are."""
+    """Writes ``weights`` ``[nodes, children]`` into the parameters of a fully connected sum vector, as they are; the nodes and
+    children that it lacks get zeros."""
     s, e = ns._param_range
     order = ((ns._param_ids - s) // (ns.block_size * ns.ch_block_size)).to(pc.device)
-    full = weights.view(ns.num_node_blocks, ns.block_size, ns.num_ch_node_blocks, ns.ch_block_size)
+    rows, cols = ns.edge_ids[0].to(pc.device), ns.edge_ids[1].to(pc.device)
+    full = torch.zeros(ns.num_node_blocks * ns.block_size, ns.num_ch_node_blocks * ns.ch_block_size, device=pc.device)
+    full[:weights.size(0), :weights.size(1)] = weights
+    full = full.view(ns.num_node_blocks, ns.block_size, ns.num_ch_node_blocks, ns.ch_block_size)
     tiles = pc.params[s:e].view(order.numel(), ns.ch_block_size, ns.block_size)      # (tables derived from them follow)
-    for at, i, j in zip(order.tolist(), ns.edge_ids[0].tolist(), ns.edge_ids[1].tolist()):
-        tiles[at].copy_(full[i, :, j].t())
+    some = max(1, (1 << 24) // (ns.block_size * ns.ch_block_size))                   # 64 MB of tiles at a time
+    for at in range(0, order.numel(), some):
+        i, j, k = rows[at:at + some], cols[at:at + some], order[at:at + some]
+        tiles[k] = full[i, :, j].transpose(1, 2)
 
 
 class HMMDecoder:
@@ -54,7 +66,7 @@ class HMMDecoder:
         self._root, self._transition, self._emission = root, chain[0], chain[1]
         self.num_latents = self._emission.num_nodes
         self.vocab = self._emission.dist.num_cats
-        L, V = self.num_latents, self.vocab
+        V, L = self.vocab, _padded(self.num_latents)
         bs = _power_of_two(L, 1024)
         # emissions: sum nodes are tokens, padded to whole blocks with nodes of probability zero
         vbs = 1
@@ -124,14 +136,12 @@ class HMMDecoder:
         s, e = self._emission._param_range
         emission = layer.params.data[s:e].view(L, V)
         self._initial = _dense(self.pc, self._root).view(L).log()
-        _set_dense(self._step, self._step_ns, _dense(self.pc, self._transition).t().contiguous())
-        spoken = torch.zeros(self._v_pad, L, device=self.device)
-        spoken[:V] = emission.t()
-        _set_dense(self._speak, self._speak_ns, spoken)
+        _set_dense(self._step, self._step_ns, _dense(self.pc, self._transition).t())
+        _set_dense(self._speak, self._speak_ns, emission.t())
         leaf = self._step.input_layer_group[0]
         s, e = self._said_ns._param_range
-        said = leaf.params[s:e].view(L, V + 2)
-        said[:, :V], said[:, V], said[:, V + 1] = emission, 0.0, 1.0
+        said = leaf.params[s:e].view(-1, V + 2)
+        said[:L, :V], said[:L, V], said[:L, V + 1], said[L:] = emission, 0.0, 1.0, 0.0
 
     def start(self, n: int) -> torch.Tensor:
         """States of ``n`` beams without tokens."""
@@ -175,16 +185,17 @@ class HMMDecoder:
             state = state - log_probs.nan_to_num(0.0, neginf=0.0)
         tokens = tokens.long()
         x = torch.stack([torch.zeros_like(tokens), tokens.clamp(-1, self.vocab).remainder_(self.vocab + 2)], 1)
-        return self._step._values_of_inner([(self._state_ns, state)], N, x)[:, :N].clone()
+        return self._step._values_of_inner([(self._state_ns, state)], N, x)[:self.num_latents, :N].clone()
 
 
 @torch.no_grad()
 def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1, num_beams: int = 4, batch: int = 1,
                 eos_id: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The likeliest continuations of ``prompts`` ``[B, P]`` (integer; None: ``batch`` empty ones) under an HMM circuit or an
-    :class:`HMMDecoder`: tokens ``[B, num_beams, num_tokens]`` (int64) and their log-probabilities ``[B, num_beams]``, best
-    first.  A beam that says ``eos_id`` is finished and goes on with ``eos_id`` at no cost.  Where there are fewer
-    continuations than beams the rest has the score -inf and tokens -1.
+    :class:`HMMDecoder` (a circuit is laid out for decoding in every call: keep a decoder to ask more than once): tokens ``[B,
+    num_beams, num_tokens]`` (int64) and their log-probabilities ``[B, num_beams]``, best first.  A beam that says ``eos_id`` is
+    finished and goes on with ``eos_id`` at no cost.  Where there are fewer continuations than beams the rest has the score -inf and
+    tokens -1.
 
     A negative token of a prompt is one that is not known (its position is marginalised, as a circuit's variable without slots);
     after one that is impossible, or that the vocabulary does not have, there are no continuations."""

@@ -835,7 +835,8 @@ class TensorCircuit(nn.Module):
 
     def _values_of_inner(self, leaves, B: int, inputs: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Log-values of the root nodes, ``[num_roots, W]`` (a view of the value buffer), for B columns whose input vectors
-        hold given log-values: ``leaves`` lists (vector, ``[nodes, B]``); the other vectors look at ``inputs``."""
+        hold given log-values: ``leaves`` lists (vector, ``[nodes, B]``; nodes that the values lack have -inf); the other vectors look
+        at ``inputs``."""
         self._require_cuda()
         with torch.no_grad(), _lib.use_sum_mode(self.sum_mode):
             self._ensure_buffers(B)
@@ -846,7 +847,9 @@ class TensorCircuit(nn.Module):
                     layer.forward(data, self._nm)
             for ns, values in leaves:
                 s, e = ns._output_ind_range
-                self._nm[s:e, :B].copy_(values)
+                self._nm[s:s + values.size(0), :B].copy_(values)
+                if values.size(0) < e - s:
+                    self._nm[s + values.size(0):e, :B].fill_(NEG_INF)
             plan = self._column_plan()
             if _lib.sum_mode() != 0 and self._packer.stale(self._sum_params, plan):
                 self._packer.prepare(plan)

@@ -322,3 +322,30 @@ def test_batches_of_many_slot_counts_leave_no_passes_behind():
     for teacher, (lls, flows) in held:
         eager = step(teacher)
         assert torch.equal(eager[0], lls) and torch.equal(eager[1], flows)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("latents,vocab", [(1, 5), (2, 1), (3, 70), (20, 33), (64, 65), (65, 300), (96, 1000), (130, 9), (201, 500), (1000, 2001)])
+def test_decoders_of_any_number_of_states(latents, vocab):
+    """Blocks of 64 states at least, few tiles of parameters, and the distributions of the definition."""
+    from pyjuice_b200.decoding import HMMDecoder, beam_search
+    pc, model = hmm(latents, vocab)
+    decoder = HMMDecoder(pc)
+    for ns in (decoder._speak_ns, decoder._step_ns):
+        assert ns.edge_ids.size(1) <= (latents / 64 + 1) * (max(latents, vocab) / 64 + 2)
+    said = torch.randint(vocab, (3, 3), generator=torch.Generator().manual_seed(1))
+    state, joint = decoder.start(3), decoder.start(3)
+    for t in range(3):
+        got, again = decoder.log_probs(state), decoder.log_probs(joint)
+        assert state.shape == (latents, 3) and got.shape == (3, vocab)
+        want = torch.stack([after(model, row[:t].tolist())[1] for row in said])
+        assert float((got.double().cpu() - want).abs().max()) < (t + 1) * DECODE_TOL
+        assert float((again.double().cpu() - want).abs().max()) < (t + 1) * DECODE_TOL
+        tokens = said[:, t].cuda()
+        state = decoder.advance(state, tokens, got.gather(1, tokens[:, None])[:, 0])
+        joint = decoder.advance(joint - 400.0, tokens)             # (a state of any size: what it lacks does not show)
+    before = decoder.log_probs(state)
+    decoder.reload()
+    assert torch.equal(decoder.log_probs(state), before)
+    tokens, scores = beam_search(decoder, said, 2, 3)
+    assert tokens.shape == (3, 3, 2) and bool(scores[:, :min(3, vocab)].isfinite().all())
