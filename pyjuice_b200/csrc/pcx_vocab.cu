@@ -12,6 +12,7 @@
 // For beams another kernel joins the rows of a sequence and adds the scores, in 64 bits: a sum of a score and a logit is
 // rounded only in the returned score, never before it is compared.
 #include "pcx_common.cuh"
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <algorithm>
@@ -61,15 +62,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // scale), more slowly.
 constexpr float kNear = 2147483648.0f;
 __device__ __forceinline__ bool near(float r) { return fabsf(r) < kNear; }
-// What the sum relative to (m, r) is multiplied by to be relative to (top, nr).
+// What the sum relative to (m, r) is multiplied by to be relative to (top, nr): the difference of the r is taken to the last bit.
 __device__ __forceinline__ float to_other(float m, float r, float top, float nr, float scale) {
-    if (m == top) return 1.0f;
-    if (near(r) && near(nr)) return exp2_fast(r - nr);
+    if (near(r) && near(nr)) {
+        const float d = r - nr, z = d - r, rest = (r - (d - z)) - (nr + z);
+        const float f = exp2_fast(d);
+        return fmaf(f, rest * 0.69314718f, f);
+    }
     return exp2_fast((m - top) * scale + (near(r) ? fmaf(-m, scale, r) : 0.0f) - (near(nr) ? fmaf(-top, scale, nr) : 0.0f));
 }
-// The sum relative to m itself.
-__device__ __forceinline__ double to_own(float s, float m, float r, float scale) {
-    return near(r) ? (double)s * exp2((double)fmaf(-m, scale, r)) : (double)s;
+// The sum relative to (m, r) as one relative to M >= m itself.
+__device__ __forceinline__ double to_own(float s, float m, float r, float M, float scale) {
+    if (!(m > PCX_NEG_INF) || !(M < CUDART_INF_F)) return 0.0;
+    if (near(r)) return (double)s * exp2((double)r - (double)M * (double)scale);
+    return m == M ? (double)s : (double)s * exp2(((double)m - (double)M) * (double)scale);
+}
+__device__ __forceinline__ double warp_sum(double x) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+    return x;
 }
 
 // 16 bytes of logits: their maximum (NaN skipped) and the logits one by one.
@@ -105,6 +116,20 @@ template <> struct Pack<__half> {
         return i & 1 ? __high2float(h) : __low2float(h);
     }
 };
+
+// Their terms: three sums one after the other at most.
+template <typename T>
+__device__ __forceinline__ float group_sum(const uint4& v, float scale, float r) {
+    constexpr int VE = Pack<T>::N;
+    float t[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) t[i] = exp2_fast(fmaf(Pack<T>::at(v, i), scale, -r));
+#pragma unroll
+    for (int o = VE / 2; o; o /= 2)
+#pragma unroll
+        for (int i = 0; i < o; ++i) t[i] += t[i + o];
+    return t[0];
+}
 
 // The 16 bytes of elements e ... of a row, -inf beyond its ends.  (Out of line, as everything that few tiles need: the warps
 // of an SM are in different places of the code, and it has to fit the instruction cache.)
@@ -256,7 +281,7 @@ __device__ __forceinline__ void block_stats(Shared& sh, float m, double s, doubl
     if (threadIdx.x == 0 && M > PCX_NEG_INF && M < CUDART_INF_F)
 #pragma unroll
         for (int w = 0; w < kWarps; ++w)
-            if (sh.red_m[w] > PCX_NEG_INF) S += sh.red_s[w] * exp((double)(sh.red_m[w] - M) * inv_t);
+            if (sh.red_m[w] > PCX_NEG_INF) S += sh.red_s[w] * exp(((double)sh.red_m[w] - (double)M) * inv_t);
 }
 
 // An answer of top logits, or a part of one.
@@ -337,17 +362,15 @@ __device__ __forceinline__ int warp_before(int& n) {
 template <typename T>
 __device__ __noinline__ float careful_sum(const T* x, int first, int groups, int step, int end, float m, float r, float scale) {
     constexpr int VE = Pack<T>::N;
-    float s[2] = {};
+    double s = 0.0;
 #pragma unroll 1
-    for (int i = 0; i < groups * VE; i += 2)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int e = first + i / VE * step + i % VE + h;
-            if (e < 0 || e >= end) continue;
-            const float f = fmaxf((float)x[e], PCX_NEG_INF);
-            s[h] += exp2_fast(near(r) ? fmaf(f, scale, -r) : f == m ? 0.0f : (f - m) * scale);
-        }
-    return s[0] + s[1];
+    for (int i = 0; i < groups * VE; ++i) {
+        const int e = first + i / VE * step + i % VE;
+        if (e < 0 || e >= end) continue;
+        const float f = fmaxf((float)x[e], PCX_NEG_INF);
+        s += (double)exp2_fast(near(r) ? fmaf(f, scale, -r) : f == m ? 0.0f : (f - m) * scale);
+    }
+    return (float)s;
 }
 
 // Many rows, or short ones: a warp a row, sixteen rows under way per SM (128 registers: a tile is on its way while the one
@@ -413,12 +436,10 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
                 if (m > PCX_NEG_INF) {
                     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < G; ++j)
-#pragma unroll
-                        for (int i = 0; i < VE; i += 2) {
-                            s0 += exp2_fast(fmaf(Pack<T>::at(v[j], i), a.scale, -r));
-                            s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
-                        }
+                    for (int j = 0; j < G; j += 2) {
+                        s0 += group_sum<T>(v[j], a.scale, r);
+                        s1 += group_sum<T>(v[j + 1], a.scale, r);
+                    }
                     s0 += s1;
                     if (!(s0 < CUDART_INF_F) || !near(r))
                         s0 = careful_sum<T>(x, (chunk + t * 32 * G + lane) * VE - off, G, 32 * VE, a.vocab, m, r, a.scale);
@@ -522,15 +543,11 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
             __syncwarp();
         }
     }
-    // statistics in fp32
+    // the lanes' sums become one in 64 bits
     float M = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
-    const float R = M * a.scale;
-    s = m > PCX_NEG_INF ? s * to_other(m, r, M, R, a.scale) : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    const double S = M > PCX_NEG_INF && M < CUDART_INF_F ? to_own(s, M, R, a.scale) : 0.0;
+    const double S = warp_sum(to_own(s, m, r, M, a.scale));
     // the set in order: a key's place is the number of larger ones
     if (count > a.n + a.n / 2 + 16) count = cut(keys, count, a.n, &bound);
     __syncwarp();
@@ -609,12 +626,10 @@ top_rows_block_kernel(RowArgs a) {
             if (m > PCX_NEG_INF) {
                 float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int i = 0; i < VE; i += 2) {
-                        s0 += exp2_fast(fmaf(Pack<T>::at(v[j], i), a.scale, -r));
-                        s1 += exp2_fast(fmaf(Pack<T>::at(v[j], i + 1), a.scale, -r));
-                    }
+                for (int j = 0; j < G; j += 2) {
+                    s0 += group_sum<T>(v[j], a.scale, r);
+                    s1 += group_sum<T>(v[j + 1], a.scale, r);
+                }
                 s0 += s1;
                 if (!(s0 < CUDART_INF_F) || !near(r))
                     s0 = careful_sum<T>(x, (g + tid) * VE - off, G, kThreads * VE, min(a.vocab, g1 * VE - off), m, r, a.scale);
@@ -698,18 +713,13 @@ top_rows_block_kernel(RowArgs a) {
             if (have == a.n) bound = value_of(sh.keys[a.n - 1]);
         }
     }
-    // a warp's statistics in fp32 ...
+    // the lanes' and warps' sums become one in 64 bits
     float wm = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(~0u, wm, o));
-    const float wr = wm * a.scale;
-    s = m > PCX_NEG_INF ? s * to_other(m, r, wm, wr, a.scale) : 0.0f;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    // ... and those of the warps in 64 bits
     float M;
     double S;
-    block_stats(sh, wm, to_own(s, wm, wr, a.scale), a.inv_t, M, S);
+    block_stats(sh, wm, warp_sum(to_own(s, m, r, wm, a.scale)), a.inv_t, M, S);
     leave<T>(a, sh, row, have, M, S);
 }
 
@@ -736,9 +746,8 @@ join_parts_kernel(RowArgs a, const u64* keys, const Part* parts) {
         float wm = m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(~0u, wm, o));
-        s = m > PCX_NEG_INF && wm < CUDART_INF_F ? s * exp((double)(m - wm) * a.inv_t) : 0.0;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+        s = m > PCX_NEG_INF && wm < CUDART_INF_F ? s * exp(((double)m - (double)wm) * a.inv_t) : 0.0;
+        s = warp_sum(s);
         m = wm;
     }
     for (int i = tid; i < a.splits * a.n; i += kThreads)
@@ -768,55 +777,99 @@ struct BeamArgs {
 };
 
 constexpr int kBeamTile = 2048;                     // candidates looked at together
+constexpr int kBehind = 4;                         // continuations that are kept behind the n best
 struct BeamShared {
     u64 score[kBeamTile + kMaxTop];
     uint32_t place[kBeamTile + kMaxTop];            // beam * vocab + token: a lower one first among equal scores
-    u64 list_s[kMaxTop + 1];
-    uint32_t list_p[kMaxTop + 1];
+    u64 list_s[kMaxTop + kBehind];
+    uint32_t list_p[kMaxTop + kBehind];
     double norm[kMaxTop], red[kWarps];              // what a beam's logits are lowered by
     float own[kMaxTop];                             // its score
     uint8_t exact[kMaxTop], doubt[kMaxTop];
+    int any_doubt;                                  // (the first CTA's word to the others of its cluster)
     uint32_t low[kWarps], high[kWarps];
     int count;
 };
 
-// log sum exp of a row in 64 bits, from its maximum.  The order of the sum goes by the places alone: equal rows, wherever they
-// lie, have equal bits.
-template <typename T>
-__device__ __noinline__ double exact_norm(const T* x, int vocab, float m, double* red) {
+// Part `seg` of kSegments of sum exp(x - m) over a row, in 64 bits, to thread 0.  The order of the sum goes by the places alone: equal
+// rows, wherever they lie, have equal bits.
+constexpr int kSegments = 8;
+template <int PER_SM, typename T>
+__device__ __noinline__ double segment_sum(const T* x, int vocab, int seg, float m, double* red) {
     constexpr int AHEAD = 8;
+    constexpr int64_t STEP = kSegments * kThreads;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     double s = 0.0;
-    for (int64_t e0 = threadIdx.x; e0 < vocab; e0 += kThreads * AHEAD) {
-        float f[AHEAD];
+    float next[AHEAD];
+    int64_t e0 = (int64_t)seg * kThreads + threadIdx.x;
+    auto fetch = [&]() {                            // (NaN counts nothing)
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) f[i] = e0 + i * kThreads < vocab ? (float)x[e0 + i * kThreads] : PCX_NEG_INF;
+        for (int i = 0; i < AHEAD; ++i) next[i] = fmaxf(e0 + i * STEP < vocab ? (float)x[e0 + i * STEP] : PCX_NEG_INF, PCX_NEG_INF);
+        e0 += AHEAD * STEP;
+    };
+    fetch();
+    for (int64_t left = (int64_t)vocab - seg * kThreads; left > 0; left -= AHEAD * STEP) {
+        double t[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-            if (f[i] > PCX_NEG_INF) s += exp((double)f[i] - (double)m);      // (not NaN)
+        for (int i = 0; i < AHEAD; ++i) t[i] = (double)next[i] - (double)m;
+        fetch();
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) t[i] = exp(t[i]);
+#pragma unroll
+        for (int o = 1; o < AHEAD; o *= 2)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i += 2 * o) t[i] += t[i + o];
+        s += t[0];
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    s = warp_sum(s);
     __syncthreads();
     if (lane == 0) red[warp] = s;
     __syncthreads();
     s = 0.0;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) s += red[w];
-    return log_norm(m, s, 1.0);
+    return s;
 }
 
-// One CTA per sequence; 64 sequences of 16 lists of 32: 8 us, in which 512 candidates are bisected down to at most 64 before
+// One CTA per sequence; 64 sequences of 16 lists of 32: 10 us, in which 512 candidates are bisected down to at most 64 before
 // they are ranked (ranking them all: 65 us).
 // The normalisers of the rows carry the error of their fp32 terms.  Where that leaves two continuations of different beams in
 // doubt, among the n best or at their end, those beams' normalisers are taken again in 64 bits and the choice is made again.  Once is
-// enough: a score moves by half the slack at most, so that only pairs within the slack can change places.
-__global__ void __launch_bounds__(kThreads)
+// enough: a score moves by half the slack at most, so that only pairs within the slack can change places.  Few sequences have
+// clusters of CTAs that share these sums; the first CTA does all the rest, for which the others wait.  64 sequences of 16 beams over
+// 32768 tokens, a call: 43 us, 57 with two beams in doubt (one call in twelve of random rows), 155 with all (350 by one CTA a
+// sequence).  What bounds the sums are fp64 instructions; with PER_SM = 2 they have the registers for eight exponentials at a time.
+template <int PER_SM>
+__global__ void __launch_bounds__(kThreads, PER_SM)
 join_beams_kernel(BeamArgs a) {
     __shared__ BeamShared sh;
-    const int tid = threadIdx.x;
-    const int64_t first = (int64_t)blockIdx.x * a.beams;
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, ctas = cluster.num_blocks(), rank = cluster.block_rank();
+    const int64_t sequence = blockIdx.x / ctas, first = sequence * a.beams;
+    cluster.sync();                                 // (all CTAs have started: their shared memory may be written)
     after_previous();
+    // the sums in doubt: kSegments for every beam, in the first CTA's `score`
+    auto take_sums = [&]() {
+        double* sums = (double*)cluster.map_shared_rank(sh.score, 0);
+        for (int b = 0; b < a.beams; ++b) {
+            if (!sh.doubt[b]) continue;
+            const char* row = (const char*)a.logits + (sequence * a.stride_batch + b * a.stride_beam) * (a.dtype == 0 ? 4 : 2);
+            const float m = a.parts[first + b].m;
+            for (int seg = rank; seg < kSegments; seg += ctas) {
+                const double s = a.dtype == 0 ? segment_sum<PER_SM>((const float*)row, a.vocab, seg, m, sh.red)
+                    : a.dtype == 1 ? segment_sum<PER_SM>((const __nv_bfloat16*)row, a.vocab, seg, m, sh.red)
+                                   : segment_sum<PER_SM>((const __half*)row, a.vocab, seg, m, sh.red);
+                if (tid == 0) sums[b * kSegments + seg] = s;
+            }
+        }
+        cluster.sync();
+    };
+    if (rank > 0) {
+        cluster.sync();                             // (the first CTA says what is in doubt)
+        if (sh.any_doubt) take_sums();
+        return;
+    }
     for (int b = tid; b < a.beams; b += kThreads) {
         const Part p = a.parts[first + b];
         const bool done = a.finished != nullptr && a.finished[first + b] != 0;
@@ -836,7 +889,18 @@ join_beams_kernel(BeamArgs a) {
         return ((double)sh.own[b] + (double)value_of(k)) - sh.norm[b];
     };
     auto is_finished = [&](int b) { return a.finished != nullptr && a.finished[first + b] != 0 && sh.own[b] > PCX_NEG_INF; };
-    int have = 0;                                   // (one entry more than asked for: the best that is left out)
+    // to the other CTAs, which wait for it at a barrier
+    auto tell = [&](int doubt) {
+        for (int r = 1; r < ctas; ++r) {
+            BeamShared* other = cluster.map_shared_rank(&sh, r);
+            if (tid == 0) other->any_doubt = doubt;
+            if (doubt)
+                for (int b = tid; b < a.beams; b += kThreads) other->doubt[b] = sh.doubt[b];
+        }
+    };
+    bool any = false;                               // normalisers are taken again
+    const int kept = a.n + kBehind;
+    int have = 0;
     for (bool again = false;; again = true) {
         if (tid == 0) sh.count = 0;
         __syncthreads();
@@ -863,7 +927,7 @@ join_beams_kernel(BeamArgs a) {
             if (total > few) {
                 u64 t, most;
                 key_range(sh.score, total, sh.low, sh.high, t, most);
-                t = bisect(total, a.n + 1, few, t, most, [&](int i, u64 mid) { return sh.score[i] >= mid; });
+                t = bisect(total, kept, few, t, most, [&](int i, u64 mid) { return sh.score[i] >= mid; });
                 __syncthreads();
                 if (tid == 0) sh.count = 0;
                 for (int i0 = 0; i0 < total; i0 += kThreads) {
@@ -888,52 +952,64 @@ join_beams_kernel(BeamArgs a) {
                     const u64 o = sh.score[j];
                     rank += (int)(o > s) | ((int)(o == s) & (int)(sh.place[j] < p));
                 }
-                if (rank <= a.n) { sh.list_s[rank] = s; sh.list_p[rank] = p; }
+                if (rank < kept) { sh.list_s[rank] = s; sh.list_p[rank] = p; }
             }
             __syncthreads();
-            have = min(total, a.n + 1);
+            have = min(total, kept);
             for (int i = tid; i < have; i += kThreads) { sh.score[i] = sh.list_s[i]; sh.place[i] = sh.list_p[i]; }
             if (tid == 0) sh.count = have;
             __syncthreads();
         }
         if (again || a.beams == 1 || !a.normalize) break;
-        // neighbours of different beams, or at the end of the n best, within the slack
-        bool close = false;
-        for (int i = tid; i + 1 < have; i += kThreads) {
-            const int b = sh.place[i] / (uint32_t)a.vocab, c = sh.place[i + 1] / (uint32_t)a.vocab;
-            close |= unordered(sh.score[i]) - unordered(sh.score[i + 1]) <= a.slack &&
-                     (i + 1 == a.n || (b != c && !(sh.exact[b] && sh.exact[c])));
-        }
-        if (!__syncthreads_or(close)) break;
-        // every pair of one of the n best and any continuation within the slack
-        const int chosen = min(have, a.n);
-        const double least = have > a.n ? unordered(sh.score[a.n - 1]) - a.slack : -CUDART_INF;
-        auto against = [&](double score, int b) {
-            for (int i = 0; i < chosen; ++i) {
-                const int c = sh.place[i] / (uint32_t)a.vocab;
-                if (c != b && fabs(score - unordered(sh.score[i])) <= a.slack) sh.doubt[b] = sh.doubt[c] = 1;
+        // pairs of one of the n best and any continuation behind it within the slack
+        bool more = false;                          // they reach beyond what is kept
+        for (int i = tid; i < min(have, a.n); i += kThreads) {
+            const double score = unordered(sh.score[i]);
+            int j = i + 1;
+            for (; j < have && score - unordered(sh.score[j]) <= a.slack; ++j) {
+                const int b = sh.place[i] / (uint32_t)a.vocab, c = sh.place[j] / (uint32_t)a.vocab;
+                if (b != c) sh.doubt[b] = sh.doubt[c] = 1;
             }
-        };
-        for (int b = tid; b < a.beams; b += kThreads)
-            if (is_finished(b)) against((double)sh.own[b], b);
-        for (int i = tid; i < slots; i += kThreads) {
-            uint32_t place;
-            const double score = candidate(i, place);
-            if (score > -CUDART_INF && score >= least) against(score, i / a.n);
+            more |= j == kept;
+        }
+        if (__syncthreads_or(more)) {               // (rows of equal logits)
+            const double least = unordered(sh.score[a.n - 1]) - a.slack;
+            auto against = [&](double score, int b) {
+                for (int i = 0; i < a.n; ++i) {
+                    const int c = sh.place[i] / (uint32_t)a.vocab;
+                    if (c != b && fabs(score - unordered(sh.score[i])) <= a.slack) sh.doubt[b] = sh.doubt[c] = 1;
+                }
+            };
+            for (int b = tid; b < a.beams; b += kThreads)
+                if (is_finished(b)) against((double)sh.own[b], b);
+            for (int i = tid; i < slots; i += kThreads) {
+                uint32_t place;
+                const double score = candidate(i, place);
+                if (score >= least) against(score, i / a.n);
+            }
         }
         __syncthreads();
-        for (int b = 0; b < a.beams; ++b) {
-            if (!sh.doubt[b] || sh.exact[b]) continue;
-            const char* row = (const char*)a.logits + (blockIdx.x * a.stride_batch + b * a.stride_beam) * (a.dtype == 0 ? 4 : 2);
-            const float m = a.parts[first + b].m;
-            const double norm = a.dtype == 0 ? exact_norm((const float*)row, a.vocab, m, sh.red)
-                : a.dtype == 1 ? exact_norm((const __nv_bfloat16*)row, a.vocab, m, sh.red) : exact_norm((const __half*)row, a.vocab, m, sh.red);
-            if (tid == 0) sh.norm[b] = norm;
-        }
+        any = __syncthreads_or(tid < a.beams && sh.doubt[tid] && !sh.exact[tid]);
+        if (!any) break;
+        for (int b = tid; b < a.beams; b += kThreads) sh.doubt[b] = sh.doubt[b] && !sh.exact[b];
+        __syncthreads();
+        tell(1);
+        cluster.sync();
+        take_sums();
+        for (int b = tid; b < a.beams; b += kThreads)
+            if (sh.doubt[b]) {
+                double s = 0.0;
+                for (int i = 0; i < kSegments; ++i) s += ((const double*)sh.score)[b * kSegments + i];
+                sh.norm[b] = log_norm(a.parts[first + b].m, s, 1.0);
+            }
         __syncthreads();
     }
+    if (!any) {
+        tell(0);
+        cluster.sync();
+    }
     for (int i = tid; i < a.n; i += kThreads) {
-        const int64_t to = (int64_t)blockIdx.x * a.n + i;
+        const int64_t to = sequence * a.n + i;
         const bool is = i < have;
         const uint32_t p = is ? sh.place[i] : 0;
         a.tokens[to] = is ? (int64_t)(p % (uint32_t)a.vocab) : -1;
@@ -942,13 +1018,13 @@ join_beams_kernel(BeamArgs a) {
     }
 }
 
-// How far log_norm may be off, in steps of 2^-24 of the sum: an exponential of 2^-22 (4); its argument, rounded twice, whose distance
-// from the maximum is at most log2(vocab) + 2 bits on average under the weights (2 ln 2 each); the sums of a tile (34); for every
-// tile of a lane a sum, and a product with an exponential where the maximum rises (6), whose arguments add up to log2(vocab) bits
-// while anything is left of the sum; and as much where the lanes are joined.
+// How far a row's normaliser may be off (temperature 1), in steps of 2^-24 of its sum: an exponential of 2^-22 (4); its argument a, once
+// rounded itself and by 0.23 through the scale, ln 2 |a| each, where a is at most max(3/4 b, b - 4) of b = log2(vocab) on average
+// under the weights (their entropy, less what the largest term has for itself); 8 sums one after the other in a tile; for every
+// further tile of a lane a sum, a product and its exponential (6), for the first a sum; 2 for what is left.
 double norm_error(int vocab, int tiles) {
-    const double bits = std::log2((double)vocab) + 2.0;
-    return (4.0 + 34.0 + 6.0 * tiles + 12.0 + 4.0 * 0.7 * bits) * 5.9604644775390625e-8;
+    const double bits = std::log2((double)vocab);
+    return (4.0 + 0.7 * 1.23 * std::max(0.75 * bits, bits - 4.0) + 8.0 + 6.0 * (tiles - 1) + 3.0) * 5.9604644775390625e-8;
 }
 
 // ---- reordering of states --------------------------------------------------------------------------------------------
@@ -1024,12 +1100,14 @@ __global__ void __launch_bounds__(256) reorder_kernel(MoveArgs a) {
 // A kernel of `grid` blocks whose start overlaps the end of the one before it in the stream (it waits for that one's results
 // itself, after_previous).  64 sequences of 16 beams, three launches: 44.8 -> 42 us a call.
 template <typename... P, typename... A>
-cudaError_t launch_next(void (*kernel)(P...), unsigned grid, cudaStream_t stream, A... args) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
+cudaError_t launch_next(void (*kernel)(P...), unsigned grid, unsigned cluster, cudaStream_t stream, A... args) {
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kThreads); cfg.stream = stream; cfg.attrs = &attr; cfg.numAttrs = 1;
+    cfg.gridDim = dim3(grid); cfg.blockDim = dim3(kThreads); cfg.stream = stream; cfg.attrs = attr; cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
@@ -1071,7 +1149,7 @@ int select_rows(RowArgs a, void* scratch, int64_t rows, cudaStream_t stream) {
     PCX_LAUNCH_CHECK();
     a.keys = joined_keys;
     a.parts = joined_parts;
-    return (int)launch_next(join_parts_kernel<T>, (unsigned)rows, stream, a, keys, parts);
+    return (int)launch_next(join_parts_kernel<T>, (unsigned)rows, 1, stream, a, keys, parts);
 }
 int select_rows(const RowArgs& a, int dtype, void* scratch, int64_t rows, cudaStream_t stream) {
     switch (dtype) {
@@ -1117,8 +1195,8 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
     a.scale = 1.4426950408889634f;
     const int rc = select_rows(a, dtype, scratch, rows, (cudaStream_t)stream);
     if (rc != 0) return rc;
-    const int ve = dtype == 0 ? 4 : 8, part = vocab / std::max(splits, 1);
-    const int in_tile = ve * (splits == 0 ? 32 * kGroups : kThreads * block_groups(vocab, ve, splits));
+    const int ve = dtype == 0 ? 4 : 8, parts = std::max(splits, 1);
+    const int64_t in_tile = splits == 0 ? 32 * kGroups : kThreads * block_groups(vocab, ve, splits);
     BeamArgs j{};
     j.keys = (const u64*)((const char*)scratch + rows * std::max(splits, 1) * ((int64_t)n * 8 + (int64_t)sizeof(Part)));
     j.parts = (const Part*)(j.keys + rows * n);
@@ -1126,8 +1204,13 @@ int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* 
     j.out_scores = out_scores; j.tokens = tokens; j.parents = parents;
     j.logits = logits; j.stride_batch = stride_batch; j.stride_beam = stride_beam; j.dtype = dtype;
     j.beams = beams; j.n = n; j.vocab = vocab; j.pad_id = pad_id; j.normalize = normalize;
-    j.slack = 2.0 * norm_error(vocab, part / in_tile + 1);
-    return (int)launch_next(join_beams_kernel, (unsigned)batch, (cudaStream_t)stream, j);
+    j.slack = 2.0 * norm_error(vocab, (int)pcx_cdiv(pcx_cdiv(vocab / ve + 2, parts), in_tile));
+    // CTAs a sequence: they share the sums that are taken again, and only wait otherwise: two an SM at most.  Many sequences are done
+    // sooner where more CTAs fit an SM (512 of 8 beams over 4096 tokens: 26.8 us a call against 29.4)
+    unsigned ctas = 1;
+    while (ctas < kSegments && normalize && beams > 1 && batch * ctas * 2 <= 148 * 2) ctas *= 2;
+    if (ctas == 1) return (int)launch_next(join_beams_kernel<4>, (unsigned)batch, 1, (cudaStream_t)stream, j);
+    return (int)launch_next(join_beams_kernel<2>, (unsigned)batch * ctas, ctas, (cudaStream_t)stream, j);
 }
 
 // `states`: n_tensors times (source, destination, outer rows, bytes per beam, source strides in bytes of outer rows and
