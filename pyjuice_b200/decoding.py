@@ -183,8 +183,15 @@ class HMMDecoder:
             return state.clone()
         if log_probs is not None:
             state = state - log_probs.nan_to_num(0.0, neginf=0.0)
-        tokens = tokens.long()
-        x = torch.stack([torch.zeros_like(tokens), tokens.clamp(-1, self.vocab).remainder_(self.vocab + 2)], 1)
+        return self._advance(state, self._categories(tokens.long()))
+
+    def _categories(self, tokens: torch.Tensor) -> torch.Tensor:
+        """What `_advance` takes: the vocabulary's tokens as they are, then one that it does not have, one that is not known."""
+        return tokens.clamp(-1, self.vocab).remainder_(self.vocab + 2)
+
+    def _advance(self, state: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
+        N = state.size(1)
+        x = torch.stack([torch.zeros_like(tokens), tokens], 1)
         return self._step._values_of_inner([(self._state_ns, state)], N, x)[:self.num_latents, :N].clone()
 
 
@@ -212,10 +219,11 @@ def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1,
     prompts = prompts.to(device)
     B, K = prompts.size(0), num_beams
     state = decoder.start(B)
-    for t in range(prompts.size(1)):
-        said = prompts[:, t].long()
-        heard = decoder._next(state).gather(1, said.clamp(0, V - 1)[:, None])[:, 0]
-        state = decoder.advance(state, said, heard.masked_fill_(said < 0, 0.0))
+    prompts = prompts.long()
+    said, at, unknown = decoder._categories(prompts), prompts.clamp(0, V - 1), prompts < 0
+    for t in range(prompts.size(1) if B > 0 else 0):
+        heard = decoder._next(state).gather(1, at[:, t:t + 1])[:, 0]
+        state = decoder._advance(state - heard.masked_fill_(unknown[:, t], 0.0).nan_to_num_(0.0, neginf=0.0), said[:, t])
     scores = torch.zeros(B, 1, device=device)
     finished = torch.zeros(B, 1, dtype=torch.bool, device=device)
     tokens = torch.empty(B, 0, dtype=torch.int64, device=device)
@@ -233,8 +241,8 @@ def beam_search(pc, prompts: Optional[torch.Tensor] = None, num_tokens: int = 1,
             finished = finished.view(B, n) | (said == eos_id)
         else:
             finished = finished.view(B, n)
-        if t + 1 < num_tokens:
-            state = decoder.advance(state, said.reshape(-1).clamp_min(0), picked.reshape(-1))
+        if t + 1 < num_tokens and B > 0:
+            state = decoder._advance(state - picked.reshape(-1), said.reshape(-1).clamp_min(0))        # (of dead beams: anything)
     if scores.size(1) < K:
         scores = torch.nn.functional.pad(scores, (0, K - scores.size(1)), value=float("-inf"))
         tokens = torch.nn.functional.pad(tokens, (0, 0, 0, K - tokens.size(1)), value=-1)

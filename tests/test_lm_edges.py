@@ -349,3 +349,16 @@ def test_decoders_of_any_number_of_states(latents, vocab):
     assert torch.equal(decoder.log_probs(state), before)
     tokens, scores = beam_search(decoder, said, 2, 3)
     assert tokens.shape == (3, 3, 2) and bool(scores[:, :min(3, vocab)].isfinite().all())
+
+
+@pytest.mark.gpu
+def test_no_sequences_and_no_prompts():
+    from pyjuice_b200.decoding import HMMDecoder, beam_search
+    decoder = HMMDecoder(hmm(20, 33)[0])
+    for prompts in (torch.empty(0, 4, dtype=torch.int64), None):
+        tokens, scores = beam_search(decoder, prompts, 3, 5, batch=0)
+        assert tokens.shape == (0, 5, 3) and scores.shape == (0, 5)
+    a, b = beam_search(decoder, torch.empty(2, 0, dtype=torch.int32), 3, 5), beam_search(decoder, None, 3, 5, batch=2)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert decoder.advance(decoder.start(0), torch.empty(0, dtype=torch.int64, device="cuda")).shape == (20, 0)
+    assert decoder.log_probs(decoder.start(0)).shape == (0, 33)
