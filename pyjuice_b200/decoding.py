@@ -54,7 +54,7 @@ class HMMDecoder:
     """Next-token distributions of a compiled homogeneous HMM, for any number of beams.
 
     The parameters are taken over when the decoder is made and on ``reload()``; training the circuit later does not change
-    it.  A state is a ``[num_latents, N]`` tensor: column n holds the logarithm of the distribution of beam n's next hidden
+    it.  The arithmetic is the circuit's present ``sum_mode``.  A state is a ``[num_latents, N]`` tensor: column n holds the logarithm of the distribution of beam n's next hidden
     state given its tokens, up to a constant, which ``log_probs`` takes out.  As in every circuit, a sum is at least 1e-24 of its
     largest term: what has a probability of zero beside others that have not has that one."""
 
@@ -87,7 +87,6 @@ class HMMDecoder:
         self._step = compile(self._step_ns, verbose=False).to(self.device)
         for small in (self._speak, self._step):
             small.use_cuda_graphs = False            # a decoding loop may be captured as a whole
-            small.sum_mode = pc.sum_mode
         self.reload()
 
     @staticmethod
@@ -163,6 +162,7 @@ class HMMDecoder:
         N = state.size(1)
         if N == 0:
             return torch.empty(0, self.vocab, device=self.device)
+        self._speak.sum_mode = self.pc.sum_mode
         rows = self._speak._values_of_inner([(self._heard_ns, state)], N)
         W = rows.size(1)
         out = torch.empty(W, self._v_pad, device=self.device)
@@ -192,6 +192,7 @@ class HMMDecoder:
     def _advance(self, state: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
         N = state.size(1)
         x = torch.stack([torch.zeros_like(tokens), tokens], 1)
+        self._step.sum_mode = self.pc.sum_mode
         return self._step._values_of_inner([(self._state_ns, state)], N, x)[:self.num_latents, :N].clone()
 
 

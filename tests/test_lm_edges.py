@@ -362,3 +362,26 @@ def test_no_sequences_and_no_prompts():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     assert decoder.advance(decoder.start(0), torch.empty(0, dtype=torch.int64, device="cuda")).shape == (20, 0)
     assert decoder.log_probs(decoder.start(0)).shape == (0, 33)
+
+
+@pytest.mark.gpu
+def test_a_decoder_follows_its_circuits_arithmetic():
+    from pyjuice_b200.decoding import HMMDecoder
+    pc, _ = hmm(256, 1024)
+    x = torch.randint(1024, (32, 2), generator=torch.Generator().manual_seed(0)).cuda()
+
+    def answers(decoder):
+        state = decoder.start(32)
+        for t in range(2):
+            state = decoder.advance(state, x[:, t])
+        return decoder.log_probs(state)
+
+    decoder = HMMDecoder(pc)
+    seen = {}
+    for mode in (None, 0, 2, 1, 0, None):
+        pc.sum_mode = mode
+        got = answers(decoder)
+        assert torch.equal(got, answers(HMMDecoder(pc)))
+        assert mode not in seen or torch.equal(got, seen[mode])
+        seen[mode] = got
+    assert not torch.equal(seen[0], seen[2]) and torch.equal(seen[1], seen[None])
