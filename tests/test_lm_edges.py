@@ -385,3 +385,54 @@ def test_a_decoder_follows_its_circuits_arithmetic():
         assert mode not in seen or torch.equal(got, seen[mode])
         seen[mode] = got
     assert not torch.equal(seen[0], seen[2]) and torch.equal(seen[1], seen[None])
+
+
+def rows_of_all_kinds(vocab, dtype, seed=0):
+    """[9, vocab] at an odd place of a wider tensor."""
+    g = torch.Generator().manual_seed(seed)
+    at = torch.arange(vocab, dtype=torch.float32)
+    noise = torch.randn(vocab, generator=g)
+    rows = [noise * 3, torch.full((vocab,), -3.5), at / 512, -at / 512, torch.where(at % 977 == 5, noise, NEG_INF), at % 2,
+            torch.where(at % 3 == 0, NAN, noise), torch.where(at % 4001 == 7, noise, -1e9 if dtype != torch.float16 else -6e4),
+            torch.full((vocab,), torch.finfo(dtype).min)]
+    wide = torch.zeros(len(rows), vocab + 5)
+    wide[:, 3:3 + vocab] = torch.stack(rows)
+    return wide.to(dtype).cuda()[:, 3:3 + vocab]
+
+
+@pytest.fixture(params=[0, 1, 2, 7, 32], ids=lambda s: "a warp a row" if s == 0 else f"{s} parts")
+def cut(request, monkeypatch):
+    """Every row is walked in this form, whatever the rule for its size."""
+    splits = request.param
+    monkeypatch.setattr(lm, "_scratch", lambda rows, row_bytes, n, device:
+                        (torch.empty(rows * (max(splits, 1) + 1) * (8 * n + 16), dtype=torch.uint8, device=device), splits))
+    return splits
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,dtype", [(32769, torch.bfloat16), (100003, torch.bfloat16), (40001, torch.float16), (16385, torch.float32),
+                                         (50257, torch.float32), (16384, torch.float32), (77, torch.float32)])
+def test_every_form_at_every_cut(vocab, dtype, cut):
+    """A warp a row over one, two and four chunks of its tiles, CTAs a row with and without parts (more of them than the row has groups
+    too): the same entries."""
+    x = rows_of_all_kinds(vocab, dtype)
+    values = x.double().cpu()
+    values = torch.where(values.isnan(), NEG_INF, values)
+    want, ids = values.sort(dim=1, descending=True, stable=True)
+    norms = [exact_norm(row) for row in values.tolist()]
+    for k in (1, 40, min(128, vocab)):
+        got = lm.top_logits(x, k)
+        assert torch.equal(got.logits.double().cpu(), want[:, :k])
+        assert torch.equal(got.ids.cpu(), torch.where(want[:, :k] == NEG_INF, -1, ids[:, :k]))
+        for a, b in zip(got.log_norm.double().cpu().tolist(), norms):
+            assert a == b or abs(a - b) <= norm_tol(vocab) + abs(b) * STEP
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,dtype", [(33001, torch.bfloat16), (40001, torch.float32)])
+def test_beams_in_every_form(vocab, dtype, cut):
+    x = rows_of_all_kinds(vocab, dtype)
+    beams = torch.stack([x[[0, 2, 6]], x[[4, 7, 4]], x[[8, 1, 5]]])
+    scores = torch.tensor([[-1.0, -3.0, -1.5], [-2.0, -2.0, -2.0], [-1.0, -1.0, -1.0]]).cuda()
+    for n in (1, 9, 128):
+        check_best(beams, scores, n)
