@@ -436,3 +436,24 @@ def test_beams_in_every_form(vocab, dtype, cut):
     scores = torch.tensor([[-1.0, -3.0, -1.5], [-2.0, -2.0, -2.0], [-1.0, -1.0, -1.0]]).cuda()
     for n in (1, 9, 128):
         check_best(beams, scores, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eos", [None, 3])
+def test_a_captured_search_replays_on_other_prompts(eos):
+    from pyjuice_b200.decoding import HMMDecoder, beam_search
+    decoder = HMMDecoder(hmm(64, 700)[0])
+    g = torch.Generator().manual_seed(0)
+    prompts = torch.randint(700, (5, 3), generator=g).cuda()
+    for _ in range(2):
+        beam_search(decoder, prompts, 4, 6, eos_id=eos)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = beam_search(decoder, prompts, 4, 6, eos_id=eos)
+    for _ in range(3):
+        prompts.copy_(torch.randint(-1, 700, (5, 3), generator=g))
+        graph.replay()
+        got = [t.clone() for t in held]
+        for a, b in zip(got, beam_search(decoder, prompts, 4, 6, eos_id=eos)):
+            assert torch.equal(a, b)
