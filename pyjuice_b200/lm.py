@@ -31,7 +31,8 @@ class TopLogits(NamedTuple):
     logits float32, bfloat16 or float16.  A slot is empty when its id is negative or its logit is -inf or NaN.  The weight
     of a slot is ``exp(logits / temperature - log_norm)``; without ``log_norm`` (the shape of ``ids`` less its last
     dimension), or where it is not finite, the weights of a position's slots sum to one.  A position whose slots are all
-    empty says nothing: it is marginalised.  Logits of +inf share the whole weight of their position, with or without ``log_norm``."""
+    empty says nothing: it is marginalised.  Logits of +inf share the whole weight of their position, with or without ``log_norm``.
+    (A normaliser of 32 bits is exact to 2^-24 of its size: where logits go into the thousands, the weights' last digits go with it.)"""
     ids: torch.Tensor
     logits: torch.Tensor
     temperature: float = 1.0
@@ -251,8 +252,10 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
     Empty slots add nothing, whatever they hold; a weight of zero takes nothing of a log-probability of -inf; an id of C
     or more has the log-probability -inf.  Returns float32 ``[T, M, B]``.  The gradient goes to ``log_probs`` (sums in a
     fixed order: the same bits on every call), none to the teacher; second and forward-mode derivatives are refused.  Up
-    to a million categories.  A backward pass captured into a CUDA graph needs, as torch's own do, that no eager graph of the
-    same leaf is alive while it is captured."""
+    to a million categories, 2^30 slots that share a table, 2^31 nodes over all positions.  A backward pass captured into a CUDA
+    graph needs, as torch's own do, that no eager graph of the same leaf is alive while it is captured.
+
+    Where a table's slots name a quarter of its categories or more, the call makes a turned copy of the tables, as large as they are."""
     teacher._check()
     if log_probs.dtype != torch.float32 or log_probs.dim() not in (2, 3):
         raise TypeError("log_probs must be float32 [M, C] or [T, M, C]")
@@ -265,8 +268,8 @@ def expected_log_probs(log_probs: torch.Tensor, teacher: TopLogits) -> torch.Ten
         raise ValueError("tables of 1 to 1000000 categories are supported")
     if max(B * K, 1) * (T if log_probs.dim() == 2 else 1) >= 2 ** 30:
         raise ValueError("more than 2^30 slots share a table")
-    if T * log_probs.size(-2) >= 2 ** 31:
-        raise ValueError("more than 2^31 nodes over all positions")
+    if T * log_probs.size(-2) >= 2 ** 31 or log_probs.size(-2) > 2 ** 30 - 4:         # (rows of flows are addressed with 32 bits)
+        raise ValueError("more than 2^31 nodes over all positions, or 2^30 of one")
     _refuse_tangents("expected_log_probs", log_probs)
     _require_cuda(log_probs, teacher.ids, teacher.logits, teacher.log_norm)
     if log_probs.requires_grad and torch.is_grad_enabled():

@@ -457,3 +457,11 @@ def test_a_captured_search_replays_on_other_prompts(eos):
         got = [t.clone() for t in held]
         for a, b in zip(got, beam_search(decoder, prompts, 4, 6, eos_id=eos)):
             assert torch.equal(a, b)
+
+
+def test_tables_of_more_nodes_than_are_addressed_are_refused():
+    teacher = lambda T: lm.TopLogits(torch.zeros(2, T, 1, dtype=torch.int64), torch.zeros(2, T, 1))
+    for shape, T in (((2 ** 30 - 3, 1), 1), ((1, 2 ** 30, 1), 1), ((2 ** 30 - 4, 1), 3), ((2, 2 ** 30 - 4, 1), 2)):
+        fits = T * shape[-2] < 2 ** 31 and shape[-2] <= 2 ** 30 - 4
+        with pytest.raises(NotImplementedError if fits else ValueError):
+            lm.expected_log_probs(torch.zeros(1, 1).expand(shape), teacher(T))
