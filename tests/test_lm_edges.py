@@ -465,3 +465,26 @@ def test_tables_of_more_nodes_than_are_addressed_are_refused():
         fits = T * shape[-2] < 2 ** 31 and shape[-2] <= 2 ** 30 - 4
         with pytest.raises(NotImplementedError if fits else ValueError):
             lm.expected_log_probs(torch.zeros(1, 1).expand(shape), teacher(T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tied", [True, False])
+@pytest.mark.parametrize("T,M,C,B,K", [(2, 6, 200000, 2600, 2), (2, 40, 200000, 3000, 2), (3, 70, 900, 500, 4), (2, 300, 64, 700, 3), (1, 3, 5, 50, 2)])
+def test_a_category_that_has_half_of_all_slots(T, M, C, B, K, tied):
+    """Both forms of the backward pass: only categories that occur (few slots in large tables), tiles of categories."""
+    g = torch.Generator().manual_seed(T + C)
+    ids = torch.randint(C, (B, T, K), generator=g)
+    ids[torch.rand(B, T, K, generator=g) < 0.5] = C // 3
+    lp = torch.randn(*((M, C) if tied else (T, M, C)), generator=g).cuda().requires_grad_()
+    out = lm.expected_log_probs(lp, lm.TopLogits(ids.cuda(), torch.zeros(B, T, K, device="cuda")))
+    # (weights 1 / K; sums of small whole numbers over it: K a power of two or not, every sum is off by its terms' roundings at most)
+    flow = torch.randint(0, 3, out.shape, generator=g).float().cuda()
+    grad, = torch.autograd.grad(out, lp, flow)
+    want = torch.zeros(T, C, M, dtype=torch.float64)
+    q = float(torch.tensor(1.0) / K)
+    for t in range(T):
+        for k in range(K):
+            want[t].index_add_(0, ids[:, t, k], flow[t].t().double().cpu() * q)
+    want = want.sum(0).t() if tied else want.transpose(1, 2)
+    terms = B * K * (T if tied else 1)
+    assert bool(((grad.double().cpu() - want).abs() <= (terms * STEP) * want).all())
