@@ -581,7 +581,8 @@ int pcx_colplan_blob_free(void* blob);
 int pcx_top_logits(int64_t* ids, void* values, float* norms, void* scratch, const void* logits, int dtype, int64_t rows,
                    int vocab, int64_t row_stride, int n, int splits, double temperature, void* stream);
 /* The n best of scores[b][k] + logits[b][k][v] - (normalize ? log sum_v exp(logits[b][k][v]) : 0) over k and v, compared in 64
- * bits, a lower k * vocab + v first among equals.  Beams whose score is -inf or NaN are dead; a beam flagged in `finished`
+ * bits, a lower k * vocab + v first among equals (equal rows at equal scores are equals, wherever they lie; a row whose fp32
+ * normaliser leaves the order in doubt is read once more).  Beams whose score is -inf or NaN are dead; a beam flagged in `finished`
  * (null = none) has one candidate, pad_id at its own score.  Missing entries: score -inf, parent 0, token -1.
  * beams <= 128, beams * vocab < 2^31. */
 int pcx_beam_select(float* out_scores, int64_t* parents, int64_t* tokens, void* scratch, const void* logits, int dtype,

@@ -10,7 +10,7 @@
 //   CTAs a row     The CTA keeps the n largest so far; rows are cut into parts until the device is full, and a second kernel
 //                  joins their lists, one CTA per row.
 // For beams another kernel joins the rows of a sequence and adds the scores, in 64 bits: a sum of a score and a logit is
-// rounded only in the returned score, never before it is compared.
+// rounded only in the returned score, never before it is compared, and normalisers that leave the order in doubt are taken again.
 #include "pcx_common.cuh"
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -584,8 +584,8 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
 // Few rows: a CTA a row or part of one, tiles of G groups of 16 bytes a thread (8; 2 for parts too short for that).  The CTA
 // keeps the n largest logits so far, sorted; the last of them is a bound that few later logits pass, so that a tile costs a
 // comparison a thread and a barrier.  The first tile's bound comes from its threads' maxima.  1024 rows of 32768 bf16, n = 32:
-// 36 us (1.9 TB/s); 1001 rows of 50257 fp32, n = 100: 107 us (1.9 TB/s), of which the walk is 41: what bounds it are the
-// barriers and the ranking of a tile's candidates.  (8192 rows with tiles of 4, 8 and 16 groups: 271, 235, 250 us.)
+// 36 us a call (1.9 TB/s); 1001 rows of 50257 fp32, n = 100: 107 us (1.9 TB/s), of which the walk is 41: what bounds it are the
+// barriers and the ranking of a tile's candidates, after nearly every tile (up to seven a row here).  (8192 rows with tiles of 4, 8 and 16 groups: 271, 235, 250 us.)
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, G > 4 ? 3 : 4)
 top_rows_block_kernel(RowArgs a) {

@@ -285,9 +285,12 @@ def _sm_count(index: int) -> int:
 def _scratch(rows: int, row_bytes: int, n: int, device) -> Tuple[torch.Tensor, int]:
     """Workspace of a selection, and how its rows are walked: 0 for a warp a row, else the parts that a row is cut into.
 
-    A warp a row keeps sixteen rows in flight per SM, without barriers (8192 rows of 64 KB: 188 us against 235 for a CTA a
-    row; 1024 rows, not half of what the device holds: 41 both), and costs short rows no idle threads.  Fewer and longer
-    rows go to CTAs, four per SM if the rows give as many parts of 8 KB."""
+    A warp a row keeps sixteen rows in flight per SM, without barriers, and costs short rows no idle threads.  Fewer and longer
+    rows go to CTAs, four per SM if the rows give as many parts of 8 KB.  Calls of a warp a row against a CTA a row, us: 8192 rows of
+    64 KB bf16, n = 32: 190, 231; 1024 of them: 36 both; 1776 of 16, 64, 196, 512 KB: n = 32: 30, 38; 56, 68; 144, 139; 298, 276;
+    n = 128: 122, 227; 109, 351; 254, 485; 450, 687; the same in fp32: n = 32: 18, 32; 33, 52; 90, 111; 183, 218.  Long lists of fewer
+    rows would be better off with a warp too, which the rule leaves out (1024 rows of 196 KB bf16, n = 128: 204, 308; 1001 of fp32, n =
+    100: 96, 107)."""
     sms = _sm_count(device.index)
     splits = 0 if rows >= sms * 12 or row_bytes <= 8192 else max(1, min(-(-sms * 4 // rows), -(-row_bytes // 8192), 32))
     return torch.empty(rows * (max(splits, 1) + 1) * (8 * n + 16), dtype=torch.uint8, device=device), splits
