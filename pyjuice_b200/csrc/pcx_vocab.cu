@@ -585,7 +585,8 @@ top_rows_warp_kernel(RowArgs a, int64_t n_rows) {
 // keeps the n largest logits so far, sorted; the last of them is a bound that few later logits pass, so that a tile costs a
 // comparison a thread and a barrier.  The first tile's bound comes from its threads' maxima.  1024 rows of 32768 bf16, n = 32:
 // 36 us a call (1.9 TB/s); 1001 rows of 50257 fp32, n = 100: 107 us (1.9 TB/s), of which the walk is 41: what bounds it are the
-// barriers and the ranking of a tile's candidates, after nearly every tile (up to seven a row here).  (8192 rows with tiles of 4, 8 and 16 groups: 271, 235, 250 us.)
+// barriers and the ranking of a tile's candidates, after nearly every tile (up to seven a row here).  (8192 rows with tiles of 4,
+// 8 and 16 groups: 271, 235, 250 us.)
 template <typename T, int G>
 __global__ void __launch_bounds__(kThreads, G > 4 ? 3 : 4)
 top_rows_block_kernel(RowArgs a) {
@@ -962,17 +963,20 @@ join_beams_kernel(BeamArgs a) {
         }
         if (again || a.beams == 1 || !a.normalize) break;
         // pairs of one of the n best and any continuation behind it within the slack
-        bool more = false;                          // they reach beyond what is kept
+        int seen = 0;                               // 1: such a pair; 2: they reach beyond what is kept
         for (int i = tid; i < min(have, a.n); i += kThreads) {
             const double score = unordered(sh.score[i]);
             int j = i + 1;
             for (; j < have && score - unordered(sh.score[j]) <= a.slack; ++j) {
                 const int b = sh.place[i] / (uint32_t)a.vocab, c = sh.place[j] / (uint32_t)a.vocab;
-                if (b != c) sh.doubt[b] = sh.doubt[c] = 1;
+                if (b == c) continue;
+                sh.doubt[b] = sh.doubt[c] = 1;
+                seen |= 1;
             }
-            more |= j == kept;
+            if (j == kept) seen |= 2;
         }
-        if (__syncthreads_or(more)) {               // (rows of equal logits)
+        if (!__syncthreads_or(seen)) break;
+        if (__syncthreads_or(seen & 2)) {           // (rows of equal logits)
             const double least = unordered(sh.score[a.n - 1]) - a.slack;
             auto against = [&](double score, int b) {
                 for (int i = 0; i < a.n; ++i) {

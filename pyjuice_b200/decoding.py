@@ -54,8 +54,11 @@ class HMMDecoder:
     """Next-token distributions of a compiled homogeneous HMM, for any number of beams.
 
     The parameters are taken over when the decoder is made and on ``reload()``; training the circuit later does not change
-    it.  The arithmetic is the circuit's present ``sum_mode``.  A state is a ``[num_latents, N]`` tensor: column n holds the logarithm of the distribution of beam n's next hidden
-    state given its tokens, up to a constant, which ``log_probs`` takes out.  As in every circuit, a sum is at least 1e-24 of its
+    it.  The arithmetic is the circuit's present ``sum_mode``.  A decoder serves one call at a time: all of them use its circuits'
+    buffers.
+
+    A state is a ``[num_latents, N]`` tensor: column n holds the logarithm of the distribution of beam n's next hidden state
+    given its tokens, up to a constant, which ``log_probs`` takes out.  As in every circuit, a sum is at least 1e-24 of its
     largest term: what has a probability of zero beside others that have not has that one."""
 
     def __init__(self, pc: TensorCircuit):
